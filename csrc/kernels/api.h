@@ -366,6 +366,44 @@ int embedding_index_block();
 // ids.
 cudaError_t launch_embedding_rows(const int* start, const long long* perm, const __nv_bfloat16* grad_out, __nv_bfloat16* grad_table, int V, int H, cudaStream_t stream);
 cudaError_t launch_embedding_few(const long long* ids, const __nv_bfloat16* grad_out, __nv_bfloat16* grad_table, int T, int V, int H, cudaStream_t stream);
+// ---------------------------------------------------------------------------------------------
+// the dense side of a block: row norm, balance loss (row_norm.cu, balance_loss.cu)
+// ---------------------------------------------------------------------------------------------
+// h = x + residual rounded to the rows' type (no residual: h = x), y = h / sqrt(mean(h^2) + eps) * weight, and y in e4m3 (see quantise_rows).
+constexpr int kRowNormMaxHidden = 48 * 1024;
+struct RowNormArgs {
+  const void* x;               // [T, H], rows x_stride elements apart
+  const void* residual;        // [T, H], rows residual_stride elements apart, or null
+  long long x_stride, residual_stride;
+  const void* weight;          // [H]
+  int T, H;
+  int rows_bf16, weight_bf16;  // else fp32
+  float eps;
+  void* h;                     // [T, H] out; used with residual
+  void* y;                     // [T, H] out
+  unsigned char* q;            // [T, H] out, or null; H % 128 == 0
+  float* scales;               // [T, H / 128] out, with q
+  float* rstd;                 // [T] out, or null
+  int warps_per_row;           // set by the launcher
+};
+cudaError_t launch_row_norm(const RowNormArgs& a, cudaStream_t stream);
+// Gradients: g = dy * weight, s = mean(g * h * rstd), dx = rstd * (g - h * rstd * s) + dh, dweight = sum over rows of dy * h * rstd.
+struct RowNormBwdArgs {
+  const void* h;               // [T, H], rows h_stride elements apart
+  long long h_stride;
+  const void* weight;          // [H]
+  const float* rstd;           // [T]
+  const void* dy;              // [T, H]
+  const void* dh;              // [T, H] or null
+  int T, H;
+  int rows_bf16, weight_bf16;
+  void* dx;                    // [T, H] out
+  void* dweight;               // [H] out, the weight's type
+  float* partials;             // [blocks][H] scratch
+  int warps_per_row;           // set by the launcher
+};
+int row_norm_bwd_blocks(const RowNormBwdArgs& a, int sms);
+cudaError_t launch_row_norm_bwd(const RowNormBwdArgs& a, int blocks, cudaStream_t stream);
 // AdamW on bf16 parameters with fp32 master weights and moments, several tensors per launch.
 struct AdamWTensor {
   __nv_bfloat16* param;

@@ -15,6 +15,7 @@
 
 #include "announce_blocks.h"
 #include "api.h"
+#include "e4m3_rows.cuh"
 #include "early_start.cuh"
 #include "route_splits.cuh"
 
@@ -57,9 +58,7 @@ constexpr int kMaxScaleGroups = 128;  // fp8 dispatch: rows of up to 128 x 128 =
 
 // 16 bf16 elements of a lane -> 16 e4m3 bytes; 8 consecutive lanes (128 elements) share one scale.
 // Every lane of the warp calls this together (lanes past the row's end pass zeros).
-// The scale is amax / 448 rounded UP to the next value a bf16 can hold: quantised values still fit
-// e4m3, and a receiver that multiplies in bf16 (the expert GEMM's converter warps) reproduces
-// value x scale without a second rounding. The abs / max run on bf16 pairs, the conversion on float pairs.
+// The scale is e4m3_scale's. The abs / max run on bf16 pairs, the conversion on float pairs.
 __device__ __forceinline__ uint4 quantise16(const uint4 (&raw)[2], float& sc) {
   const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw[0]);  // 8 pairs = my 16 elements
   __nv_bfloat162 m2 = __habs2(h[0]);
@@ -68,14 +67,14 @@ __device__ __forceinline__ uint4 quantise16(const uint4 (&raw)[2], float& sc) {
   float amax = fmaxf(__low2float(m2), __high2float(m2));
 #pragma unroll
   for (int o = 4; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  sc = __uint_as_float((__float_as_uint(fmaxf(amax, 1e-12f) * (1.0f / 448.0f)) + 0xFFFFu) & 0xFFFF0000u);
+  sc = e4m3_scale(amax);
   const float inv = 1.0f / sc;
   uint4 q;
   unsigned short* qs = reinterpret_cast<unsigned short*>(&q);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float2 f = __bfloat1622float2(h[i]);
-    qs[i] = __nv_cvt_float2_to_fp8x2(make_float2(f.x * inv, f.y * inv), __NV_SATFINITE, __NV_E4M3);
+    qs[i] = e4m3_pair(f.x, f.y, inv);
   }
   return q;
 }
@@ -88,12 +87,12 @@ __device__ __forceinline__ uint4 through_e4m3(const uint4& raw) {
   float amax = fmaxf(__low2float(m2), __high2float(m2));
 #pragma unroll
   for (int o = 8; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  const float sc = __uint_as_float((__float_as_uint(fmaxf(amax, 1e-12f) * (1.0f / 448.0f)) + 0xFFFFu) & 0xFFFF0000u), inv = 1.0f / sc;
+  const float sc = e4m3_scale(amax), inv = 1.0f / sc;
   float f[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 v = __bfloat1622float2(h[i]);
-    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(__nv_cvt_float2_to_fp8x2(make_float2(v.x * inv, v.y * inv), __NV_SATFINITE, __NV_E4M3), __NV_E4M3);
+    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(e4m3_pair(v.x, v.y, inv), __NV_E4M3);
     const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&r));
     f[2 * i] = d.x * sc;
     f[2 * i + 1] = d.y * sc;

@@ -174,6 +174,7 @@ bool a2a_launch_group(const A2AGroupPy& group, const std::vector<const A2AProgra
 }  // namespace
 
 void bind_moe(py::module_& m);  // defined in moe_bindings.cpp
+void bind_dense(py::module_& m);  // defined in dense_bindings.cpp
 
 PYBIND11_MODULE(_C, m) {
   m.doc() = "fast_b200 native runtime and sm_100a kernels";
@@ -235,4 +236,5 @@ PYBIND11_MODULE(_C, m) {
   });
   m.def("launch_count", &launch_count);
   bind_moe(m);
+  bind_dense(m);
 }

@@ -1,8 +1,12 @@
-"""Small fused autograd ops around the MoE block: embedding with a segmented-sum backward, and the
-mean-square loss of a residual sum computed without materialising fp32 copies."""
+"""Small fused autograd ops around the MoE block: embedding with a segmented-sum backward, the
+mean-square loss of a residual sum computed without materialising fp32 copies, and the dense side of a block (residual
+sum and RMS norm of rows)."""
 from __future__ import annotations
 
+from typing import NamedTuple, Optional
+
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import runtime
 
@@ -50,3 +54,55 @@ class _ResidualMeanSquare(torch.autograd.Function):
 def residual_mean_square(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
     """mean((a + b)^2) with the sum rounded to bf16, as a scalar fp32 tensor (bf16 inputs)."""
     return _ResidualMeanSquare.apply(a, b)
+
+
+class NormRows(NamedTuple):
+    """What ``add_rms_norm`` returns: the normalised rows ``y``, the sum ``h`` that was normalised (``x`` itself without a residual) and, if
+    asked for, ``y`` in e4m3: bytes ``q`` (uint8) and fp32 ``scales``, one per 128 columns."""
+
+    y: torch.Tensor
+    h: torch.Tensor
+    q: Optional[torch.Tensor]
+    scales: Optional[torch.Tensor]
+
+
+class _AddRMSNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps, quantise):
+        y, h, q, scales, rstd = runtime.ext().row_norm(x, weight, eps, residual, quantise, True)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x if h is None else h, weight, rstd)
+        if quantise:
+            ctx.mark_non_differentiable(q, scales)
+        return y, h, q, scales
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh, _dq, _dscales):
+        h, weight, rstd = ctx.saved_tensors
+        want_x, want_w, want_r = ctx.needs_input_grad[:3]
+        if dy is None:   # only the sum was used
+            dx, dw = dh, (torch.zeros_like(weight) if want_w else None)
+        else:
+            dx, dw = runtime.ext().row_norm_bwd(h, weight, rstd, dy, dh)
+        return dx if want_x else None, dw if want_w else None, dx if want_r else None, None, None
+
+
+def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residual: Optional[torch.Tensor] = None, quantise: bool = False) -> NormRows:
+    """RMS norm of rows, with the residual's addition in front of it and optionally an output in e4m3.
+
+    ``h = x + residual`` rounded to x's type; ``y = h / sqrt(mean(h^2) + eps) * weight`` over the last dimension, rounded once. x: bf16 or
+    fp32 [..., hidden], rows in any strides (16-byte aligned rows of whole 16-byte words are fastest); ``residual``: the same shape and type;
+    ``weight``: bf16 or fp32 [hidden]; hidden up to 49152. ``quantise`` (hidden a multiple of 128): ``y`` also as the e4m3 rows that the
+    fp8 dispatch would send for it (``dequantise_rows`` reads them back). Gradients flow through y and h, not through q and scales; the weight's
+    gradient is summed in a fixed order."""
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
+        y, h, q, scales = _AddRMSNorm.apply(x, weight, residual, eps, quantise)
+    else:
+        y, h, q, scales, _ = runtime.ext().row_norm(x, weight, eps, residual, quantise, False)
+    return NormRows(y, x if h is None else h, q, scales)
+
+
+def dequantise_rows(q: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """bf16 rows of e4m3 bytes (uint8 [..., hidden]) and fp32 scales [..., hidden / 128], as ``add_rms_norm`` makes them."""
+    return runtime.ext().dequantise_rows(q, scales)

@@ -1,0 +1,37 @@
+"""What the dense operators refuse, with the message that says why (no GPU: an argument is checked before anything runs)."""
+import pytest
+import torch
+
+from fast_b200.ops import fused
+
+BF = torch.bfloat16
+
+
+def test_row_norm_refuses_tensors_of_the_host():
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        fused.add_rms_norm(torch.zeros(2, 128, dtype=BF), torch.ones(128, dtype=BF))
+    with pytest.raises(RuntimeError, match="contiguous e4m3 bytes"):
+        fused.dequantise_rows(torch.zeros(2, 128, dtype=torch.uint8), torch.zeros(2, 1))
+
+
+@pytest.mark.gpu
+def test_row_norm_refusals():
+    x, w = torch.zeros(4, 200, device="cuda", dtype=BF), torch.ones(200, device="cuda", dtype=BF)
+    for bad, match in [
+        (lambda: fused.add_rms_norm(x.half(), w), "bf16 or fp32"),
+        (lambda: fused.add_rms_norm(x, w[:100].contiguous()), "weight"),
+        (lambda: fused.add_rms_norm(x, torch.ones(400, device="cuda", dtype=BF)[::2]), "weight"),
+        (lambda: fused.add_rms_norm(x, w.half()), "weight"),
+        (lambda: fused.add_rms_norm(x, w.cpu()), "weight"),
+        (lambda: fused.add_rms_norm(x, w, residual=x.float()), "residual"),
+        (lambda: fused.add_rms_norm(x, w, residual=x[:2]), "residual"),
+        (lambda: fused.add_rms_norm(x, w, residual=x[:1]), "residual"),
+        (lambda: fused.add_rms_norm(x, w, quantise=True), "multiple of 128"),
+        (lambda: fused.add_rms_norm(x, w, eps=-1.0), "eps"),
+        (lambda: fused.add_rms_norm(x[:, :0], w[:0]), "hidden size"),
+        (lambda: fused.add_rms_norm(torch.zeros(1, 49153, device="cuda"), torch.ones(49153, device="cuda")), "hidden size"),
+        (lambda: fused.dequantise_rows(torch.zeros(2, 130, device="cuda", dtype=torch.uint8), torch.zeros(2, 1, device="cuda")), "multiple of 128"),
+        (lambda: fused.dequantise_rows(torch.zeros(2, 256, device="cuda", dtype=torch.uint8), torch.zeros(2, 1, device="cuda")), "scales"),
+    ]:
+        with pytest.raises(RuntimeError, match=match):
+            bad()
