@@ -404,6 +404,40 @@ struct RowNormBwdArgs {
 };
 int row_norm_bwd_blocks(const RowNormBwdArgs& a, int sms);
 cudaError_t launch_row_norm_bwd(const RowNormBwdArgs& a, int blocks, cudaStream_t stream);
+// Balance loss of a router: c_e = how often live tokens chose expert e, s = softmax of a token's logits or its sigmoids over their sum,
+// loss = E / (K N^2) * sum over e of c_e * (sum over the N live tokens of s_e). NaN counts as -inf; a token without a finite or
+// infinite score adds nothing.
+constexpr int kBalanceMaxExperts = 1024;
+struct BalanceArgs {
+  const void* logits;          // [T, E], rows stride elements apart
+  long long stride;
+  int logits_bf16;             // else fp32
+  const int* topk_idx;         // [T, K]; entries outside [0, E) count for no expert
+  const unsigned char* mask;   // [T] or null: live tokens are nonzero
+  int T, E, K;
+  int sigmoid;
+  float* sums;                 // [blocks][E] scratch
+  int* chosen;                 // [blocks][E + 1] scratch: counts, live tokens
+  float* loss;                 // out
+  int* counts;                 // [E] out
+  int* live;                   // out: N
+};
+int balance_blocks(const BalanceArgs& a, int sms);
+cudaError_t launch_balance(const BalanceArgs& a, int blocks, cudaStream_t stream);
+// dlogits [T, E], the logits' type, from the forward pass's counts and N: E / (K N^2) * *dloss * ds/dlogits . c.
+struct BalanceBwdArgs {
+  const void* logits;
+  long long stride;
+  int logits_bf16;
+  const unsigned char* mask;
+  int T, E, K;
+  int sigmoid;
+  const int* counts;
+  const int* live;
+  const float* dloss;
+  void* dlogits;               // [T, E] out
+};
+cudaError_t launch_balance_bwd(const BalanceBwdArgs& a, int sms, cudaStream_t stream);
 // AdamW on bf16 parameters with fp32 master weights and moments, several tensors per launch.
 struct AdamWTensor {
   __nv_bfloat16* param;

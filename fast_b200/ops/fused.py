@@ -1,12 +1,11 @@
 """Small fused autograd ops around the MoE block: embedding with a segmented-sum backward, the
 mean-square loss of a residual sum computed without materialising fp32 copies, and the dense side of a block (residual
-sum and RMS norm of rows)."""
+sum and RMS norm of rows, the router's balance loss)."""
 from __future__ import annotations
 
-from typing import NamedTuple, Optional
+from typing import NamedTuple, Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import runtime
 
@@ -66,28 +65,6 @@ class NormRows(NamedTuple):
     scales: Optional[torch.Tensor]
 
 
-class _AddRMSNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, residual, eps, quantise):
-        y, h, q, scales, rstd = runtime.ext().row_norm(x, weight, eps, residual, quantise, True)
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x if h is None else h, weight, rstd)
-        if quantise:
-            ctx.mark_non_differentiable(q, scales)
-        return y, h, q, scales
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dh, _dq, _dscales):
-        h, weight, rstd = ctx.saved_tensors
-        want_x, want_w, want_r = ctx.needs_input_grad[:3]
-        if dy is None:   # only the sum was used
-            dx, dw = dh, (torch.zeros_like(weight) if want_w else None)
-        else:
-            dx, dw = runtime.ext().row_norm_bwd(h, weight, rstd, dy, dh)
-        return dx if want_x else None, dw if want_w else None, dx if want_r else None, None, None
-
-
 def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residual: Optional[torch.Tensor] = None, quantise: bool = False) -> NormRows:
     """RMS norm of rows, with the residual's addition in front of it and optionally an output in e4m3.
 
@@ -96,13 +73,23 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, resid
     ``weight``: bf16 or fp32 [hidden]; hidden up to 49152. ``quantise`` (hidden a multiple of 128): ``y`` also as the e4m3 rows that the
     fp8 dispatch would send for it (``dequantise_rows`` reads them back). Gradients flow through y and h, not through q and scales; the weight's
     gradient is summed in a fixed order."""
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
-        y, h, q, scales = _AddRMSNorm.apply(x, weight, residual, eps, quantise)
-    else:
-        y, h, q, scales, _ = runtime.ext().row_norm(x, weight, eps, residual, quantise, False)
-    return NormRows(y, x if h is None else h, q, scales)
+    return NormRows(*runtime.ext().add_rms_norm(x, weight, eps, residual, quantise))
 
 
 def dequantise_rows(q: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     """bf16 rows of e4m3 bytes (uint8 [..., hidden]) and fp32 scales [..., hidden / 128], as ``add_rms_norm`` makes them."""
     return runtime.ext().dequantise_rows(q, scales)
+
+
+def balance_loss(logits: torch.Tensor, topk_idx: torch.Tensor, mask: Optional[torch.Tensor] = None, scores: str = "softmax") -> Tuple[torch.Tensor, torch.Tensor]:
+    """Balance loss of a router and how often each expert was chosen: ``(loss, counts)``, an fp32 scalar and int32 [experts].
+
+    ``loss = E / (K N^2) * sum_e counts[e] * sum_t s[t, e]`` over the N live tokens: 1 when choices and scores are spread evenly, more when the
+    experts that are chosen often are also those with high scores. ``s``: the softmax of a token's logits, or with ``scores="sigmoid"`` their sigmoids
+    divided by the sum of these. logits: bf16 or fp32 [..., experts] (up to 1024), without a bias that only the choice uses; ``topk_idx``: int32
+    [..., k] as the routing returns it (entries outside the experts' range count for none); ``mask``: bool [...], False for padding, which has
+    no part in anything. NaN logits count as -inf; a token whose scores are all zero adds no score; without live tokens the loss is 0. Gradients
+    flow to the logits only. The result does not change from run to run."""
+    if scores not in ("softmax", "sigmoid"):
+        raise ValueError(f"balance_loss: scores must be 'softmax' or 'sigmoid', got {scores!r}")
+    return runtime.ext().balance_loss(logits, topk_idx, mask, scores == "sigmoid")

@@ -14,6 +14,34 @@ def test_row_norm_refuses_tensors_of_the_host():
         fused.dequantise_rows(torch.zeros(2, 128, dtype=torch.uint8), torch.zeros(2, 1))
 
 
+def test_balance_loss_refuses_what_it_does_not_know():
+    logits, idx = torch.zeros(4, 8), torch.zeros(4, 2, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        fused.balance_loss(logits, idx)
+    with pytest.raises(ValueError, match="scores"):
+        fused.balance_loss(logits, idx, scores="tanh")
+
+
+@pytest.mark.gpu
+def test_balance_loss_refusals():
+    logits, idx = torch.zeros(4, 8, device="cuda"), torch.zeros(4, 2, dtype=torch.int32, device="cuda")
+    mask = torch.ones(4, dtype=torch.bool, device="cuda")
+    for bad, match in [
+        (lambda: fused.balance_loss(logits.half(), idx), "bf16 or fp32"),
+        (lambda: fused.balance_loss(torch.zeros(4, 1025, device="cuda"), idx), "experts"),
+        (lambda: fused.balance_loss(logits[:, :0], idx), "experts"),
+        (lambda: fused.balance_loss(logits, idx.long()), "topk_idx"),
+        (lambda: fused.balance_loss(logits, idx[:3]), "topk_idx"),
+        (lambda: fused.balance_loss(logits, idx[:, :0]), "topk_idx"),
+        (lambda: fused.balance_loss(logits, idx.cpu()), "topk_idx"),
+        (lambda: fused.balance_loss(logits, idx, mask=mask[:3]), "mask"),
+        (lambda: fused.balance_loss(logits, idx, mask=mask.float()), "mask"),
+        (lambda: fused.balance_loss(logits, idx, mask=mask.unsqueeze(1)), "mask"),
+    ]:
+        with pytest.raises(RuntimeError, match=match):
+            bad()
+
+
 @pytest.mark.gpu
 def test_row_norm_refusals():
     x, w = torch.zeros(4, 200, device="cuda", dtype=BF), torch.ones(200, device="cuda", dtype=BF)

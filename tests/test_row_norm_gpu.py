@@ -220,3 +220,11 @@ def test_training_step_captured_and_replayed():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(grads, step(x, res)))
+
+
+def test_its_backward_has_no_gradient():
+    x, w = rand((3, 256), BF, 1).requires_grad_(), rand((256,), BF, 2).requires_grad_()
+    g = torch.autograd.grad(fused.add_rms_norm(x, w, residual=x).y.float().sum(), [x, w], create_graph=True)
+    for t in g:
+        with pytest.raises(RuntimeError, match="no gradient"):
+            t.float().sum().backward()
