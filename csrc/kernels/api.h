@@ -79,7 +79,9 @@ enum class GemmEpilogue : int {
   kSwiGLU = 1,     // forward: out = silu(gate) * up (+ optional raw gate|up tile)
   kSwiGLUBwd = 2,  // dgrad of the second projection: the tile is d(act); c2 holds the saved gate|up tiles and c
                    // receives d(gate|up) in the same layout (CTA-pair kernel only)
+  kLinear = 3,     // dense forward: out = act(tile + bias) + residual (launch_dense_gemm)
 };
+enum class Activation : int { kNone = 0, kRelu = 1, kSilu = 2, kGelu = 3 };
 
 struct GemmArgs {
   const int* group_off;    // [num_groups + 1] row offsets of the groups, multiples of 128 (device)
@@ -108,6 +110,7 @@ struct GemmArgs {
                            // over them up to a multiple of 64
   int gate_tile_rows;      // 0: gate_counter / gate_target are indexed by group; > 0: by (row of the grouped matrix) / gate_tile_rows
   int gate_slots;          // entries of gate_counter / gate_target (indices are clamped to the last one)
+  int dense_rows;          // weight gradients without group_off: one group of this many rows
   int wide;                // CTA-pair weight gradients: tiles of 512 columns (tiles_n counts those) instead of 256; map_c has boxes {64,32}
 };
 
@@ -163,6 +166,26 @@ struct TokGemmArgs {
   int gate_tile_rows, gate_slots;
 };
 cudaError_t launch_grouped_gemm_tokens(GemmMode mode, GemmEpilogue epi, const TokGemmMaps& maps, const TokGemmArgs& args, int ctas, cudaStream_t stream);
+
+// The same for one weight matrix of any size (sizes that are multiples of 8; what a tile has past the end is zeros on its way in and stays
+// unwritten on its way out). num_groups = 1, no group tables. partials and counters (zeroed, num_counters = 0, counters_next null) only where
+// dense_is_cut says so; counters are zero again afterwards.
+struct TokDenseArgs : TokGemmArgs {
+  int dense_rows;            // tokens
+  int features;              // columns of the output
+  // kLinear
+  const __nv_bfloat16* bias; // [features] or null
+  Activation act;
+  int has_residual, keep_pre;   // maps.c2, maps.c3
+};
+struct TokDenseMaps : TokGemmMaps {
+  const CUtensorMap* c3;     // kLinear with keep_pre: what the activation is taken of, written as bf16 {64,32}
+};
+bool dense_is_cut(const TokDenseArgs& args, int ctas);
+// kForward: kStore, kSwiGLU, kLinear (maps.c2: the residual {64,32}); kDgrad: kStore.
+cudaError_t launch_dense_gemm(GemmMode mode, GemmEpilogue epi, const TokDenseMaps& maps, const TokDenseArgs& args, int ctas, cudaStream_t stream);
+// Where dense launches on the current device report a wait that gave up.
+DeviceStatus* dense_status();
 
 // ---------------------------------------------------------------------------------------------
 // MoE routing / dispatch / combine
@@ -367,7 +390,7 @@ int embedding_index_block();
 cudaError_t launch_embedding_rows(const int* start, const long long* perm, const __nv_bfloat16* grad_out, __nv_bfloat16* grad_table, int V, int H, cudaStream_t stream);
 cudaError_t launch_embedding_few(const long long* ids, const __nv_bfloat16* grad_out, __nv_bfloat16* grad_table, int T, int V, int H, cudaStream_t stream);
 // ---------------------------------------------------------------------------------------------
-// the dense side of a block: row norm, balance loss (row_norm.cu, balance_loss.cu)
+// the dense side of a block: row norm, balance loss, the epilogue of linear layers (row_norm.cu, balance_loss.cu, linear_grads.cu)
 // ---------------------------------------------------------------------------------------------
 // h = x + residual rounded to the rows' type (no residual: h = x), y = h / sqrt(mean(h^2) + eps) * weight, and y in e4m3 (see quantise_rows).
 constexpr int kRowNormMaxHidden = 48 * 1024;
@@ -438,6 +461,11 @@ struct BalanceBwdArgs {
   void* dlogits;               // [T, E] out
 };
 cudaError_t launch_balance_bwd(const BalanceBwdArgs& a, int sms, cudaStream_t stream);
+// out[c] = sum over `blocks` rows of partials [blocks][n], in a fixed order; bf16 or fp32.
+cudaError_t launch_fold_columns(const float* partials, int blocks, int n, bool as_bf16, void* out, cudaStream_t stream);
+// dz = dy * act'(z) [T, N] (kNone: dz is dy, nothing is written) and, with partials [blocks][N], dbias [N] = the column sums of dz. N % 8 == 0.
+int linear_dz_blocks(int T, int N, int sms);
+cudaError_t launch_linear_dz(Activation act, const __nv_bfloat16* dy, const __nv_bfloat16* z, __nv_bfloat16* dz, float* partials, int T, int N, int blocks, __nv_bfloat16* dbias, cudaStream_t stream);
 // AdamW on bf16 parameters with fp32 master weights and moments, several tensors per launch.
 struct AdamWTensor {
   __nv_bfloat16* param;

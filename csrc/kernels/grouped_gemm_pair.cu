@@ -69,6 +69,7 @@ struct __align__(8) SmemCtl {
   uint64_t full[kStages], empty[kStages], acc_full[kAccStages], acc_empty[kAccStages], q_full[kQStages], q_empty[kQStages];
   uint32_t tmem_base;
   int abort_flag;
+  int dense_off[2];                // the group table of a launch without one
 };
 constexpr int kSmemBytes = kStages * kStageBytes + kEpiBytes + 1024 + sizeof(SmemCtl);
 constexpr int kSmemBytesFp8 = kStagesFp8 * kStageBytes + kQStages * kQBytes + kEpiBytes + 1024 + sizeof(SmemCtl);
@@ -123,6 +124,8 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     for (int a = 0; a < kAccStages; ++a) { mbar_init(&ctl->acc_full[a], 1); mbar_init(&ctl->acc_empty[a], 2 * kEpiWarps); }
     for (int q = 0; q < kQStages; ++q) { mbar_init(&ctl->q_full[q], 1); mbar_init(&ctl->q_empty[q], 1); }
     ctl->abort_flag = 0;
+    ctl->dense_off[0] = 0;
+    ctl->dense_off[1] = (p.dense_rows + BK - 1) / BK * BK;   // rows past the real ones come in as zeros: they lie outside the matrices
     mbar_fence_init();
     prefetch_tmap(&map_a);
     prefetch_tmap(&map_b);
@@ -140,7 +143,7 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
   volatile int* abort_flag = &ctl->abort_flag;
 
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  TileWalker<TILE_M> walk{p.group_off, p.num_groups, p.tiles_n, p.fixed_m_tiles, p.red_len, MODE == GemmMode::kWgrad, p.band_rows, MODE == GemmMode::kWgrad ? p.group_rows : nullptr};
+  TileWalker<TILE_M> walk{MODE == GemmMode::kWgrad && p.group_off == nullptr ? ctl->dense_off : p.group_off, p.num_groups, p.tiles_n, p.fixed_m_tiles, p.red_len, MODE == GemmMode::kWgrad, p.band_rows, MODE == GemmMode::kWgrad ? p.group_rows : nullptr};
   TileCoord tc;
   auto give_registers = [] {
     if constexpr (WIDE) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
@@ -468,6 +471,7 @@ cudaError_t launch_kernel(Kernel kern, int threads, int smem, const CUtensorMap&
 cudaError_t launch_grouped_gemm_pair(GemmMode mode, GemmEpilogue epi, const CUtensorMap& map_a, const CUtensorMap& map_b, const CUtensorMap& map_c,
                                      const CUtensorMap* map_c2, const GemmArgs& args, int ctas, cudaStream_t stream) {
   if (ctas < 2) return cudaErrorInvalidValue;
+  if (args.group_off == nullptr && (mode != GemmMode::kWgrad || args.num_groups != 1 || args.dense_rows < 0 || args.direct_epilogue)) return cudaErrorInvalidValue;
   if ((args.c2 != nullptr) != (map_c2 != nullptr)) return cudaErrorInvalidValue;
   const CUtensorMap& c2 = map_c2 ? *map_c2 : map_c;  // unused by the kernel when args.c2 is null
   if (args.a_scales != nullptr) {

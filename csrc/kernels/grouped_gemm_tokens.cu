@@ -70,7 +70,7 @@ struct __align__(8) TokCtl {
   int abort_flag, last_arrived, widest, share_weights;
   int base[kTokPrefix + 1];                         // tiles of the groups before entry i
 };
-__host__ __device__ constexpr int epi_boxes(GemmEpilogue e) { return e == GemmEpilogue::kStore ? 2 : e == GemmEpilogue::kSwiGLU ? 3 : 4; }
+__host__ __device__ constexpr int epi_boxes(GemmEpilogue e) { return e == GemmEpilogue::kStore ? 2 : e == GemmEpilogue::kSwiGLU ? 3 : 4; }   // kLinear: two of the residual and the output, two of the pre-activation
 constexpr int kSmemLimit = 227 * 1024;
 constexpr int other_bytes(GemmEpilogue e) { return 2 * epi_boxes(e) * kBox + 1024 + static_cast<int>(sizeof(TokCtl)); }
 // Operand stages that fit. Tiles of up to 256 tokens: 6 of 32 KiB. Where few tokens meet the weights, the loop is bound by
@@ -121,11 +121,22 @@ __device__ __forceinline__ float as_f(uint32_t x) { return __uint_as_float(x); }
 // Tokens of a tile of n that accumulator `sub` holds.
 __device__ __forceinline__ int acc_n(int n, int sub) { return sub == 0 ? min(n, kTokAccN) : max(n - kTokAccN, 0); }
 
-template <GemmMode MODE, GemmEpilogue EPI, int SUB>
+// gelu(z) = z Phi(z)
+__device__ __forceinline__ float activate(Activation act, float z) {
+  switch (act) {
+    case Activation::kRelu: return fmaxf(z, 0.0f);
+    case Activation::kSilu: return silu(z);
+    case Activation::kGelu: return 0.5f * z * (1.0f + erff(z * 0.70710678f));
+    default: return z;
+  }
+}
+
+template <GemmMode MODE, GemmEpilogue EPI, int SUB, class Args>
 __global__ void __launch_bounds__(threads_for(SUB), 1)
 grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ TokMapsX map_x, const __grid_constant__ CUtensorMap map_c,
-                           const __grid_constant__ CUtensorMap map_c2,
-                           const TokGemmArgs p) {
+                           const __grid_constant__ CUtensorMap map_c2, const __grid_constant__ CUtensorMap map_c3, const Args p) {
+  constexpr bool DENSE = tok_dense<Args>::value;
+  static_assert(EPI != GemmEpilogue::kLinear || (DENSE && SUB == 1 && MODE == GemmMode::kForward), "one weight matrix, tiles of one accumulator");
   constexpr bool A_MN = MODE == GemmMode::kDgrad;
   constexpr int kRing = epi_boxes(EPI) * kBox;
   extern __shared__ uint8_t smem_raw[];
@@ -183,7 +194,7 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const TokSplit split = TokSplit::make(ctl->base[div_up(p.num_groups, per_entry)], p.red_blocks, pairs, ctl->widest, ctl->share_weights != 0);
   TokSegments segs(split, pair);
-  TokTiles<TokGemmArgs> walk{p, ctl->base, per_entry};
+  TokTiles<Args> walk{p, ctl->base, per_entry};
   TokSegment sg;
   auto give_registers = [] {
     if constexpr (SUB == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
@@ -395,6 +406,7 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
         __threadfence();
       }
       const int feat0 = tc.m * kPairM + cta * kHalfM;          // my 128 features
+      auto inside = [&](int feature) { if constexpr (DENSE) return feature < p.features; else return true; };   // boxes past the last feature stay where they are
       auto row_of = [&](int sub, int st) { return tc.row0 + sub * kTokAccN + st * kStepTokens; };
       // 32 tokens of my features, (r[0..15]: lanes 0-15 of the warp, r[16..31]: lanes 16-31): from tensor memory, or the parts in
       // the order of the reduction.
@@ -460,8 +472,8 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
           fence_proxy_async_smem();
           group_bar(group);
           if (issuer) {
-            tma_store_2d(&map_c, b, feat0, y);
-            tma_store_2d(&map_c, b + kBox, feat0 + 64, y);
+            if (inside(feat0)) tma_store_2d(&map_c, b, feat0, y);
+            if (inside(feat0 + 64)) tma_store_2d(&map_c, b + kBox, feat0 + 64, y);
             bulk_commit();
           }
           ++ring_n;
@@ -537,7 +549,86 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
         }
         ++ring_n;
       };
-      if constexpr (SUB == 1) {
+      if constexpr (EPI == GemmEpilogue::kLinear) {
+        // 32 tokens at a time: residual boxes come in by TMA two steps ahead and are overwritten by what goes out.
+        auto load_residual = [&](int st) {                     // issuer only
+          uint8_t* b = ring + (st & 1) * kRing;
+          mbar_arrive_expect_tx(&ctl->epi_load[st & 1], 2 * kBox);
+#pragma unroll
+          for (int q = 0; q < 2; ++q) tma_load_2d(b + q * kBox, &map_c2, feat0 + q * 64, row_of(0, st), &ctl->epi_load[st & 1]);
+        };
+        if (p.has_residual && issuer) {
+          bulk_wait_read<0>();
+          load_residual(0);
+          if (steps_of(0) > 1) load_residual(1);
+        }
+        float bias[4];                                          // of features lane / 4 + 8 i
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int f = feat0 + quarter * 32 + 8 * i + (lane >> 2);
+          bias[i] = p.bias != nullptr && f < p.features ? __bfloat162float(p.bias[f]) : 0.0f;
+        }
+        if (sg.parts == 1) wait_acc(0);
+#pragma unroll 1
+        for (int st = 0; ok && st < steps_of(0); ++st) {
+          uint32_t r[32], h[16];
+          load_acc(0, st, r);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(as_f(r[i]) + bias[(i >> 4) * 2 + (i >> 1 & 1)]);
+          uint8_t* b;
+          if (p.has_residual) {
+            b = ring + (st & 1) * kRing;
+            if (!(ok = mbar_wait_bounded(&ctl->epi_load[st & 1], (load_ph >> (st & 1)) & 1u, abort_flag, p.status, 500, p.timeout_ns))) break;
+            load_ph ^= 1u << (st & 1);
+          } else {
+            b = acquire();
+          }
+          const uint32_t sb = smem_u32(b) + (quarter >> 1) * kBox;
+          const int chunk = (quarter & 1) * 4;
+          if (p.keep_pre) {
+            to_bf16(r, h);
+            put(sb + 2 * kBox, chunk, h);
+            put(sb + 2 * kBox, chunk + 2, h + 8);
+          }
+          if (p.act != Activation::kNone) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(activate(p.act, as_f(r[i])));
+          }
+          if (p.has_residual) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t v[4];
+              ldmatrix_trans(box_row(sb, lane, e & 1, chunk + (e >> 1) * 2), v);
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v[q]));
+                uint32_t* at = r + 2 * (4 * e + q);
+                at[0] = __float_as_uint(as_f(at[0]) + f.x);
+                at[1] = __float_as_uint(as_f(at[1]) + f.y);
+              }
+            }
+          }
+          to_bf16(r, h);
+          put(sb, chunk, h);
+          put(sb, chunk + 2, h + 8);
+          fence_proxy_async_smem();
+          group_bar(group);
+          if (issuer) {
+            const int y = row_of(0, st);
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+              if (inside(feat0 + q * 64)) {
+                tma_store_2d(&map_c, b + q * kBox, feat0 + q * 64, y);
+                if (p.keep_pre) tma_store_2d(&map_c3, b + (2 + q) * kBox, feat0 + q * 64, y);
+              }
+            bulk_commit();
+            if (p.has_residual && st + 2 < steps_of(0)) { bulk_wait_read<0>(); load_residual(st + 2); }
+          }
+          ++ring_n;
+        }
+        if (!ok) break;
+        if (sg.parts == 1) release_acc(0);
+      } else if constexpr (SUB == 1) {
         if (EPI == GemmEpilogue::kSwiGLUBwd) begin_gu(0);       // the saved tiles arrive while the MMAs still run
         if (sg.parts == 1) wait_acc(0);
         for (int st = 0; ok && st < steps_of(0); ++st) {
@@ -646,9 +737,9 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
   if (warp == 1) { tc_fence_after_sync(); tmem_dealloc_pair(tmem_base, kTmemCols); }
 }
 
-template <GemmMode MODE, GemmEpilogue EPI, int SUB>
-cudaError_t launch_sub(const TokGemmMaps& m, TokGemmArgs args, int ctas, cudaStream_t stream) {
-  auto kern = grouped_gemm_tokens_kernel<MODE, EPI, SUB>;
+template <GemmMode MODE, GemmEpilogue EPI, int SUB, class Args>
+cudaError_t launch_sub(const TokGemmMaps& m, const CUtensorMap* c3, Args args, int ctas, cudaStream_t stream) {
+  auto kern = grouped_gemm_tokens_kernel<MODE, EPI, SUB, Args>;
   args.stages = stages_for(EPI, args.tile_n);
   const int smem = smem_bytes(EPI, args.tile_n);
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -664,16 +755,44 @@ cudaError_t launch_sub(const TokGemmMaps& m, TokGemmArgs args, int ctas, cudaStr
   attr[1] = early_start_attribute();
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  e = cudaLaunchKernelEx(&cfg, kern, *m.w, *m.x, *m.c, m.c2 ? *m.c2 : *m.c, args);
+  e = cudaLaunchKernelEx(&cfg, kern, *m.w, *m.x, *m.c, m.c2 ? *m.c2 : *m.c, c3 ? *c3 : *m.c, args);
   if (e == cudaSuccess) note_launch();
   return e;
 }
-template <GemmMode MODE, GemmEpilogue EPI>
-cudaError_t launch(const TokGemmMaps& m, const TokGemmArgs& args, int ctas, cudaStream_t stream) {
-  return args.tile_n > kTokAccN ? launch_sub<MODE, EPI, 2>(m, args, ctas, stream) : launch_sub<MODE, EPI, 1>(m, args, ctas, stream);
+template <GemmMode MODE, GemmEpilogue EPI, class Args>
+cudaError_t launch(const TokGemmMaps& m, const Args& args, int ctas, cudaStream_t stream) {
+  return args.tile_n > kTokAccN ? launch_sub<MODE, EPI, 2>(m, nullptr, args, ctas, stream) : launch_sub<MODE, EPI, 1>(m, nullptr, args, ctas, stream);
 }
 
+TokSplit dense_split(const TokDenseArgs& a, int ctas) {
+  const int rows = tok_rows(a, 0);
+  return TokSplit::make(tok_group_tiles(a, 0), a.red_blocks, ctas / 2, tok_tile_size(rows, a.tile_n), tok_tiles(rows, a.tile_n) > 1);
+}
+
+__device__ DeviceStatus g_dense_status;   // one on every device that the library runs on
+
 }  // namespace
+
+DeviceStatus* dense_status() {
+  void* p = nullptr;
+  return cudaGetSymbolAddress(&p, g_dense_status) == cudaSuccess ? static_cast<DeviceStatus*>(p) : nullptr;
+}
+
+bool dense_is_cut(const TokDenseArgs& args, int ctas) { return dense_split(args, ctas).cut_tiles > 0; }
+
+cudaError_t launch_dense_gemm(GemmMode mode, GemmEpilogue epi, const TokDenseMaps& maps, const TokDenseArgs& args, int ctas, cudaStream_t stream) {
+  if (ctas < 2 || args.num_groups != 1 || args.dense_rows < 1 || args.features < 1 || args.m_tiles != div_up(args.features, kPairM) || args.red_blocks < 1 || args.band_tiles < 1) return cudaErrorInvalidValue;
+  if (args.tile_n != 64 && args.tile_n != 128 && args.tile_n != kTokAccN && (args.tile_n != 2 * kTokAccN || epi == GemmEpilogue::kLinear)) return cudaErrorInvalidValue;
+  if (args.granule != 32 || args.num_counters != 0 || args.status == nullptr || args.gate_counter != nullptr) return cudaErrorInvalidValue;
+  if (dense_is_cut(args, ctas) && (args.partials == nullptr || args.counters == nullptr)) return cudaErrorInvalidValue;
+  if (mode == GemmMode::kDgrad && epi == GemmEpilogue::kStore) return launch<GemmMode::kDgrad, GemmEpilogue::kStore>(maps, args, ctas, stream);
+  if (mode != GemmMode::kForward) return cudaErrorInvalidValue;
+  if (epi == GemmEpilogue::kStore) return launch<GemmMode::kForward, GemmEpilogue::kStore>(maps, args, ctas, stream);
+  if (epi == GemmEpilogue::kSwiGLU && args.features % kPairM == 0 && (args.keep_gate_up != 0) == (maps.c2 != nullptr)) return launch<GemmMode::kForward, GemmEpilogue::kSwiGLU>(maps, args, ctas, stream);
+  if (epi == GemmEpilogue::kLinear && (args.has_residual != 0) == (maps.c2 != nullptr) && (args.keep_pre != 0) == (maps.c3 != nullptr))
+    return launch_sub<GemmMode::kForward, GemmEpilogue::kLinear, 1>(maps, maps.c3, args, ctas, stream);
+  return cudaErrorInvalidValue;
+}
 
 cudaError_t launch_grouped_gemm_tokens(GemmMode mode, GemmEpilogue epi, const TokGemmMaps& maps, const TokGemmArgs& args, int ctas, cudaStream_t stream) {
   if (ctas < 2 || args.num_groups < 1 || args.m_tiles < 1 || args.red_blocks < 1 || args.band_tiles < 1) return cudaErrorInvalidValue;

@@ -1,0 +1,103 @@
+// Backward of a linear layer's epilogue: out = act(z) + residual, z = x W^T + bias.
+//
+//   dz = dy act'(z), rounded to bf16 for the two products that take it;  dbias = sum over rows of dz, from the values before that rounding
+//
+// One pass: 8 columns a thread, rows in turn, column sums in registers and one partial sum a block of rows, added up in a fixed order.
+// What bounds it: HBM, 6 bytes an element (2 where there is no activation: then dz is dy, and only the bias wants its sums).
+#include <algorithm>
+
+#include "early_start.cuh"
+#include "gemm_common.cuh"
+
+namespace fastb {
+
+namespace {
+
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+
+// act'(z)
+template <Activation ACT>
+__device__ __forceinline__ float slope(float z) {
+  if (ACT == Activation::kRelu) return z > 0.0f ? 1.0f : 0.0f;
+  if (ACT == Activation::kSilu) {
+    const float s = gemm::sigmoid(z);
+    return s * (1.0f + z * (1.0f - s));
+  }
+  if (ACT == Activation::kGelu) return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * 0.39894228f * __expf(-0.5f * z * z);
+  return 1.0f;
+}
+__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { const float2 t = __bfloat1622float2(h[i]); f[2 * i] = t.x; f[2 * i + 1] = t.y; }
+}
+
+// blockIdx.x: 256 columns; blockIdx.y: every gridDim.y-th group of eight rows, a row a warp.
+template <Activation ACT>
+__global__ void __launch_bounds__(kThreads) linear_dz_kernel(const __nv_bfloat16* __restrict__ dy, const __nv_bfloat16* __restrict__ z, __nv_bfloat16* __restrict__ dz, float* __restrict__ partials, int T,
+                                                             int N) {
+  constexpr int U = 4;   // rows in flight
+  __shared__ float s_sum[kWarps][256];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane, chunks = N / 8;
+  grid_dependency_wait();
+  launch_dependents();
+  float acc[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
+  const int step = gridDim.y * kWarps;
+  for (long long t0 = blockIdx.y * kWarps + warp; t0 < T; t0 += static_cast<long long>(U) * step) {
+    uint4 g[U], v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long t = t0 + static_cast<long long>(u) * step;
+      const bool in = t < T && c < chunks;
+      g[u] = in ? __ldg(reinterpret_cast<const uint4*>(dy) + t * chunks + c) : make_uint4(0, 0, 0, 0);
+      if (ACT != Activation::kNone) v[u] = in ? __ldcs(reinterpret_cast<const uint4*>(z) + t * chunks + c) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long t = t0 + static_cast<long long>(u) * step;
+      float d[8];
+      unpack8(g[u], d);
+      if (ACT != Activation::kNone) {
+        float f[8];
+        unpack8(v[u], f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) d[k] *= slope<ACT>(f[k]);
+        if (t < T && c < chunks)
+          reinterpret_cast<uint4*>(dz)[t * chunks + c] = make_uint4(gemm::pack_bf16(d[0], d[1]), gemm::pack_bf16(d[2], d[3]), gemm::pack_bf16(d[4], d[5]), gemm::pack_bf16(d[6], d[7]));
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) acc[k] += d[k];
+    }
+  }
+  if (partials == nullptr) return;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) s_sum[warp][k * 32 + lane] = acc[k];
+  __syncthreads();
+  float v = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) v += s_sum[w][threadIdx.x];
+  const int column = (blockIdx.x * 32 + (threadIdx.x & 31)) * 8 + (threadIdx.x >> 5);
+  if (column < N) partials[static_cast<size_t>(blockIdx.y) * N + column] = v;
+}
+
+}  // namespace
+
+int linear_dz_blocks(int T, int N, int sms) {
+  const int columns = (N + 255) / 256;
+  return std::max(1, std::min((T + 4 * kWarps - 1) / (4 * kWarps), (8 * sms + columns - 1) / columns));
+}
+
+cudaError_t launch_linear_dz(Activation act, const __nv_bfloat16* dy, const __nv_bfloat16* z, __nv_bfloat16* dz, float* partials, int T, int N, int blocks, __nv_bfloat16* dbias, cudaStream_t stream) {
+  if (T < 1 || N < 8 || N % 8 || blocks < 1 || (partials == nullptr) != (dbias == nullptr) || (act != Activation::kNone && (z == nullptr || dz == nullptr))) return cudaErrorInvalidValue;
+  const dim3 grid((N + 255) / 256, blocks);
+  const auto go = [&](auto kern) { return launch_early(kern, grid, kThreads, 0, stream, dy, z, dz, partials, T, N); };
+  const cudaError_t e = act == Activation::kRelu ? go(linear_dz_kernel<Activation::kRelu>) : act == Activation::kSilu ? go(linear_dz_kernel<Activation::kSilu>)
+                        : act == Activation::kGelu ? go(linear_dz_kernel<Activation::kGelu>) : go(linear_dz_kernel<Activation::kNone>);
+  note_launch();
+  if (e != cudaSuccess || partials == nullptr) return e;
+  return launch_fold_columns(partials, blocks, N, true, dbias, stream);
+}
+
+}  // namespace fastb

@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(256) row_norm_bwd_any_kernel(const RowNormBwdA
   for (int c = threadIdx.x; c < a.H; c += blockDim.x) a.partials[static_cast<size_t>(blockIdx.x) * a.H + c] = s_dw[c];
 }
 
-// dweight = the blocks' partial sums, added in a fixed order: 32 columns a block, a warp every 32nd partial.
+// The blocks' partial sums, added in a fixed order: 32 columns a block, a warp every 32nd partial.
 template <class W>
 __global__ void __launch_bounds__(1024) fold_columns_kernel(const float* __restrict__ partials, int blocks, int H, W* __restrict__ out) {
   __shared__ float s[32][33];
@@ -451,10 +451,15 @@ cudaError_t launch_row_norm_bwd(const RowNormBwdArgs& args, int blocks, cudaStre
     return a.dh != nullptr ? go(std::true_type()) : go(std::false_type());
   });
   if (e != cudaSuccess) return e;
-  const dim3 grid((a.H + 31) / 32);
-  if (a.weight_bf16) e = launch_early(fold_columns_kernel<bf16>, grid, 1024, 0, stream, static_cast<const float*>(a.partials), blocks, a.H, static_cast<bf16*>(a.dweight));
-  else e = launch_early(fold_columns_kernel<float>, grid, 1024, 0, stream, static_cast<const float*>(a.partials), blocks, a.H, static_cast<float*>(a.dweight));
-  note_launch(2);
+  note_launch();
+  return launch_fold_columns(a.partials, blocks, a.H, a.weight_bf16 != 0, a.dweight, stream);
+}
+
+cudaError_t launch_fold_columns(const float* partials, int blocks, int n, bool as_bf16, void* out, cudaStream_t stream) {
+  const dim3 grid((n + 31) / 32);
+  const cudaError_t e = as_bf16 ? launch_early(fold_columns_kernel<bf16>, grid, 1024, 0, stream, partials, blocks, n, static_cast<bf16*>(out))
+                                : launch_early(fold_columns_kernel<float>, grid, 1024, 0, stream, partials, blocks, n, static_cast<float*>(out));
+  note_launch();
   return e;
 }
 

@@ -37,6 +37,13 @@ constexpr long long kBackBandBytes = 32ll << 20;
 FASTB_HD inline bool wgrad_back(int red_blocks, int band_rows) {
   return 2ll * red_blocks * kWalkBK * (band_rows > 0 ? band_rows : kDefaultBandRows) > kBackBandBytes;
 }
+// Whether weight gradients take tiles of 512 columns instead of 256 (wide_columns in ops/gemm.py says why and what was measured).
+FASTB_HD inline bool wgrad_wide(int row_tiles, int columns, int pairs, int mean_rows) {
+  if (columns % 512) return false;
+  const int narrow = (row_tiles * (columns / 256) + pairs - 1) / pairs, wide = (row_tiles * (columns / 512) + pairs - 1) / pairs;
+  if (mean_rows < 512) return narrow >= 4 && 14 * wide <= 8 * narrow;
+  return (mean_rows <= 640 ? narrow >= 14 : mean_rows >= 1536) && 50 * wide <= 26 * narrow;
+}
 template <int TILE_M>
 struct TileWalker {
   const int* off; int G, tiles_n, fixed_m, red_len; bool wgrad; int band_rows;

@@ -9,6 +9,8 @@
 #define FASTB_HD
 #endif
 
+#include <type_traits>
+
 namespace fastb {
 namespace gemm {
 
@@ -157,10 +159,22 @@ FASTB_HD inline TokPlace tok_place(int local, int m_tiles, int t_tiles, int band
   return TokPlace{rem / cur, t0 + rem % cur};
 }
 
+// Args with dense_rows (TokDenseArgs) are one group of that many rows, which the host knows: no table in device memory.
+template <class Args, class = void> struct tok_dense : std::false_type {};
+template <class Args> struct tok_dense<Args, std::void_t<decltype(Args::dense_rows)>> : std::true_type {};
+
 // Rows of group q that are worked on: the real ones, up to a multiple of the granule. Args: TokGemmArgs, or on the host anything with its
 // group_off, group_rows, granule, tile_n, m_tiles and band_tiles.
 template <class Args>
-FASTB_HD inline int tok_rows(const Args& p, int q) { return p.group_rows ? ceil_to(p.group_rows[q], p.granule) : p.group_off[q + 1] - p.group_off[q]; }
+FASTB_HD inline int tok_rows(const Args& p, int q) {
+  if constexpr (tok_dense<Args>::value) return ceil_to(p.dense_rows, p.granule);
+  else return p.group_rows ? ceil_to(p.group_rows[q], p.granule) : p.group_off[q + 1] - p.group_off[q];
+}
+template <class Args>
+FASTB_HD inline int tok_first_row(const Args& p, int q) {
+  if constexpr (tok_dense<Args>::value) return 0;
+  else return p.group_off[q];
+}
 template <class Args>
 FASTB_HD inline int tok_group_tiles(const Args& p, int q) { return tok_tiles(tok_rows(p, q), p.tile_n) * p.m_tiles; }
 
@@ -185,7 +199,7 @@ struct TokTiles {
     while (tile >= g_base + tok_tiles(rows, p.tile_n) * p.m_tiles) { g_base += tok_tiles(rows, p.tile_n) * p.m_tiles; rows = tok_rows(p, ++g); }
     const TokPlace at = tok_place(tile - g_base, p.m_tiles, tok_tiles(rows, p.tile_n), p.band_tiles);
     const TokSpan span = tok_span(rows, p.tile_n, at.t);
-    return TokTile{g, at.m, p.group_off[g] + span.begin, span.n};
+    return TokTile{g, at.m, tok_first_row(p, g) + span.begin, span.n};
   }
 };
 

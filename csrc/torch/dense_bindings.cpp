@@ -4,7 +4,10 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include "../kernels/tile_walker.h"
+#include "../kernels/token_walker.h"
 #include "py_types.h"
+#include "tensor_maps.h"
 
 namespace py = pybind11;
 using namespace fastb;
@@ -246,10 +249,223 @@ std::tuple<torch::Tensor, torch::Tensor> balance_loss(const torch::Tensor& logit
   return {out[0], out[1]};
 }
 
+// ---- linear layers ----------------------------------------------------------------------------------------
+enum class LinearKind : int { kNone = 0, kRelu = 1, kSilu = 2, kGelu = 3, kSwiGLU = 4 };   // the first four are Activation's
+
+// Rows [n, cols] that TMA can read: contiguous rows, 16-byte aligned, a multiple of 16 bytes apart. What is not is copied.
+torch::Tensor tma_rows(const torch::Tensor& t, int64_t cols) {
+  torch::Tensor m = as_rows(t, cols);
+  const bool ok = reinterpret_cast<uintptr_t>(m.data_ptr()) % 16 == 0 && m.stride(1) == 1 && (m.size(0) <= 1 || (m.stride(0) % 8 == 0 && m.stride(0) >= cols));
+  return ok ? m : m.clone(at::MemoryFormat::Contiguous);
+}
+CUtensorMap rows_map(const torch::Tensor& m, int box_rows) {
+  const cuuint64_t rows = static_cast<cuuint64_t>(m.size(0)), cols = static_cast<cuuint64_t>(m.size(1)), dims[2] = {cols, rows}, strides[1] = {2 * (rows > 1 ? static_cast<cuuint64_t>(m.stride(0)) : cols)};
+  const cuuint32_t box[2] = {64u, static_cast<cuuint32_t>(box_rows)};
+  return bf16_map(2, reinterpret_cast<int64_t>(m.data_ptr()), dims, strides, box);
+}
+
+struct DenseEpilogue {
+  GemmEpilogue kind = GemmEpilogue::kStore;
+  const torch::Tensor *bias = nullptr, *residual = nullptr, *pre = nullptr;   // pre: pre-activation, or gate|up of kSwiGLU
+  Activation act = Activation::kNone;
+};
+
+// forward: out [T, N] = epilogue(x [T, K] . weight [N, K]^T); dgrad: out [T, K] = x [T, N] . weight [N, K]. All bf16 rows as tma_rows makes them.
+void dense_gemm(GemmMode mode, const torch::Tensor& weight, const torch::Tensor& x, const torch::Tensor& out, const DenseEpilogue& ep, uint64_t timeout_ns) {
+  const bool fwd = mode == GemmMode::kForward;
+  const int64_t N = weight.size(0), K = weight.size(1), features = fwd ? N : K, reduction = fwd ? K : N;
+  const int ctas = sm_count(x) & ~1;
+  TokDenseArgs a{};
+  a.num_groups = 1;
+  a.dense_rows = static_cast<int>(x.size(0)); a.features = static_cast<int>(features);
+  a.m_tiles = static_cast<int>((features + 255) / 256); a.red_blocks = static_cast<int>((reduction + 63) / 64);
+  a.granule = 32;
+  // Where all tokens fit a narrow tile, narrow tiles leave shared memory to the weights in flight.
+  a.tile_n = a.dense_rows <= 64 ? 64 : a.dense_rows <= 128 ? 128 : 256;
+  a.band_tiles = gemm::tok_band(0, 64 * a.red_blocks, a.m_tiles, a.tile_n);
+  a.back_tiles = gemm::tok_back_tiles(64 * a.red_blocks, a.band_tiles, std::max(a.tile_n, gemm::kTokAccN));
+  a.status = dense_status();
+  TORCH_CHECK(a.status != nullptr, "linear: no status block on this device");
+  a.timeout_ns = timeout_ns;
+  CUtensorMap w, c = rows_map(out, 32), c2, c3;
+  TokMapsX xm;
+  if (ep.kind == GemmEpilogue::kSwiGLU) {
+    // [N / 256 tiles][8 groups of 16 features][gate, up][16][K], fetched as four groups with both halves
+    const cuuint64_t k = static_cast<cuuint64_t>(K), dims[5] = {k, 16, 2, 8, static_cast<cuuint64_t>(N / 256)}, strides[4] = {2 * k, 256 * k, 32 * k, 512 * k};
+    const cuuint32_t box[5] = {64, 16, 2, 4, 1};
+    w = bf16_map(5, reinterpret_cast<int64_t>(weight.data_ptr()), dims, strides, box);
+  } else {
+    w = rows_map(weight, fwd ? 128 : 64);
+  }
+  for (int j = 0; j < kTokBoxes; ++j) xm.box[j] = rows_map(x, 16 << j);
+  TokDenseMaps maps{};
+  maps.w = &w; maps.x = &xm; maps.c = &c;
+  if (ep.kind == GemmEpilogue::kSwiGLU) {
+    if (ep.pre) { c2 = rows_map(*ep.pre, 32); maps.c2 = &c2; a.keep_gate_up = 1; }
+  } else if (ep.kind == GemmEpilogue::kLinear) {
+    a.act = ep.act;
+    if (ep.bias) a.bias = reinterpret_cast<const __nv_bfloat16*>(ep.bias->data_ptr());
+    if (ep.residual) { c2 = rows_map(*ep.residual, 32); maps.c2 = &c2; a.has_residual = 1; }
+    if (ep.pre) { c3 = rows_map(*ep.pre, 32); maps.c3 = &c3; a.keep_pre = 1; }
+  }
+  torch::Tensor partials, counters;
+  if (dense_is_cut(a, ctas)) {
+    partials = torch::empty({tok_partial_floats(ctas, a.tile_n)}, x.options().dtype(torch::kFloat32));
+    counters = torch::zeros({tok_counters(ctas)}, x.options().dtype(torch::kInt32));
+    a.partials = partials.data_ptr<float>();
+    a.counters = reinterpret_cast<unsigned int*>(counters.data_ptr<int>());
+  }
+  cuda_check(launch_dense_gemm(mode, ep.kind, maps, a, ctas, cur_stream()), "linear");
+}
+
+// out [N, K] = dz [T, N]^T . x [T, K]
+void dense_wgrad(const torch::Tensor& dz, const torch::Tensor& x, const torch::Tensor& out, uint64_t timeout_ns) {
+  const int64_t N = out.size(0), K = out.size(1);
+  const int ctas = sm_count(x) & ~1;
+  GemmArgs g{};
+  g.num_groups = 1;
+  g.dense_rows = static_cast<int>(x.size(0));
+  g.fixed_m_tiles = static_cast<int>((N + 255) / 256);
+  g.wide = gemm::wgrad_wide(g.fixed_m_tiles, static_cast<int>(K), ctas / 2, g.dense_rows);
+  g.tiles_n = static_cast<int>((K + 255) / 256) / (g.wide ? 2 : 1);
+  g.c_rows_per_group = static_cast<int>(N);
+  g.c = reinterpret_cast<__nv_bfloat16*>(out.data_ptr()); g.ldc = K;
+  g.status = dense_status();
+  TORCH_CHECK(g.status != nullptr, "linear: no status block on this device");
+  g.timeout_ns = timeout_ns;
+  cuda_check(launch_grouped_gemm_pair(GemmMode::kWgrad, GemmEpilogue::kStore, rows_map(dz, 64), rows_map(x, 64), rows_map(out, g.wide ? 32 : 128), nullptr, g, ctas, cur_stream()), "linear weight gradient");
+}
+
+struct LinearOut { torch::Tensor y, pre; };
+LinearOut linear_forward(const torch::Tensor& x, const torch::Tensor& weight, const OptTensor& bias, LinearKind kind, const OptTensor& residual, bool keep, uint64_t timeout_ns) {
+  const auto bf = torch::kBFloat16;
+  TORCH_CHECK(x.is_cuda() && x.scalar_type() == bf && x.dim() >= 1, "linear: x must be a bf16 CUDA tensor [..., inputs]");
+  TORCH_CHECK(weight.device() == x.device() && weight.scalar_type() == bf && weight.dim() == 2 && weight.size(1) == x.size(-1), "linear: weight must be bf16 [outputs, inputs] on x's device");
+  const int64_t N = weight.size(0), K = weight.size(1), cols = kind == LinearKind::kSwiGLU ? N / 2 : N;
+  TORCH_CHECK(K >= 8 && K % 8 == 0 && N >= 8 && N % 8 == 0, "linear: inputs and outputs must be multiples of 8 (rows of whole 16-byte words), got ", K, " and ", N);
+  TORCH_CHECK(K <= 1 << 24 && N <= 1 << 24, "linear: at most 2^24 inputs and outputs");
+  TORCH_CHECK(kind != LinearKind::kSwiGLU || (N % 256 == 0 && !bias.has_value() && !residual.has_value()),
+              "linear: swiglu takes weights in tiles of 128 gate rows and 128 up rows (outputs a multiple of 256), no bias and no residual");
+  TORCH_CHECK(!bias.has_value() || (bias->device() == x.device() && bias->scalar_type() == bf && bias->dim() == 1 && bias->size(0) == N && bias->is_contiguous()), "linear: bias must be contiguous bf16 [outputs] on x's device");
+  auto shape = x.sizes().vec();
+  shape.back() = cols;
+  TORCH_CHECK(!residual.has_value() || (residual->device() == x.device() && residual->scalar_type() == bf && residual->sizes() == at::IntArrayRef(shape)), "linear: residual must be bf16 with the output's shape, on x's device");
+  c10::cuda::CUDAGuard guard(x.device());
+  LinearOut o{torch::empty(shape, x.options()), {}};
+  const int64_t T = x.numel() / K;
+  TORCH_CHECK(T <= 1 << 30, "linear: more than 2^30 rows");
+  const bool pre = keep && kind != LinearKind::kNone;
+  if (pre) o.pre = torch::empty({T, N}, x.options());
+  if (T == 0) return o;
+  const torch::Tensor xm = tma_rows(x, K), wm = kind == LinearKind::kSwiGLU && !weight.is_contiguous() ? weight.contiguous() : tma_rows(weight, K), ym = o.y.view({T, cols});
+  torch::Tensor rm;
+  DenseEpilogue ep;
+  if (kind == LinearKind::kSwiGLU) {
+    ep.kind = GemmEpilogue::kSwiGLU;
+  } else if (bias.has_value() || residual.has_value() || kind != LinearKind::kNone) {
+    ep.kind = GemmEpilogue::kLinear;
+    ep.act = static_cast<Activation>(kind);
+    if (bias.has_value()) ep.bias = &*bias;
+    if (residual.has_value()) { rm = tma_rows(*residual, cols); ep.residual = &rm; }
+  }
+  if (pre) ep.pre = &o.pre;
+  dense_gemm(GemmMode::kForward, wm, xm, ym, ep, timeout_ns);
+  return o;
+}
+
+struct Linear : torch::autograd::Function<Linear> {
+  static variable_list forward(AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& weight, const OptTensor& bias, const OptTensor& residual, int64_t kind, int64_t timeout_ns) {
+    const bool through = x.requires_grad() || weight.requires_grad() || wants_grad(bias);   // the gradient goes past the activation
+    LinearOut o = linear_forward(x, weight, bias, static_cast<LinearKind>(kind), residual, through, timeout_ns);
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["kind"] = kind;
+    ctx->saved_data["timeout_ns"] = timeout_ns;
+    ctx->saved_data["bias"] = bias.has_value();
+    ctx->saved_data["residual"] = residual.has_value();
+    ctx->save_for_backward({weight.requires_grad() ? x : torch::Tensor(), x.requires_grad() ? weight : torch::Tensor(), o.pre});
+    ctx->saved_data["outputs"] = weight.size(0);
+    ctx->saved_data["inputs"] = weight.size(1);
+    ctx->saved_data["shape"] = x.sizes().vec();
+    return {o.y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(6);
+    if (!grads[0].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const bool has_bias = ctx->saved_data["bias"].toBool(), has_residual = ctx->saved_data["residual"].toBool();
+    const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1), want_b = has_bias && ctx->needs_input_grad(2), want_r = has_residual && ctx->needs_input_grad(has_bias ? 3 : 2);
+    const auto kind = static_cast<LinearKind>(ctx->saved_data["kind"].toInt());
+    const uint64_t timeout_ns = static_cast<uint64_t>(ctx->saved_data["timeout_ns"].toInt());
+    const int64_t N = ctx->saved_data["outputs"].toInt(), K = ctx->saved_data["inputs"].toInt();
+    if (want_r) out[3] = grads[0];
+    if (want_x || want_w || want_b) {
+      torch::NoGradGuard no_grad;
+      c10::cuda::CUDAGuard guard(grads[0].device());
+      const torch::Tensor dy = tma_rows(grads[0], kind == LinearKind::kSwiGLU ? N / 2 : N);
+      const int64_t T = dy.size(0);
+      TORCH_CHECK(dy.scalar_type() == torch::kBFloat16, "linear backward: the gradient must be bf16");
+      const auto shape = ctx->saved_data["shape"].toIntVector();
+      if (T == 0) {
+        if (want_x) out[0] = torch::zeros(shape, dy.options());
+        if (want_w) out[1] = torch::zeros({N, K}, dy.options());
+        if (want_b) out[2] = torch::zeros({N}, dy.options());
+      } else {
+        torch::Tensor dz = dy;
+        if (kind == LinearKind::kSwiGLU) {
+          const torch::Tensor d = dy.contiguous();
+          dz = torch::empty({T, N}, dy.options());
+          cuda_check(launch_swiglu_bwd(reinterpret_cast<const __nv_bfloat16*>(saved[2].data_ptr()), reinterpret_cast<const __nv_bfloat16*>(d.data_ptr()), reinterpret_cast<__nv_bfloat16*>(dz.data_ptr()),
+                                       T, static_cast<int>(N / 2), nullptr, cur_stream()), "linear backward: swiglu");
+        } else if (kind != LinearKind::kNone || want_b) {
+          const torch::Tensor d = dy.contiguous();
+          torch::Tensor partials;
+          const int blocks = linear_dz_blocks(static_cast<int>(T), static_cast<int>(N), sm_count(dy));
+          if (kind != LinearKind::kNone) dz = torch::empty({T, N}, dy.options());
+          if (want_b) {
+            out[2] = torch::empty({N}, dy.options());
+            partials = torch::empty({blocks, N}, dy.options().dtype(torch::kFloat32));
+          }
+          const auto ptr = [](const torch::Tensor& t) { return t.defined() ? reinterpret_cast<__nv_bfloat16*>(t.data_ptr()) : nullptr; };
+          cuda_check(launch_linear_dz(static_cast<Activation>(kind), ptr(d), ptr(saved[2]), kind != LinearKind::kNone ? ptr(dz) : nullptr, want_b ? partials.data_ptr<float>() : nullptr, static_cast<int>(T),
+                                      static_cast<int>(N), blocks, ptr(out[2]), cur_stream()), "linear backward: activation");
+        }
+        if (want_x) {
+          out[0] = torch::empty(shape, dy.options());
+          dense_gemm(GemmMode::kDgrad, tma_rows(saved[1], K), dz, out[0].view({T, K}), {}, timeout_ns);
+        }
+        if (want_w) {
+          out[1] = torch::empty({N, K}, dy.options());
+          dense_wgrad(dz, tma_rows(saved[0], K), out[1], timeout_ns);
+        }
+      }
+    }
+    variable_list in = grads;
+    in.insert(in.end(), saved.begin(), saved.end());
+    return once("linear", in, out);
+  }
+};
+torch::Tensor linear(const torch::Tensor& x, const torch::Tensor& weight, const OptTensor& bias, const OptTensor& residual, int kind, double timeout_s) {
+  TORCH_CHECK(kind >= 0 && kind <= 4 && timeout_s > 0, "linear: activation or limit");
+  const int64_t timeout_ns = static_cast<int64_t>(timeout_s * 1e9);
+  if (!recorded(x, weight, bias, residual)) return linear_forward(x, weight, bias, static_cast<LinearKind>(kind), residual, false, timeout_ns).y;
+  return Linear::apply(x, weight, bias, residual, kind, timeout_ns)[0];
+}
+// What a dense launch on the current device reported, which is forgotten with that: (code, site, detail, seen, want). Synchronises the current stream.
+py::tuple take_dense_status() {
+  DeviceStatus s{}, *d = dense_status();
+  TORCH_CHECK(d != nullptr, "linear: no status block on this device");
+  cuda_check(cudaStreamSynchronize(cur_stream()), "sync before status read");
+  cuda_check(cudaMemcpy(&s, d, sizeof(s), cudaMemcpyDeviceToHost), "read status");
+  if (s.code != 0) cuda_check(cudaMemset(d, 0, sizeof(s)), "clear status");
+  return py::make_tuple(s.code, s.site, s.detail, s.seen, s.want);
+}
+
 }  // namespace
 
 void bind_dense(py::module_& m) {
   m.def("add_rms_norm", &add_rms_norm, py::arg("x"), py::arg("weight"), py::arg("eps"), py::arg("residual"), py::arg("quantise"));
   m.def("balance_loss", &balance_loss, py::arg("logits"), py::arg("topk_idx"), py::arg("mask"), py::arg("sigmoid"));
+  m.def("linear", &linear, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("residual"), py::arg("kind"), py::arg("timeout_s"));
+  m.def("take_dense_status", &take_dense_status);
   m.def("dequantise_rows", &dequantise_rows, py::arg("q"), py::arg("scales"));
 }

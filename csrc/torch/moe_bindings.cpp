@@ -1,9 +1,10 @@
 // Bindings of the MoE kernels (routing, split scan, dispatch, grouped GEMM, combine).
-#include <cuda.h>
 #include <cuda_runtime.h>
 
+#include "../kernels/tile_walker.h"
 #include "../kernels/token_walker.h"
 #include "py_types.h"
+#include "tensor_maps.h"
 
 namespace py = pybind11;
 using namespace fastb;
@@ -24,21 +25,6 @@ void want_aligned(const torch::Tensor& t, c10::ScalarType dt, const char* name, 
   TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % word == 0, name, ": must start at a multiple of ", word, " bytes (clone a view that does not)");
 }
 void want16(const torch::Tensor& t, c10::ScalarType dt, const char* name) { want_aligned(t, dt, name, 16); }
-
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_tiled() {
-  static EncodeTiledFn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    cu_check(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q), "cudaGetDriverEntryPoint");
-    TORCH_CHECK(p != nullptr && q == cudaDriverEntryPointSuccess, "cuTensorMapEncodeTiled is not available in this driver");
-    return reinterpret_cast<EncodeTiledFn>(p);
-  }();
-  return fn;
-}
 
 // A 2-D bf16 row-major matrix [rows, cols] (row pitch in elements) tiled in boxes of
 // {box_cols, box_rows} with the 128-byte swizzle. box_cols must be 64 (one 128-byte line).
@@ -73,23 +59,6 @@ struct TensorMap2D {
     TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code ", static_cast<int>(r));
   }
 };
-
-CUtensorMap bf16_map(int rank, int64_t ptr, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
-  TORCH_CHECK(ptr % 16 == 0, "tensor map base must be 16-byte aligned");
-  for (int i = 0; i + 1 < rank; ++i) TORCH_CHECK(strides[i] % 16 == 0, "tensor map strides must be multiples of 16 bytes");
-  alignas(64) CUtensorMap m;
-  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-  CUresult r = encode_tiled()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, reinterpret_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code ", static_cast<int>(r));
-  return m;
-}
-CUtensorMap bf16_map_2d(const torch::Tensor& t, int box_rows) {
-  TORCH_CHECK(t.is_cuda() && t.scalar_type() == torch::kBFloat16 && t.dim() == 2 && t.stride(1) == 1, "expected a CUDA bf16 matrix with contiguous rows");
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(t.size(1)), static_cast<cuuint64_t>(t.size(0))}, strides[1] = {static_cast<cuuint64_t>(t.stride(0)) * 2};
-  const cuuint32_t box[2] = {64u, static_cast<cuuint32_t>(box_rows)};
-  return bf16_map(2, reinterpret_cast<int64_t>(t.data_ptr()), dims, strides, box);
-}
 
 // One contraction on fixed buffers (weights, tokens, outputs): everything about the launch of grouped_gemm_tokens that does not
 // change from call to call, the tensor maps above all.
@@ -515,6 +484,7 @@ void bind_moe(py::module_& m) {
         py::arg("status_ptr"), py::arg("timeout_ns"), py::arg("ctas"), py::arg("gate_counter_ptr"), py::arg("gate_target"), py::arg("pair"),
         py::arg("band_rows"), py::arg("map_c") = nullptr, py::arg("map_c2") = nullptr, py::arg("direct_epilogue") = false, py::arg("a_scales") = py::none(),
         py::arg("group_rows") = py::none(), py::arg("gate_tile_rows") = 0, py::arg("wide") = false);
+  m.def("wgrad_wide", &gemm::wgrad_wide, py::arg("row_tiles"), py::arg("columns"), py::arg("pairs"), py::arg("mean_rows"));
   m.def("grouped_gemm_smem_bytes", &grouped_gemm_smem_bytes);
   m.attr("ROUTE_TOKENS_PER_BLOCK") = kRouteTokensPerBlock;
   m.def("route_topk", &route_topk);

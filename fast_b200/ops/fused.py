@@ -1,6 +1,6 @@
 """Small fused autograd ops around the MoE block: embedding with a segmented-sum backward, the
 mean-square loss of a residual sum computed without materialising fp32 copies, and the dense side of a block (residual
-sum and RMS norm of rows, the router's balance loss)."""
+sum and RMS norm of rows, the router's balance loss, linear layers)."""
 from __future__ import annotations
 
 from typing import NamedTuple, Optional, Tuple
@@ -8,6 +8,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from .. import runtime
+from ..utils.config import CONFIG
 
 
 class _Embedding(torch.autograd.Function):
@@ -93,3 +94,20 @@ def balance_loss(logits: torch.Tensor, topk_idx: torch.Tensor, mask: Optional[to
     if scores not in ("softmax", "sigmoid"):
         raise ValueError(f"balance_loss: scores must be 'softmax' or 'sigmoid', got {scores!r}")
     return runtime.ext().balance_loss(logits, topk_idx, mask, scores == "sigmoid")
+
+
+_ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "swiglu": 4}
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``activation(x @ weight.T + bias) + residual`` in one kernel (tcgen05, fp32 accumulation, the result rounded once), with its backward pass.
+
+    x: bf16 [..., inputs]; ``weight``: bf16 [outputs, inputs], both sizes multiples of 8; ``bias``: bf16 [outputs]; ``residual``: bf16 with the
+    result's shape. ``activation``: None, "relu", "silu", "gelu" (z Phi(z)), or "swiglu": the weight holds tiles of 128 gate rows and the 128 up rows of
+    the same features, as an expert's does (``models.moe.interleave_gate_up``), outputs a multiple of 256, the result [..., outputs / 2] =
+    silu(gate) * up, without bias and residual. Any number of rows from none on; rows that are not contiguous, 16-byte aligned and a multiple of 16 bytes
+    apart are copied first. Where a gradient needs it, what the activation was taken of is kept in bf16. A device wait that gave up is
+    reported by ``ops.gemm.check()``."""
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"linear: activation must be one of {', '.join(map(repr, _ACTIVATIONS))}, got {activation!r}")
+    return runtime.ext().linear(x, weight, bias, residual, _ACTIVATIONS[activation], CONFIG.timeout_s)

@@ -41,10 +41,10 @@ def _st():
 
 
 def check() -> None:
-    """Raise if a GEMM launched through this module gave up on an mbarrier wait."""
-    code, site, detail, seen, want = _st().read()
-    if code:
-        raise runtime.CollectiveTimeout(code, site, detail, seen, want)
+    """Raise if a GEMM launched through this module, or a ``fused.linear`` on the current device, gave up on an mbarrier wait."""
+    for code, site, detail, seen, want in (_st().read(), runtime.ext().take_dense_status()):
+        if code:
+            raise runtime.CollectiveTimeout(code, site, detail, seen, want)
 
 
 def _tmap(t: torch.Tensor, box_rows: int):
@@ -145,12 +145,7 @@ def wide_columns(row_tiles: int, columns: int, pairs: int, mean_rows: int) -> bo
     them (4 to 2) 20.5 -> 18.5, 22.6 -> 20.5, 26.6 -> 26.6, 28.7 -> 28.7, 28.7 -> 30.7, 47 -> 49; 8 of 1024 x 1024 (2 to 1) 14.3 -> 14.3, 16.4 -> 16.4, 18.4 -> 20.5;
     2 of them (1 to 1) 12.3 -> 14.3, 12.3 -> 16.3, 14.3 -> 18.4. In a stream, W13 of 8 of 4096 x 14336 with 1536, 2048, 4096, 8192 rows 1920 -> 1892, 2486 -> 2447,
     4897 -> 4850, 12177 -> 11402; whole training steps of 8192 tokens (2048 rows) 20050 -> 20065."""
-    if columns % 512:
-        return False
-    narrow, wide = (-(-row_tiles * (columns // n) // pairs) for n in (256, 512))
-    if mean_rows < 512:
-        return narrow >= 4 and 14 * wide <= 8 * narrow
-    return (narrow >= 14 if mean_rows <= 640 else mean_rows >= 1536) and 50 * wide <= 26 * narrow
+    return runtime.ext().wgrad_wide(row_tiles, columns, pairs, mean_rows)
 
 
 def token_tile(epi: int, reduction: int, most_rows: int, mean_rows: int, groups: int, features: int, pairs: int) -> int:

@@ -22,6 +22,39 @@ def test_balance_loss_refuses_what_it_does_not_know():
         fused.balance_loss(logits, idx, scores="tanh")
 
 
+def test_linear_refuses_what_it_does_not_know():
+    x, w = torch.zeros(4, 64, dtype=BF), torch.zeros(16, 64, dtype=BF)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        fused.linear(x, w)
+    with pytest.raises(ValueError, match="activation"):
+        fused.linear(x, w, activation="tanh")
+
+
+@pytest.mark.gpu
+def test_linear_refusals():
+    x, w, b, r = (torch.zeros(*s, device="cuda", dtype=BF) for s in ((4, 64), (256, 64), (256,), (4, 256)))
+    for bad, match in [
+        (lambda: fused.linear(x.float(), w), "x must be"),
+        (lambda: fused.linear(x, w.float()), "weight"),
+        (lambda: fused.linear(x, w[:, :32]), "weight"),
+        (lambda: fused.linear(x, w.unsqueeze(0)), "weight"),
+        (lambda: fused.linear(x, w.cpu()), "weight"),
+        (lambda: fused.linear(x[:, :60], w[:, :60]), "multiples of 8"),
+        (lambda: fused.linear(x, w[:250]), "multiples of 8"),
+        (lambda: fused.linear(x[:, :0], w[:, :0]), "multiples of 8"),
+        (lambda: fused.linear(x, w[:0]), "multiples of 8"),
+        (lambda: fused.linear(x, w, bias=b.float()), "bias"),
+        (lambda: fused.linear(x, w, bias=b[:128]), "bias"),
+        (lambda: fused.linear(x, w, residual=r[:1]), "residual"),
+        (lambda: fused.linear(x, w, residual=r.float()), "residual"),
+        (lambda: fused.linear(x, w[:128], activation="swiglu"), "swiglu"),
+        (lambda: fused.linear(x, w, bias=b, activation="swiglu"), "swiglu"),
+        (lambda: fused.linear(x, w, residual=r[:, :128], activation="swiglu"), "swiglu"),
+    ]:
+        with pytest.raises(RuntimeError, match=match):
+            bad()
+
+
 @pytest.mark.gpu
 def test_balance_loss_refusals():
     logits, idx = torch.zeros(4, 8, device="cuda"), torch.zeros(4, 2, dtype=torch.int32, device="cuda")
