@@ -184,6 +184,23 @@ struct TokDenseMaps : TokGemmMaps {
 bool dense_is_cut(const TokDenseArgs& args, int ctas);
 // kForward: kStore, kSwiGLU, kLinear (maps.c2: the residual {64,32}); kDgrad: kStore.
 cudaError_t launch_dense_gemm(GemmMode mode, GemmEpilogue epi, const TokDenseMaps& maps, const TokDenseArgs& args, int ctas, cudaStream_t stream);
+// The same for few tokens (linear_few.cu): forward, any epilogue, no scratch.
+constexpr int kFewTokens = 128;   // of a tile
+struct FewArgs {
+  int T, columns;              // tokens, columns of the output
+  int red_blocks;              // 64-wide blocks of the reduction
+  const __nv_bfloat16* bias;   // [columns], 8-byte aligned, or null
+  const __nv_bfloat16* residual;   // [T, columns], rows residual_stride elements apart, 8-byte aligned, or null
+  long long residual_stride;
+  __nv_bfloat16* out;          // [T, columns]
+  __nv_bfloat16* pre;          // what the activation is taken of: [T, columns], SwiGLU [T, 2 columns]; or null
+  int n, stages, parts;        // set by the launcher: tokens of a tile, operand stages, CTAs that share a tile's reduction
+  DeviceStatus* status;
+  unsigned long long timeout_ns;
+};
+bool few_pays(int T, int columns, int red_blocks, bool swiglu, int sms);
+int few_box_rows(int T);       // rows of map_x's boxes {64, rows}; map_w's are {64,128}, SwiGLU {64,64}
+cudaError_t launch_linear_few(Activation act, bool swiglu, const CUtensorMap& map_w, const CUtensorMap& map_x, const FewArgs& args, int sms, cudaStream_t stream);
 // Where dense launches on the current device report a wait that gave up.
 DeviceStatus* dense_status();
 

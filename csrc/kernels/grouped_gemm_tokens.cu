@@ -121,16 +121,6 @@ __device__ __forceinline__ float as_f(uint32_t x) { return __uint_as_float(x); }
 // Tokens of a tile of n that accumulator `sub` holds.
 __device__ __forceinline__ int acc_n(int n, int sub) { return sub == 0 ? min(n, kTokAccN) : max(n - kTokAccN, 0); }
 
-// gelu(z) = z Phi(z)
-__device__ __forceinline__ float activate(Activation act, float z) {
-  switch (act) {
-    case Activation::kRelu: return fmaxf(z, 0.0f);
-    case Activation::kSilu: return silu(z);
-    case Activation::kGelu: return 0.5f * z * (1.0f + erff(z * 0.70710678f));
-    default: return z;
-  }
-}
-
 template <GemmMode MODE, GemmEpilogue EPI, int SUB, class Args>
 __global__ void __launch_bounds__(threads_for(SUB), 1)
 grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ TokMapsX map_x, const __grid_constant__ CUtensorMap map_c,
@@ -590,10 +580,14 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
             put(sb + 2 * kBox, chunk, h);
             put(sb + 2 * kBox, chunk + 2, h + 8);
           }
-          if (p.act != Activation::kNone) {
+          const auto each = [&](auto f) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(activate(p.act, as_f(r[i])));
-          }
+            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(f(as_f(r[i])));
+          };
+          // One branch a step: taken value by value it cost more than the activation (relu, 1235 x 1000 -> 2760: 31 us, 16 without).
+          if (p.act == Activation::kRelu) each([](float z) { return fmaxf(z, 0.0f); });
+          else if (p.act == Activation::kSilu) each([](float z) { return silu(z); });
+          else if (p.act == Activation::kGelu) each([](float z) { return gelu(z); });
           if (p.has_residual) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {

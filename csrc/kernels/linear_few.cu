@@ -1,0 +1,279 @@
+// A linear layer on a few tokens: out = act(x W^T + bias) + residual, or SwiGLU, in tiles of 128 rows of the weight by up to kFewTokens tokens.
+//
+// What bounds it: the weight's bytes. A cluster of CTAs has a tile and shares out the reduction; a CTA streams its part of the weight's
+// rows through shared memory (TMA) as operand A of M = 128 MMAs, the tokens are N (rounded up to 16), so a decode step does no more work
+// than its tokens are. The CTAs' fp32 sums meet in distributed shared memory: each CTA adds up an equal share of the tile's features, in the order
+// of the reduction, and finishes them (bias, activation, residual, store): no counters, no scratch in global memory, nothing to
+// clear beforehand, one launch. 1 token, weight from HBM: 4096 -> 14336 21 us (5.6 TB/s), 14336 -> 4096 21 us, 4096 -> 4096 8.2 us (4.1 TB/s; 3 us of a launch are setting up, the
+// first loads and the sums' way). Stages leave room for two CTAs an SM, so that the next launch is set up while this one runs.
+// SwiGLU: the 128 rows are 64 gate rows and the 64 up rows of the same features.
+#include <algorithm>
+
+#include "early_start.cuh"
+#include "gemm_common.cuh"
+
+namespace fastb {
+
+namespace {
+
+using namespace ptx;
+using namespace gemm;
+
+constexpr int kRows = 128;                       // of the weight, a tile
+constexpr int kThreads = 256;                    // two warps for every quarter of tensor memory
+constexpr int kMaxStages = 6;
+constexpr int kFewABytes = kRows * BK * 2;       // 16 KiB
+constexpr int kFewSmem = 110 * 1024;             // two CTAs an SM
+__host__ __device__ constexpr int few_stage(int n) { return kFewABytes + n * BK * 2; }
+
+struct __align__(8) FewCtl {
+  uint64_t full[kMaxStages], empty[kMaxStages], done;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+constexpr int few_stages(int n) { return std::min(kMaxStages, (kFewSmem - 1024 - static_cast<int>(sizeof(FewCtl))) / few_stage(n)); }
+// The CTA's sums [n][few_pitch] lie where the stages were. A warp reads several tokens' shares at once: the pitch puts them on different banks.
+__host__ __device__ constexpr int few_pitch(int mine) { return kRows + mine % 32; }
+__host__ __device__ constexpr int few_sums(int n) { return n * (kRows + 16) * 4; }
+constexpr int few_smem(int n) { return std::max(few_stages(n) * few_stage(n), few_sums(n)) + 1024 + static_cast<int>(sizeof(FewCtl)); }
+static_assert(few_stages(16) == 6 && few_stages(kFewTokens) >= 3 && few_smem(kFewTokens) <= kFewSmem, "stages at both ends of the range");
+
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 pack4(const float4& v) { return make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w)); }
+__device__ __forceinline__ float4 unpack4(const __nv_bfloat16* at) {
+  const uint2 v = *reinterpret_cast<const uint2*>(at);
+  const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.x)), b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.y));
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+template <Activation ACT>
+__device__ __forceinline__ float activated(float z) {
+  return ACT == Activation::kRelu ? fmaxf(z, 0.0f) : ACT == Activation::kSilu ? silu(z) : ACT == Activation::kGelu ? gelu(z) : z;
+}
+
+template <Activation ACT, bool SWIGLU, int PARTS>
+__global__ void __launch_bounds__(kThreads) linear_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const FewArgs p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int n = p.n, stage_size = few_stage(n), stages = p.stages;
+  float* sums = reinterpret_cast<float*>(tiles);                       // once the products are done
+  FewCtl* ctl = reinterpret_cast<FewCtl*>(tiles + max(stages * stage_size, few_sums(n)));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = static_cast<int>(cluster_cta_rank());
+  const int tile = blockIdx.x / PARTS, t0 = blockIdx.y * n, T = min(n, p.T - t0);   // rows of the weight, tokens
+  constexpr int F = SWIGLU ? kRows / 2 : kRows, MINE = F / PARTS, PITCH = few_pitch(MINE);   // features of a tile, and those that I finish
+  const uint32_t columns = n <= 32 ? 32 : n <= 64 ? 64 : 128;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) { mbar_init(&ctl->full[s], 1); mbar_init(&ctl->empty[s], 1); }
+    mbar_init(&ctl->done, 1);
+    ctl->abort_flag = 0;
+    mbar_fence_init();
+    prefetch_tmap(&map_w);
+    prefetch_tmap(&map_x);
+  }
+  if (warp == 1) { tmem_alloc(&ctl->tmem_base, columns); tmem_relinquish(); }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = ctl->tmem_base;
+  volatile int* abort_flag = &ctl->abort_flag;
+  grid_dependency_wait();
+  launch_dependents();
+  // This CTA's blocks of 64 of the reduction; a part has one at least.
+  const int kb0 = static_cast<int>(static_cast<long long>(p.red_blocks) * rank / PARTS), kb1 = static_cast<int>(static_cast<long long>(p.red_blocks) * (rank + 1) / PARTS), blocks = kb1 - kb0;
+  if (warp == 0) {
+    if (elect_one()) {
+      uint32_t ph = 0;
+      for (int i = 0, s = 0; i < blocks; ++i) {
+        if (i >= stages && !mbar_wait_bounded(&ctl->empty[s], ph ^ 1, abort_flag, p.status, 100 + s, p.timeout_ns)) break;
+        uint8_t* sa = tiles + s * stage_size;
+        const int k = (kb0 + i) * BK;
+        mbar_arrive_expect_tx(&ctl->full[s], static_cast<uint32_t>(stage_size));
+        if (SWIGLU) {   // tile t: 64 features from half t % 2 of the weight's 256-row tile t / 2
+          const int gate = tile / 2 * 256 + tile % 2 * 64;
+          tma_load_2d(sa, &map_w, k, gate, &ctl->full[s]);
+          tma_load_2d(sa + kFewABytes / 2, &map_w, k, gate + 128, &ctl->full[s]);
+        } else {
+          tma_load_2d(sa, &map_w, k, tile * kRows, &ctl->full[s]);
+        }
+        tma_load_2d(sa + kFewABytes, &map_x, k, t0, &ctl->full[s]);
+        if (++s == stages) { s = 0; ph ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint32_t idesc = make_idesc_bf16(kRows, n, false, false);
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int i = 0, s = 0; i < blocks; ++i) {
+        if (!(ok = mbar_wait_bounded(&ctl->full[s], ph, abort_flag, p.status, 300 + s, p.timeout_ns))) break;
+        tc_fence_after_sync();
+        const uint32_t sa = smem_u32(tiles + s * stage_size), sb = sa + kFewABytes;
+#pragma unroll
+        for (int k = 0; k < BK / UMMA_K; ++k)
+          mma_bf16_ss(tmem, make_smem_desc(sa + k * 32, 16, 1024), make_smem_desc(sb + k * 32, 16, 1024), idesc, (i | k) != 0 ? 1u : 0u);
+        mma_commit(&ctl->empty[s]);
+        if (++s == stages) { s = 0; ph ^= 1; }
+      }
+      if (ok) mma_commit(&ctl->done);
+    }
+  }
+  __syncwarp();
+  const bool ok = mbar_wait_bounded(&ctl->done, 0, abort_flag, p.status, 400, p.timeout_ns);
+  tc_fence_after_sync();
+  __syncthreads();
+  // All loads have landed and all products are done: the stages are free for the sums.
+  if (ok) {
+    const int feature = (warp & 3) * 32 + lane;
+    for (int c = (warp >> 2) * 32; c < n; c += 64) {
+      uint32_t r[32];
+      tmem_ld_32x32(tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + c, r);
+      tmem_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (c + i < T) sums[(c + i) * PITCH + feature] = __uint_as_float(r[i]);
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (PARTS > 1) cluster_sync_all();
+  if (ok) {
+    // Four features of a token at a time, U of them in flight: what this takes is the way to the peers' shared memory. Pairs of features one after
+    // the other, by half the threads, took 13 us instead of 8.4 for 48 x 2048 -> 7168.
+    constexpr int Q = MINE / 4, U = PARTS >= 8 ? 2 : 4;
+    const uint32_t base = smem_u32(sums);
+    for (int i0 = threadIdx.x; i0 < T * Q; i0 += U * kThreads) {
+      float4 z[U], u[SWIGLU ? U : 1];
+      const auto gather = [&](int add, float4* to) {
+        float4 w[U][PARTS];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+          const int i = min(i0 + j * kThreads, T * Q - 1);
+          const uint32_t at = base + static_cast<uint32_t>(i / Q * PITCH + rank * MINE + i % Q * 4 + add) * 4u;
+#pragma unroll
+          for (int q = 0; q < PARTS; ++q) w[j][q] = ld_cluster(PARTS > 1 ? map_to_cta(at, q) : at);
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+          to[j] = w[j][0];
+#pragma unroll
+          for (int q = 1; q < PARTS; ++q) { to[j].x += w[j][q].x; to[j].y += w[j][q].y; to[j].z += w[j][q].z; to[j].w += w[j][q].w; }
+        }
+      };
+      gather(0, z);
+      if (SWIGLU) gather(F, u);
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int i = i0 + j * kThreads, t = t0 + i / Q, f = rank * MINE + i % Q * 4, col = tile * F + f;
+        if (i >= T * Q || col >= p.columns) continue;
+        float4 v = z[j];
+        if (p.bias != nullptr) {
+          const float4 b = unpack4(p.bias + col);
+          v.x += b.x; v.y += b.y; v.z += b.z; v.w += b.w;
+        }
+        const long long at = static_cast<long long>(t) * p.columns + col;
+        if (SWIGLU) {
+          if (p.pre != nullptr) {
+            __nv_bfloat16* gu = p.pre + static_cast<long long>(t) * p.columns * 2 + tile / 2 * 256 + tile % 2 * 64 + f;
+            *reinterpret_cast<uint2*>(gu) = pack4(v);
+            *reinterpret_cast<uint2*>(gu + 128) = pack4(u[j]);
+          }
+          v.x = silu(v.x) * u[j].x; v.y = silu(v.y) * u[j].y; v.z = silu(v.z) * u[j].z; v.w = silu(v.w) * u[j].w;
+        } else {
+          if (p.pre != nullptr) *reinterpret_cast<uint2*>(p.pre + at) = pack4(v);
+          v.x = activated<ACT>(v.x); v.y = activated<ACT>(v.y); v.z = activated<ACT>(v.z); v.w = activated<ACT>(v.w);
+        }
+        if (p.residual != nullptr) {
+          const float4 r = unpack4(p.residual + t * p.residual_stride + col);
+          v.x += r.x; v.y += r.y; v.z += r.z; v.w += r.w;
+        }
+        *reinterpret_cast<uint2*>(p.out + at) = pack4(v);
+      }
+    }
+  }
+  __syncthreads();
+  if (PARTS > 1) cluster_sync_all();   // a peer may still read my sums
+  if (warp == 1) tmem_dealloc(tmem, columns);
+}
+
+}  // namespace
+
+// How many CTAs share a tile's reduction: as many as leave every CTA an SM, more where their parts are long (a CTA's stream alone does not fill an
+// SM's way to memory), eight only where there are few tiles or the parts are very long: a cluster of eight is harder to place, and its sums travel
+// further. us at 1, 2, 4, 8 parts: 32 tiles of 64 blocks (4096 -> 4096, 1 token) 14.6, 9.9, 8.2, 7.4, 64 tokens 20.5, 13.5, 10.7, 12.1; 56 tiles of 32
+// (2048 -> 7168), 1 token 8.4, 6.6, 6.9, 10.1; 112 tiles of 64 (4096 -> 14336), 33 tokens 26.2, 21.9, 27.9, 35.9; 224 tiles of 16 (1024 -> 28672),
+// 1 token 11.9, 14.8, 21.4, 32.7; 32 tiles of 224 (14336 -> 4096), 33 tokens 66.5, 37.6, 25.6, 23.2.
+int few_parts(int tiles, int red_blocks, int n, int sms) {
+  int parts = 1;
+  while (parts < 8 && (n > 32 ? 4 : 2) * parts <= red_blocks &&
+         ((parts == 4 ? 4 : 2) * tiles * parts <= sms || (tiles * parts < sms && red_blocks >= 48 * parts)))
+    parts *= 2;
+  return parts;
+}
+int few_box_rows(int T) {
+  const int tiles = (T + kFewTokens - 1) / kFewTokens;
+  return ((T + tiles - 1) / tiles + 15) / 16 * 16;
+}
+
+// Against the kernel with tiles of 256 features by up to 256 tokens (grouped_gemm_tokens.cu): ahead while its 128 x 128 tiles are no more than the SMs,
+// unless they are many and long. us, that kernel -> this one: 4096 -> 4096 with 1, 64, 128, 512 tokens 17.3 -> 8.2, 21.0 -> 10.7, 19.9 -> 12.7, 27.7 -> 20.4, with
+// 1024 (256 tiles) 28.9 -> 31.8; 4096 -> 14336 with 128 (112 tiles) 28.1 -> 26.3, 192 (224 tiles) 29.1 -> 31.7; 1024 -> 1024 with 1024 13.3 -> 7.4; 2048 -> 7168
+// with 256 19.2 -> 15.3, with 384 (168 tiles) 17.0 -> 18.2; 14336 -> 4096 with 256 (64 tiles) 55.9 -> 36.3, with 384 (96 tiles) 48.8 -> 54.7.
+bool few_pays(int T, int columns, int red_blocks, bool swiglu, int sms) {
+  const int per_tile = swiglu ? kRows / 2 : kRows;
+  const long long tiles = static_cast<long long>((columns + per_tile - 1) / per_tile) * ((T + kFewTokens - 1) / kFewTokens);
+  return 2 * tiles <= sms || (tiles <= sms && red_blocks <= 96);
+}
+
+cudaError_t launch_linear_few(Activation act, bool swiglu, const CUtensorMap& map_w, const CUtensorMap& map_x, const FewArgs& args, int sms, cudaStream_t stream) {
+  FewArgs a = args;
+  if (a.T < 1 || a.columns < 1 || a.red_blocks < 1 || a.status == nullptr || (swiglu && (act != Activation::kNone || a.columns % 128))) return cudaErrorInvalidValue;
+  const int per_tile = swiglu ? kRows / 2 : kRows, tiles = (a.columns + per_tile - 1) / per_tile;
+  a.n = few_box_rows(a.T);
+  a.stages = few_stages(a.n);
+  const int token_tiles = (a.T + a.n - 1) / a.n;
+  if (token_tiles > 65535) return cudaErrorInvalidValue;
+  a.parts = few_parts(tiles * token_tiles, a.red_blocks, a.n, sms);
+  const int smem = few_smem(a.n);
+  const auto go = [&](auto kern) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(tiles * a.parts, token_tiles);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = a.parts; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1] = early_start_attribute();
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kern, map_w, map_x, a);
+  };
+  const auto with = [&](auto act_c, auto swiglu_c) {
+    constexpr Activation ACT = decltype(act_c)::value;
+    constexpr bool SWIGLU = decltype(swiglu_c)::value;
+    switch (a.parts) {
+      case 1: return go(linear_few_kernel<ACT, SWIGLU, 1>);
+      case 2: return go(linear_few_kernel<ACT, SWIGLU, 2>);
+      case 4: return go(linear_few_kernel<ACT, SWIGLU, 4>);
+      case 8: return go(linear_few_kernel<ACT, SWIGLU, 8>);
+      default: return cudaErrorInvalidValue;
+    }
+  };
+  using std::integral_constant;
+  using none = integral_constant<Activation, Activation::kNone>;
+  cudaError_t e;
+  if (swiglu) e = with(none(), std::true_type());
+  else if (act == Activation::kRelu) e = with(integral_constant<Activation, Activation::kRelu>(), std::false_type());
+  else if (act == Activation::kSilu) e = with(integral_constant<Activation, Activation::kSilu>(), std::false_type());
+  else if (act == Activation::kGelu) e = with(integral_constant<Activation, Activation::kGelu>(), std::false_type());
+  else e = with(none(), std::false_type());
+  if (e == cudaSuccess) note_launch();
+  return e;
+}
+
+}  // namespace fastb

@@ -336,6 +336,21 @@ void dense_wgrad(const torch::Tensor& dz, const torch::Tensor& x, const torch::T
   cuda_check(launch_grouped_gemm_pair(GemmMode::kWgrad, GemmEpilogue::kStore, rows_map(dz, 64), rows_map(x, 64), rows_map(out, g.wide ? 32 : 128), nullptr, g, ctas, cur_stream()), "linear weight gradient");
 }
 
+// Forward on few rows.
+void dense_few(const torch::Tensor& weight, const torch::Tensor& x, const torch::Tensor& out, const DenseEpilogue& ep, uint64_t timeout_ns) {
+  const bool swiglu = ep.kind == GemmEpilogue::kSwiGLU;
+  FewArgs a{};
+  a.T = static_cast<int>(x.size(0)); a.columns = static_cast<int>(out.size(1));
+  a.red_blocks = static_cast<int>((weight.size(1) + 63) / 64);
+  const auto ptr = [](const torch::Tensor* t) { return t ? reinterpret_cast<__nv_bfloat16*>(t->data_ptr()) : nullptr; };
+  a.bias = ptr(ep.bias); a.residual = ptr(ep.residual); a.out = ptr(&out); a.pre = ptr(ep.pre);
+  a.residual_stride = ep.residual ? ep.residual->stride(0) : 0;
+  a.status = dense_status();
+  TORCH_CHECK(a.status != nullptr, "linear: no status block on this device");
+  a.timeout_ns = timeout_ns;
+  cuda_check(launch_linear_few(ep.act, swiglu, rows_map(weight, swiglu ? 64 : 128), rows_map(x, few_box_rows(a.T)), a, sm_count(x), cur_stream()), "linear");
+}
+
 struct LinearOut { torch::Tensor y, pre; };
 LinearOut linear_forward(const torch::Tensor& x, const torch::Tensor& weight, const OptTensor& bias, LinearKind kind, const OptTensor& residual, bool keep, uint64_t timeout_ns) {
   const auto bf = torch::kBFloat16;
@@ -358,18 +373,19 @@ LinearOut linear_forward(const torch::Tensor& x, const torch::Tensor& weight, co
   if (pre) o.pre = torch::empty({T, N}, x.options());
   if (T == 0) return o;
   const torch::Tensor xm = tma_rows(x, K), wm = kind == LinearKind::kSwiGLU && !weight.is_contiguous() ? weight.contiguous() : tma_rows(weight, K), ym = o.y.view({T, cols});
-  torch::Tensor rm;
+  torch::Tensor rm, bm;
   DenseEpilogue ep;
   if (kind == LinearKind::kSwiGLU) {
     ep.kind = GemmEpilogue::kSwiGLU;
   } else if (bias.has_value() || residual.has_value() || kind != LinearKind::kNone) {
     ep.kind = GemmEpilogue::kLinear;
     ep.act = static_cast<Activation>(kind);
-    if (bias.has_value()) ep.bias = &*bias;
+    if (bias.has_value()) { bm = reinterpret_cast<uintptr_t>(bias->data_ptr()) % 8 == 0 ? *bias : bias->clone(); ep.bias = &bm; }   // read in words of 8 bytes
     if (residual.has_value()) { rm = tma_rows(*residual, cols); ep.residual = &rm; }
   }
   if (pre) ep.pre = &o.pre;
-  dense_gemm(GemmMode::kForward, wm, xm, ym, ep, timeout_ns);
+  if (few_pays(static_cast<int>(T), static_cast<int>(cols), static_cast<int>((K + 63) / 64), kind == LinearKind::kSwiGLU, sm_count(x))) dense_few(wm, xm, ym, ep, timeout_ns);
+  else dense_gemm(GemmMode::kForward, wm, xm, ym, ep, timeout_ns);
   return o;
 }
 

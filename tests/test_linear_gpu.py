@@ -157,6 +157,9 @@ def test_strides_alignment_and_shapes():
         assert torch.equal(y, bf(x.double() @ other.double().t()))
         (g,) = torch.autograd.grad(y, leaf, r)
         assert torch.equal(g, bf(r.double().t() @ x.double()))
+    late = whole((N + 1,), 18)[1:]         # a bias that starts between two words
+    for rows in (x, x.repeat(3, 1)):
+        assert torch.equal(fused.linear(rows, w, bias=late), bf(rows.double() @ w.double().t() + late.double()))
     for res in (whole((N, T), 14).t(), whole((T, N + 5), 15)[:, 5:], whole((1, N), 16).expand(T, N)):
         assert torch.equal(fused.linear(x, w, residual=res), bf(x.double() @ w.double().t() + res.double()))
     y = fused.linear(x.view(5, 9, K), w, residual=r.view(5, 9, N))
