@@ -64,24 +64,35 @@ __global__ void swiglu_bwd_kernel(const uint4* __restrict__ gu, const uint4* __r
   }
 }
 
-__global__ void dequant_fp8_kernel(const uint2* __restrict__ q, const float* __restrict__ scales, uint4* __restrict__ out, long long rows, int H,
-                                   const int* __restrict__ rows_dev) {
+// H is a multiple of 128, so chunk i of 8 elements, counted through all rows, has scale i / 16. Bound by HBM; four chunks' loads in flight a thread.
+// 4096 rows of 7168: one chunk at a time, its row found by a division, 18.7 us.
+__global__ void __launch_bounds__(256) dequant_fp8_kernel(const uint2* __restrict__ q, const float* __restrict__ scales, uint4* __restrict__ out, long long rows, int H,
+                                                          const int* __restrict__ rows_dev) {
   if (rows_dev) rows = min(rows, static_cast<long long>(*rows_dev));
-  const int cpr = H / 8;
-  const long long total = rows * cpr;
-  for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < total; i += static_cast<long long>(gridDim.x) * blockDim.x) {
-    const long long r = i / cpr;
-    const int c = static_cast<int>(i % cpr);
-    const float sc = scales[r * (H / 128) + c / 16];
-    const uint2 v = q[i];
-    const unsigned char* b = reinterpret_cast<const unsigned char*>(&v);
-    float f[8];
+  constexpr int U = 4;
+  const long long total = rows * (H / 8), step = static_cast<long long>(gridDim.x) * blockDim.x * U;
+  for (long long i0 = static_cast<long long>(blockIdx.x) * blockDim.x * U + threadIdx.x; i0 < total; i0 += step) {
+    uint2 v[U];
+    float sc[U];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const __half_raw h = __nv_cvt_fp8_to_halfraw(b[k], __NV_E4M3);
-      f[k] = __half2float(*reinterpret_cast<const __half*>(&h)) * sc;
+    for (int u = 0; u < U; ++u) {
+      const long long i = min(i0 + u * static_cast<long long>(blockDim.x), total - 1);
+      v[u] = __ldg(q + i);
+      sc[u] = __ldg(scales + (i >> 4));
     }
-    out[i] = pack8(f);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long i = i0 + u * static_cast<long long>(blockDim.x);
+      if (i >= total) break;
+      const unsigned char* b = reinterpret_cast<const unsigned char*>(&v[u]);
+      float f[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const __half_raw h = __nv_cvt_fp8_to_halfraw(b[k], __NV_E4M3);
+        f[k] = __half2float(*reinterpret_cast<const __half*>(&h)) * sc[u];
+      }
+      out[i] = pack8(f);
+    }
   }
 }
 
@@ -535,7 +546,7 @@ cudaError_t launch_dequant_fp8(const unsigned char* q, const float* scales, __nv
                                cudaStream_t stream) {
   if (H % 128) return cudaErrorInvalidValue;
   if (rows == 0) return cudaSuccess;
-  dequant_fp8_kernel<<<grid_for(rows * H / 8), 256, 0, stream>>>(reinterpret_cast<const uint2*>(q), scales, reinterpret_cast<uint4*>(out), rows, H, rows_dev);
+  dequant_fp8_kernel<<<grid_for((rows * H / 8 + 3) / 4), 256, 0, stream>>>(reinterpret_cast<const uint2*>(q), scales, reinterpret_cast<uint4*>(out), rows, H, rows_dev);
   note_launch();
   return cudaGetLastError();
 }

@@ -28,8 +28,20 @@ __device__ __forceinline__ float silu(float x) { return x * sigmoid(x); }
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __expf(-x)); }
 __device__ __forceinline__ float silu(float x) { return x / (1.0f + __expf(-x)); }
 #endif
-// z Phi(z)
-__device__ __forceinline__ float gelu(float z) { return 0.5f * z * (1.0f + erff(z * 0.70710678f)); }
+// Phi(z), the normal distribution's integral, with e = exp(-z^2 / 2): Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26,
+// 1 - erf(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + 0.3275911 x), to 1.5e-7 for x >= 0; the other half by symmetry. The exponential serves the
+// density as well. (The general error function made the activation's backward pass a matter of arithmetic: 294 us for 8192 x 14336, where memory wants 107.)
+__device__ __forceinline__ float normal_integral(float z, float e) {
+  const float t = __fdividef(1.0f, fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.0f));
+  const float half = 0.5f * e * t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+  return z < 0.0f ? half : 1.0f - half;
+}
+// z Phi(z) and its derivative
+__device__ __forceinline__ float gelu(float z) { return z * normal_integral(z, __expf(-0.5f * z * z)); }
+__device__ __forceinline__ float gelu_slope(float z) {
+  const float e = __expf(-0.5f * z * z);
+  return fmaf(0.39894228f * z, e, normal_integral(z, e));
+}
 __device__ __forceinline__ uint4 pack8(const uint32_t* r) {
   return make_uint4(pack_bf16(__uint_as_float(r[0]), __uint_as_float(r[1])), pack_bf16(__uint_as_float(r[2]), __uint_as_float(r[3])),
                     pack_bf16(__uint_as_float(r[4]), __uint_as_float(r[5])), pack_bf16(__uint_as_float(r[6]), __uint_as_float(r[7])));

@@ -23,7 +23,7 @@ __device__ __forceinline__ float slope(float z) {
     const float s = gemm::sigmoid(z);
     return s * (1.0f + z * (1.0f - s));
   }
-  if (ACT == Activation::kGelu) return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * 0.39894228f * __expf(-0.5f * z * z);
+  if (ACT == Activation::kGelu) return gemm::gelu_slope(z);
   return 1.0f;
 }
 __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {

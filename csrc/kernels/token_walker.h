@@ -143,6 +143,12 @@ FASTB_HD inline int tok_band_tiles(int red_len, int m_tiles) {
 FASTB_HD inline int tok_back_tiles(int red_len, int band_tiles, int tile_n = kTokAccN) {
   return 2ll * red_len * tile_n * band_tiles > kTokBandBytes / 2 ? band_tiles : 1 << 30;
 }
+// Whether a launch takes tiles of 512 tokens instead of 256 (wide_tiles in ops/gemm.py says why and what was measured).
+inline bool tok_wide(bool swiglu, int reduction, int mean_rows, double waves) {
+  if (reduction < 4096) return false;
+  if (swiglu) return mean_rows >= 272 && mean_rows <= 368 && waves >= 5.5;
+  return static_cast<long long>(mean_rows) * reduction >= 16 << 20 && waves >= (reduction >= 8192 ? 3 : 6);
+}
 // Token tiles of a band of wide tiles (512 tokens). Same operands, 8192 rows, TFLOP/s at 2, 4, 8 and 16 tiles: reduction of 4096 (SwiGLU
 // backward) 1151, 1180, 1176, 1117; of 14336 1320, 1342, 1333, 1275; of 28672 1313, 1330, 1305, 1172.
 constexpr int kTokWideBandTiles = 4;

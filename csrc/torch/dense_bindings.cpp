@@ -282,6 +282,9 @@ void dense_gemm(GemmMode mode, const torch::Tensor& weight, const torch::Tensor&
   a.granule = 32;
   // Where all tokens fit a narrow tile, narrow tiles leave shared memory to the weights in flight.
   a.tile_n = a.dense_rows <= 64 ? 64 : a.dense_rows <= 128 ? 128 : 256;
+  if (ep.kind != GemmEpilogue::kLinear && a.tile_n == 256 &&
+      gemm::tok_wide(ep.kind == GemmEpilogue::kSwiGLU, static_cast<int>(reduction), a.dense_rows, (a.dense_rows + 511) / 512 * (features / 256.0) / (ctas / 2)))
+    a.tile_n = 512;
   a.band_tiles = gemm::tok_band(0, 64 * a.red_blocks, a.m_tiles, a.tile_n);
   a.back_tiles = gemm::tok_back_tiles(64 * a.red_blocks, a.band_tiles, std::max(a.tile_n, gemm::kTokAccN));
   a.status = dense_status();

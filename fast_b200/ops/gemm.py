@@ -121,11 +121,7 @@ def wide_tiles(epi: int, reduction: int, mean_rows: int, waves: float) -> bool:
     2794, 5912 -> 5426 / 3130 -> 3134, 6623 -> 6656. Below three waves (2 experts, 14336, 1536 and 3000 rows) 263 -> 279, 501 -> 494 / 310 -> 370,
     494 -> 554. Whole training steps of 1800 tokens (450 rows) with the data gradient of W13 wide 9920 -> 10190, of 12000, 16384, 32768 tokens
     against no wide tiles at all 26740 -> 25920, 34750 -> 33330, 66200 -> 61230. Shorter reductions lose at any size (plain, 3584 with 4096 rows 178 -> 189; a whole SwiGLU layer, 1024 with 444 rows 115 -> 122)."""
-    if reduction < 4096:
-        return False
-    if epi == SWIGLU:
-        return 272 <= mean_rows <= 368 and waves >= 5.5
-    return mean_rows * reduction >= 16 << 20 and waves >= (3 if reduction >= 8192 else 6)
+    return runtime.ext().tok_wide(epi == SWIGLU, reduction, mean_rows, waves)
 
 
 def _plan_key(mode: int, epi: int, granule: int, w: torch.Tensor, x: torch.Tensor, out: torch.Tensor, gu: Optional[torch.Tensor]) -> tuple:
