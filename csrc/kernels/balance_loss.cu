@@ -22,7 +22,7 @@ namespace fastb {
 namespace {
 
 using bf16 = __nv_bfloat16;
-constexpr int kFoldCtas = 8, kFoldThreads = 512;
+constexpr int kFoldCtas = 8, kFoldThreads = 1024;
 constexpr int kOneBlock = 4;     // rounds of the one-block launch
 
 __device__ __forceinline__ float as_logit(float v) { return v == v ? v : -INFINITY; }
@@ -149,47 +149,74 @@ __global__ void __launch_bounds__(P >= 16 ? 512 : 1024, 1) balance_kernel(const 
   }
 }
 
-// The blocks' sums and counts, added up by a cluster: CTA r has the experts r, r + 8, ..., a warp one of them at a time.
-__global__ void __cluster_dims__(kFoldCtas, 1, 1) __launch_bounds__(kFoldThreads) balance_fold_kernel(const BalanceArgs a, int blocks) {
+// The blocks' sums and counts, added up by a cluster: CTA r takes every eighth block's, all experts side by side; then an eighth of the experts, from
+// the CTAs' shared memory. Always in the same order. (An expert a warp, its lanes a row apart in memory, took 15 us for 296 blocks of 256 experts.)
+__global__ void __cluster_dims__(kFoldCtas, 1, 1) __launch_bounds__(kFoldThreads) balance_fold_kernel(const BalanceArgs a, int blocks, int across) {
   namespace cg = cooperative_groups;
-  __shared__ float s_part[kFoldThreads / 32], s_all[kFoldCtas];
-  __shared__ int s_live;
+  __shared__ float s_v[kFoldThreads], s_sum[kBalanceMaxExperts], s_part[kFoldThreads / 32], s_all[kFoldCtas];
+  __shared__ int s_n[kFoldThreads], s_count[kBalanceMaxExperts], s_live;
   const cg::cluster_group cluster = cg::this_cluster();
   const int rank = static_cast<int>(cluster.block_rank()), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int slices = kFoldThreads / across, slice = threadIdx.x / across;   // across: a power of two, as many experts as fit side by side
   grid_dependency_wait();
   launch_dependents();
-  float part = 0.0f;
-  for (int e = rank + kFoldCtas * warp; e < a.E; e += kFoldCtas * (kFoldThreads / 32)) {
+  for (int e0 = 0; e0 < a.E; e0 += across) {
+    const int e = e0 + threadIdx.x % across;
     float v = 0.0f;
     int n = 0;
-    for (int b = lane; b < blocks; b += 32) {
-      v += __ldcg(a.sums + static_cast<size_t>(b) * a.E + e);
-      n += __ldcg(a.chosen + static_cast<size_t>(b) * (a.E + 1) + e);
+    if (e < a.E) {
+#pragma unroll 8
+      for (int b = rank + kFoldCtas * slice; b < blocks; b += kFoldCtas * slices) {
+        v += __ldcg(a.sums + static_cast<size_t>(b) * a.E + e);
+        n += __ldcg(a.chosen + static_cast<size_t>(b) * (a.E + 1) + e);
+      }
     }
-    v = lanes_sum<32>(v);
-    n = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0) a.counts[e] = n;
-    part = fmaf(static_cast<float>(n), v, part);
+    s_v[threadIdx.x] = v;
+    s_n[threadIdx.x] = n;
+    __syncthreads();
+    if (slice == 0 && e < a.E) {
+      for (int q = 1; q < slices; ++q) { v += s_v[threadIdx.x + q * across]; n += s_n[threadIdx.x + q * across]; }
+      s_sum[e] = v;
+      s_count[e] = n;
+    }
+    __syncthreads();
   }
-  if (lane == 0) s_part[warp] = part;
-  if (rank == 0 && warp == 0) {
+  if (warp == 0) {
     int n = 0;
-    for (int b = lane; b < blocks; b += 32) n += __ldcg(a.chosen + static_cast<size_t>(b) * (a.E + 1) + a.E);
+    for (int b = rank + kFoldCtas * lane; b < blocks; b += kFoldCtas * 32) n += __ldcg(a.chosen + static_cast<size_t>(b) * (a.E + 1) + a.E);
     n = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0) { s_live = n; *a.live = n; }
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    part = 0.0f;
-    for (int w = 0; w < kFoldThreads / 32; ++w) part += s_part[w];
-    *cluster.map_shared_rank(s_all + rank, 0) = part;
+    if (lane == 0) s_live = n;
   }
   cluster.sync();
+  float part = 0.0f;
+  for (int e = rank + kFoldCtas * threadIdx.x; e < a.E; e += kFoldCtas * kFoldThreads) {
+    float v = 0.0f;
+    int n = 0;
+#pragma unroll
+    for (int r = 0; r < kFoldCtas; ++r) {
+      v += *cluster.map_shared_rank(s_sum + e, r);
+      n += *cluster.map_shared_rank(s_count + e, r);
+    }
+    a.counts[e] = n;
+    part = fmaf(static_cast<float>(n), v, part);
+  }
+  part = lanes_sum<32>(part);
+  if (lane == 0) s_part[warp] = part;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kFoldThreads / 32; ++w) part += s_part[w];
+    *cluster.map_shared_rank(s_all + rank, 0) = part;
+  }
+  int live = 0;
+  if (rank == 0 && threadIdx.x == 0)
+    for (int r = 0; r < kFoldCtas; ++r) live += *cluster.map_shared_rank(&s_live, r);
+  cluster.sync();   // nobody leaves while its shared memory is read
   if (rank == 0 && threadIdx.x == 0) {
     part = 0.0f;
     for (int r = 0; r < kFoldCtas; ++r) part += s_all[r];
-    const float n = static_cast<float>(max(s_live, 1));
+    const float n = static_cast<float>(max(live, 1));
     *a.loss = part / n * (static_cast<float>(a.E) / (static_cast<float>(a.K) * n));
+    *a.live = live;
   }
 }
 
@@ -260,21 +287,21 @@ cudaError_t with_shape(int E, bool is_bf16, bool sigmoid, F f) {
   return go(std::integral_constant<int, 32>(), std::integral_constant<int, 32>());
 }
 
-// Threads of a block of the one-block launch and of the others.
-int block_for(int E, bool alone) { return alone ? (E > 256 ? 512 : 1024) : 256; }
+// Threads of a block. Large ones: every block leaves sums that have to be added up (256 experts: 592 blocks of 256 threads took 7.7 + 11.5 us).
+int block_for(int E) { return E > 256 ? 512 : 1024; }
 
 }  // namespace
 
 int balance_blocks(const BalanceArgs& a, int sms) {
   const int per_warp = 32 / lanes_for(a.E);
-  if (a.T <= kOneBlock * (block_for(a.E, true) / 32) * per_warp) return 1;
-  const int per_block = block_for(a.E, false) / 32 * per_warp;
-  return std::min(2 * sms, (a.T + per_block - 1) / per_block);
+  const int per_block = block_for(a.E) / 32 * per_warp;
+  if (a.T <= kOneBlock * per_block) return 1;
+  return std::min(1024 / block_for(a.E) * sms, (a.T + per_block - 1) / per_block);
 }
 
 cudaError_t launch_balance(const BalanceArgs& a, int blocks, cudaStream_t stream) {
   if (a.T < 0 || a.E < 1 || a.E > kBalanceMaxExperts || a.K < 1 || blocks < 1 || (blocks > 1 && (a.sums == nullptr || a.chosen == nullptr))) return cudaErrorInvalidValue;
-  const int threads = block_for(a.E, blocks == 1);
+  const int threads = block_for(a.E);
   const size_t smem = static_cast<size_t>(a.E) * 4 * (1 + threads / 32);
   cudaError_t e = with_shape(a.E, a.logits_bf16 != 0, a.sigmoid != 0, [&](auto t, auto g, auto p, auto s) {
     auto kern = balance_kernel<decltype(t), decltype(g)::value, decltype(p)::value, decltype(s)::value>;
@@ -283,7 +310,9 @@ cudaError_t launch_balance(const BalanceArgs& a, int blocks, cudaStream_t stream
   });
   note_launch();
   if (e != cudaSuccess || blocks == 1) return e;
-  e = launch_early(balance_fold_kernel, dim3(kFoldCtas), kFoldThreads, 0, stream, a, blocks);
+  int across = 1;
+  while (across < a.E && across < kFoldThreads) across *= 2;
+  e = launch_early(balance_fold_kernel, dim3(kFoldCtas), kFoldThreads, 0, stream, a, blocks, across);
   note_launch();
   return e;
 }

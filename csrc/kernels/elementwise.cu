@@ -84,12 +84,14 @@ __global__ void __launch_bounds__(256) dequant_fp8_kernel(const uint2* __restric
     for (int u = 0; u < U; ++u) {
       const long long i = i0 + u * static_cast<long long>(blockDim.x);
       if (i >= total) break;
-      const unsigned char* b = reinterpret_cast<const unsigned char*>(&v[u]);
+      const unsigned short* b = reinterpret_cast<const unsigned short*>(&v[u]);
       float f[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const __half_raw h = __nv_cvt_fp8_to_halfraw(b[k], __NV_E4M3);
-        f[k] = __half2float(*reinterpret_cast<const __half*>(&h)) * sc[u];
+      for (int k = 0; k < 4; ++k) {
+        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(b[k], __NV_E4M3);
+        const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&h));
+        f[2 * k] = d.x * sc[u];
+        f[2 * k + 1] = d.y * sc[u];
       }
       out[i] = pack8(f);
     }
