@@ -294,6 +294,7 @@ struct NormGateBwdArgs {
   const int* topk_idx;          // [T, K]
   const float* topk_w;          // [T, K]
   const float* grad_w;          // [T, K] gradient of the routing weights
+  const float* grad_logits;     // [T, E] gradient of the logits from another consumer, or null
   const __nv_bfloat16* grad_hn; // [T, H] gradient of hn from its other consumer (the MoE input)
   int T, H, num_experts, K;
   __nv_bfloat16* grad_h;        // [T, H] out

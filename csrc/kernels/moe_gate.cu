@@ -186,17 +186,18 @@ __global__ void __launch_bounds__(kGateThreads) norm_gate_route_kernel(const Nor
 // a step ahead, and the tokens' few scalars are turned into logit gradients for 32 tokens at a time (read token by token,
 // they alone cost a dependent trip to L2 each: 3.6 us a token, 807 us for 32768). Narrow rows run in narrow blocks, several
 // per SM. Each block leaves its partial sums; fold_gate_grads_kernel adds them up in a fixed order.
-constexpr int kGateBwdBatch = 32;
-template <int C>
+// DENSE: every logit has a gradient of its own (a.grad_logits) beside what the selected ones get from the routing weights.
+constexpr int kGateBwdBatch = 32, kGateMaxE = 32;
+template <int C, bool DENSE>
 __global__ void __launch_bounds__(kGateBwdThreads) norm_gate_bwd_kernel(const NormGateBwdArgs a) {
   constexpr int B = C == 1 ? 2 : 1;   // tokens per step
   constexpr int kMaxK = 8;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float s_part[2][B][kGateBwdThreads / 32];
-  __shared__ float s_dl[kGateBwdBatch][kMaxK], s_rstd[kGateBwdBatch];
+  __shared__ float s_dl[kGateBwdBatch][DENSE ? kGateMaxE : kMaxK], s_rstd[kGateBwdBatch];
   __shared__ int s_ex[kGateBwdBatch][kMaxK];
   const int E = a.num_experts, H = a.H, K = a.K, nt = blockDim.x, nwarps = blockDim.x >> 5;
-  const int chunks = H / 8;
+  const int chunks = H / 8, terms = DENSE ? E : K;   // logits of a token that have a gradient
   uint4* s_gate = reinterpret_cast<uint4*>(smem);
   uint4* s_nw = s_gate + static_cast<size_t>(E) * chunks;
   float* s_dgate = reinterpret_cast<float*>(s_nw + chunks);  // [E][H]
@@ -230,6 +231,8 @@ __global__ void __launch_bounds__(kGateBwdThreads) norm_gate_bwd_kernel(const No
       // gradients of the selected logits of the next tokens: w = softmax(l_sel)  =>  dl_j = w_j (gw_j - sum_i w_i gw_i)
       __syncthreads();
       for (int q = threadIdx.x; q < kGateBwdBatch; q += nt) {
+        if (DENSE)
+          for (int e = 0; e < E; ++e) s_dl[q][e] = lt + q < n_tok ? __ldg(a.grad_logits + static_cast<long long>(t0 + lt + q) * E + e) : 0.0f;
         if (lt + q < n_tok) {
           const long long tj = static_cast<long long>(t0 + lt + q) * K;
           float w[kMaxK], gw[kMaxK], dotw = 0.0f;
@@ -241,12 +244,17 @@ __global__ void __launch_bounds__(kGateBwdThreads) norm_gate_bwd_kernel(const No
             if (j < K) {
               const int e = __ldg(a.topk_idx + tj + j);
               const bool in_range = e >= 0 && e < E;
-              s_dl[q][j] = in_range ? w[j] * (gw[j] - dotw) : 0.0f;
-              s_ex[q][j] = in_range ? e : 0;
+              const float dl = in_range ? w[j] * (gw[j] - dotw) : 0.0f;
+              if (DENSE) {
+                if (in_range) s_dl[q][e] += dl;
+              } else {
+                s_dl[q][j] = dl;
+                s_ex[q][j] = in_range ? e : 0;
+              }
             }
           s_rstd[q] = __ldg(a.rstd + t0 + lt + q);
         } else {
-          for (int j = 0; j < K; ++j) { s_dl[q][j] = 0.0f; s_ex[q][j] = 0; }
+          for (int j = 0; !DENSE && j < K; ++j) { s_dl[q][j] = 0.0f; s_ex[q][j] = 0; }
           s_rstd[q] = 0.0f;   // a token past the end adds nothing
         }
       }
@@ -276,9 +284,9 @@ __global__ void __launch_bounds__(kGateBwdThreads) norm_gate_bwd_kernel(const No
         unpack8(cg[b][ci], g);
 #pragma unroll
         for (int i = 0; i < 8; ++i) { xh[i] = x[i] * rstd; hn[i] = bf16_round(xh[i] * w[i]); }  // hn as the forward pass rounded it
-        for (int j = 0; j < K; ++j) {
+        for (int j = 0; j < terms; ++j) {
           const float dl = s_dl[q][j];
-          const int ex = s_ex[q][j];
+          const int ex = DENSE ? j : s_ex[q][j];
           float v[8];
           unpack8(s_gate[static_cast<size_t>(ex) * chunks + c], v);
           // a chunk's first four accumulators sit in the row's first half, the other four in its second
@@ -423,7 +431,8 @@ cudaError_t launch_norm_gate_bwd(const NormGateBwdArgs& a, int blocks, cudaStrea
   if (smem > 220 * 1024) return cudaErrorInvalidValue;
   if (a.T <= 0) return cudaSuccess;
   const int threads = std::min(kGateBwdThreads, (a.H / 8 + 31) / 32 * 32);
-  auto* kern = a.H / 8 > kGateBwdThreads ? norm_gate_bwd_kernel<2> : norm_gate_bwd_kernel<1>;
+  auto* kern = a.grad_logits != nullptr ? (a.H / 8 > kGateBwdThreads ? norm_gate_bwd_kernel<2, true> : norm_gate_bwd_kernel<1, true>)
+                                        : a.H / 8 > kGateBwdThreads ? norm_gate_bwd_kernel<2, false> : norm_gate_bwd_kernel<1, false>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return e;
   e = launch_early(kern, dim3(blocks), threads, smem, stream, a);

@@ -536,7 +536,7 @@ void bind_moe(py::module_& m) {
      py::arg("topk_w"), py::arg("slot_in_block"), py::arg("block_cnt"), py::arg("splits") = nullptr, py::arg("epoch") = 0);
   m.def("norm_gate_bwd", [](torch::Tensor h, torch::Tensor norm_w, torch::Tensor gate, torch::Tensor rstd, torch::Tensor topk_idx, torch::Tensor topk_w,
                             torch::Tensor grad_w, torch::Tensor grad_hn, torch::Tensor grad_h, torch::Tensor d_gate, torch::Tensor d_norm_w,
-                            c10::optional<torch::Tensor> residual) {
+                            c10::optional<torch::Tensor> residual, c10::optional<torch::Tensor> grad_logits) {
     want16(h, torch::kBFloat16, "h"); want16(norm_w, torch::kBFloat16, "norm_w"); want16(gate, torch::kBFloat16, "gate"); want(rstd, torch::kFloat32, "rstd");
     want(topk_idx, torch::kInt32, "topk_idx"); want(topk_w, torch::kFloat32, "topk_w"); want(grad_w, torch::kFloat32, "grad_w");
     want16(grad_hn, torch::kBFloat16, "grad_hn"); want16(grad_h, torch::kBFloat16, "grad_h");
@@ -557,13 +557,18 @@ void bind_moe(py::module_& m) {
       TORCH_CHECK(residual->sizes() == h.sizes(), "norm_gate_bwd: residual shape");
       a.residual = reinterpret_cast<const __nv_bfloat16*>(residual->data_ptr());
     }
+    if (grad_logits.has_value()) {
+      want(*grad_logits, torch::kFloat32, "grad_logits");
+      TORCH_CHECK(grad_logits->numel() == static_cast<int64_t>(a.T) * a.num_experts, "norm_gate_bwd: a gradient per logit");
+      a.grad_logits = grad_logits->data_ptr<float>();
+    }
     const int blocks = norm_gate_bwd_blocks(a.T, a.H, a.num_experts, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
     auto partials = torch::empty({blocks, a.num_experts + 1, a.H}, h.options().dtype(torch::kFloat32));
     a.partials = partials.data_ptr<float>();
     if (a.T == 0 && as_bf16) { d_gate.zero_(); d_norm_w.zero_(); }
     cu_check(launch_norm_gate_bwd(a, blocks, stream_now()), "norm_gate_bwd");
   }, py::arg("h"), py::arg("norm_w"), py::arg("gate"), py::arg("rstd"), py::arg("topk_idx"), py::arg("topk_w"), py::arg("grad_w"), py::arg("grad_hn"), py::arg("grad_h"),
-     py::arg("d_gate"), py::arg("d_norm_w"), py::arg("residual") = py::none());
+     py::arg("d_gate"), py::arg("d_norm_w"), py::arg("residual") = py::none(), py::arg("grad_logits") = py::none());
   m.def("dispatch_push", &dispatch_push, py::arg("heap"), py::arg("x"), py::arg("topk_idx"), py::arg("row_scale"), py::arg("slot_in_block"), py::arg("block_base"),
         py::arg("send_base"), py::arg("dest_row"), py::arg("compute_rows"), py::arg("fp8"), py::arg("recv_off"), py::arg("scale_off"), py::arg("arrive_off"),
         py::arg("entry_flags_off"), py::arg("entry_epoch"), py::arg("status"), py::arg("timeout_ns"), py::arg("ctas"), py::arg("send_list"),

@@ -25,6 +25,7 @@ class MoEConfig:
     fp8_dispatch: bool = False
     training: bool = True
     vocab: int = 0             # > 0: the block has a token embedding (and its gradient)
+    shared_inter: int = 0      # > 0: width of a dense SwiGLU expert that every token goes through, replicated
 
     def with_(self, **kw) -> "MoEConfig":
         return replace(self, **kw)
@@ -67,7 +68,9 @@ def memory_plan(cfg: MoEConfig, world: int, capacity_factor: float = 0.0) -> Dic
     workspace = 2 * cap * I + (2 * row if cfg.fp8_dispatch else 0)
     if cfg.training:
         workspace += 2 * cap * (2 * I + I + 2 * I)
-    params = el * 3 * H * I + H * cfg.num_experts + cfg.vocab * H
+    if cfg.shared_inter:   # the shared expert's activations, and in training its gate|up and their gradients
+        workspace += 2 * T * cfg.shared_inter * (1 if not cfg.training else 2 + 2 + 2)
+    params = el * 3 * H * I + H * cfg.num_experts + cfg.vocab * H + 3 * H * cfg.shared_inter
     weights = 2 * params
     grads = 2 * params if cfg.training else 0
     optimizer = 12 * params if cfg.training else 0
@@ -98,8 +101,9 @@ def flops_per_step(cfg: MoEConfig, world: int) -> Dict[str, float]:
     rows = cfg.tokens_per_rank * cfg.top_k
     fwd = 2.0 * rows * cfg.hidden * cfg.inter * 3
     total = fwd * (3 if cfg.training else 1)
+    shared = 2.0 * cfg.tokens_per_rank * cfg.hidden * cfg.shared_inter * 3 * (3 if cfg.training else 1)
     router = 2.0 * cfg.tokens_per_rank * cfg.hidden * cfg.num_experts * (3 if cfg.training else 1)
-    return {"expert_gemm_fwd": fwd, "expert_gemm_total": total, "router": router, "total": total + router}
+    return {"expert_gemm_fwd": fwd, "expert_gemm_total": total, "shared_expert": shared, "router": router, "total": total + shared + router}
 
 
 def step_roofline(cfg: MoEConfig, world: int, bf16_tflops: float, hbm_gbs: float, nvlink_gbs: float = 770.0) -> Dict[str, float]:
@@ -110,8 +114,8 @@ def step_roofline(cfg: MoEConfig, world: int, bf16_tflops: float, hbm_gbs: float
     f = flops_per_step(cfg, world)
     el = cfg.experts_per_rank(world)
     rows = cfg.tokens_per_rank * cfg.top_k
-    params = el * 3 * cfg.hidden * cfg.inter
-    gemm_ms = f["expert_gemm_total"] / (bf16_tflops * 1e12) * 1e3
+    params = el * 3 * cfg.hidden * cfg.inter + 3 * cfg.hidden * cfg.shared_inter
+    gemm_ms = (f["expert_gemm_total"] + f["shared_expert"]) / (bf16_tflops * 1e12) * 1e3
     # AdamW: bf16 grad + bf16 weight (read, write) + fp32 master, m, v (read, write) = 2 + 4 + 24 bytes per parameter
     adamw_ms = (params * 28 / (hbm_gbs * 1e9) * 1e3) if cfg.training else 0.0
     # rows that leave the GPU: dispatch + combine (and their transposes in training), (world - 1) / world of them

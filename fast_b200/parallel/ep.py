@@ -258,11 +258,15 @@ class ExpertParallel:
         return (self._gate_fits and 1 <= T <= self._C.ROUTE_TOKENS_PER_BLOCK and 2 * T * self.E * self.H <= 64 << 20 and self.E <= 256 and x.dtype == gate.dtype == torch.bfloat16
                 and x.is_contiguous() and gate.is_contiguous() and x.data_ptr() % 16 == 0 and gate.data_ptr() % 16 == 0 and T <= self.T)
 
-    def route_and_send(self, x: torch.Tensor, gate: torch.Tensor, bias: Optional[torch.Tensor] = None) -> RouteState:
+    def route_and_send(self, x: torch.Tensor, gate: torch.Tensor, bias: Optional[torch.Tensor] = None, quantised=None) -> RouteState:
         """``route_gate`` and ``dispatch``."""
         rs = self.route_gate(x, gate, bias)
-        self.dispatch(x, rs)
+        self.dispatch(x, rs) if quantised is None else self.dispatch(x, rs, quantised)
         return rs
+
+    def sends_quantised(self) -> bool:
+        """Whether ``dispatch`` sends e4m3 rows that are made in front of it (else the sending kernel makes them)."""
+        return self.fp8 and self.overlap
 
     def can_fuse_gate(self) -> bool:
         """Whether ``route_fused`` (RMSNorm + router logits + top-k in one kernel) covers this layer."""
@@ -287,7 +291,8 @@ class ExpertParallel:
         rs = self._route_state(topk_idx, topk_w, dest_row)
         return rs, hn, rstd, logits
 
-    def dispatch(self, x: torch.Tensor, rs: RouteState) -> None:
+    def dispatch(self, x: torch.Tensor, rs: RouteState, quantised=None) -> None:
+        """Send the rows to their experts. ``quantised``: ``(q, scales)`` of ``x`` as ``ops.fused.add_rms_norm`` makes them, where ``sends_quantised``."""
         if self._local is not None and gemm.USE_PAIR:
             self._local.dispatch(self.comm.heap, self.status, x, rs.topk_idx, rs.slot_in_block, rs.block_base, rs.send_base, rs.dest_row, self.timeout_ns, self.comm_ctas)
             return
@@ -304,15 +309,19 @@ class ExpertParallel:
             send_list = self.send_list
             if self.fp8:
                 # Sorted sending gives every (token, slot) entry a warp of its own: quantise each row once, entries copy bytes.
-                if self._xq_send is None:
+                if quantised is not None:
+                    xq, xs = quantised
+                elif self._xq_send is None:
                     self._xq_send = torch.empty(self.T, self.H, dtype=torch.uint8, device=x.device)
                     self._xs_send = torch.empty(self.T, self.H // 128, dtype=torch.float32, device=x.device)
-                xq, xs = self._xq_send, self._xs_send
-                C.quantise_rows(x, xq, xs, self.comm_ctas)
+                if xq is None:
+                    xq, xs = self._xq_send, self._xs_send
+                    C.quantise_rows(x, xq, xs, self.comm_ctas)
             ev = torch.cuda.Event()
             ev.record(torch.cuda.current_stream())
             self.side.wait_event(ev)
-            x.record_stream(self.side)
+            for t in (x, *(quantised or ())):
+                t.record_stream(self.side)
             ctx = torch.cuda.stream(self.side)
             ctx.__enter__()
         try:
