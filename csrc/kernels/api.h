@@ -427,7 +427,7 @@ struct RowNormArgs {
   float* rstd;                 // [T] out, or null
   int warps_per_row;           // set by the launcher
 };
-cudaError_t launch_row_norm(const RowNormArgs& a, cudaStream_t stream);
+cudaError_t launch_row_norm(const RowNormArgs& a, int sms, cudaStream_t stream);
 // Gradients: g = dy * weight, s = mean(g * h * rstd), dx = rstd * (g - h * rstd * s) + dh, dweight = sum over rows of dy * h * rstd.
 struct RowNormBwdArgs {
   const void* h;               // [T, H], rows h_stride elements apart

@@ -213,9 +213,11 @@ __global__ void __launch_bounds__(256) row_norm_any_kernel(const RowNormArgs a) 
 }
 
 // Backward: blocks walk the rows, a thread keeps the same columns for all of them and with them their part of the weight's gradient; the
-// next row's loads are under way while this one is worked on.
+// next row's loads are under way while this one is worked on. 16 columns a lane and up to 16 warps a row: with 32 columns the registers spill
+// (forward + backward of 8192 x 7168 216 us, this 156; 16384 x 4096 171, 96 % of the copy bandwidth; 16384 x 1024 52, 78 %).
+constexpr int kBwdWarps = 16;
 template <class T, class W, int C, bool DH>
-__global__ void __launch_bounds__(32 * warps_for(C)) row_norm_bwd_kernel(const RowNormBwdArgs a) {
+__global__ void __launch_bounds__(32 * kBwdWarps) row_norm_bwd_kernel(const RowNormBwdArgs a) {
   constexpr int N = Pack<T>::N;
   extern __shared__ float s_dw[];            // [H], blocks of several rows
   __shared__ float s_part[2][32];
@@ -311,6 +313,184 @@ __global__ void __launch_bounds__(32 * warps_for(C)) row_norm_bwd_kernel(const R
   }
 }
 
+// ---- rows staged in shared memory -------------------------------------------------------------------------------
+// Rows that do not start at 16-byte words or end inside one, and in the backward pass rows too long for the registers of a block (three inputs, the
+// next row's and the weight's gradient). A block keeps some rows ahead on their way to shared memory (cp.async: no registers), as the 16-byte words that
+// hold them; a thread has the same columns of every row, with their weights and sums in registers. VEC: rows are whole aligned words, a column group is
+// one of them; else it is one element, 32 a thread: many small blocks hide a row's way through two barriers better than few large ones (8 elements a
+// thread: 16384 x 4097 360 us). us forward + backward in bf16, element by element straight from memory -> this: 16384 x 4097 468 -> 295,
+// 32768 x 1001 268 -> 139, 4000 x 16383 882 -> 296; forward alone 190 -> 125, 112 -> 57, 216 -> 122.
+constexpr int kStagedSmem = 216 * 1024, kElements = 32;
+constexpr int staged_threads(bool vec) { return vec ? 1024 : 512; }   // at most
+
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from, int bytes) {   // 16 bytes, those past the first `bytes` as zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copy_wait(int left) {   // until at most `left` groups are under way
+  if (left <= 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
+  else if (left == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else asm volatile("cp.async.wait_group 2;" ::: "memory");
+}
+// All threads: the words that hold `n` elements from `row` on. What a word holds in front of the row or behind it is never used.
+template <class T>
+__device__ __forceinline__ void stage_row(unsigned char* to, const T* row, int n) {
+  const uintptr_t first = reinterpret_cast<uintptr_t>(row) & ~static_cast<uintptr_t>(15), end = reinterpret_cast<uintptr_t>(row + n);
+  const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+  for (int i = threadIdx.x; first + 16ull * i < end; i += blockDim.x) {
+    const uintptr_t src = first + 16ull * i;
+    copy_async(at + 16u * i, reinterpret_cast<const void*>(src), static_cast<int>(min(static_cast<unsigned long long>(end - src), 16ull)));
+  }
+}
+template <class T>
+__device__ __forceinline__ const T* staged(const unsigned char* stage, const T* row) {   // where the row starts in its stage
+  return reinterpret_cast<const T*>(stage + (reinterpret_cast<uintptr_t>(row) & 15));
+}
+__host__ __device__ constexpr int staged_bytes(int H, int size) { return (H * size + 15) / 16 * 16 + 16; }   // a row, wherever in a word it starts
+
+// IPT column groups a thread, `stages` (2 to 4) rows in shared memory.
+template <class T, class W, int IPT, bool VEC, bool DH>
+__global__ void __launch_bounds__(staged_threads(VEC)) row_norm_bwd_staged_kernel(const RowNormBwdArgs a, const int stages) {
+  constexpr int N = VEC ? Pack<T>::N : 1, kInputs = DH ? 3 : 2;
+  extern __shared__ __align__(16) unsigned char s_rows[];
+  __shared__ float s_part[2][32];
+  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5, groups = a.H / N, row_bytes = staged_bytes(a.H, sizeof(T));
+  grid_dependency_wait();
+  launch_dependents();
+  const T *h = static_cast<const T*>(a.h), *dy = static_cast<const T*>(a.dy), *dh = static_cast<const T*>(a.dh);
+  const auto request = [&](long long t, int s) {
+    if (t < a.T) {
+      unsigned char* to = s_rows + static_cast<size_t>(s) * kInputs * row_bytes;
+      stage_row(to, h + t * a.h_stride, a.H);
+      stage_row(to + row_bytes, dy + t * a.H, a.H);
+      if (DH) stage_row(to + 2 * row_bytes, dh + t * a.H, a.H);
+    }
+    copy_commit();
+  };
+  for (int s = 0; s + 1 < stages; ++s) request(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
+  float w[IPT][N], dw[IPT][N];
+#pragma unroll
+  for (int i = 0; i < IPT; ++i) {
+    const int c = threadIdx.x + i * blockDim.x;
+    if constexpr (VEC) load_weight<W, N>(a.weight, min(c, groups - 1), w[i]);
+    else w[i][0] = as_float<W>(static_cast<const W*>(a.weight)[min(c, groups - 1)]);
+#pragma unroll
+    for (int k = 0; k < N; ++k) dw[i][k] = 0.0f;
+  }
+  float next_r = blockIdx.x < a.T ? __ldg(a.rstd + blockIdx.x) : 0.0f;
+  int s = 0, buf = 0;
+  for (long long t = blockIdx.x; t < a.T; t += gridDim.x, buf ^= 1) {
+    copy_wait(stages - 2);
+    __syncthreads();   // this row is here, and the row before it has been read by all
+    request(t + static_cast<long long>(stages - 1) * gridDim.x, s == 0 ? stages - 1 : s - 1);
+    const unsigned char* at = s_rows + static_cast<size_t>(s) * kInputs * row_bytes;
+    const T *sh = staged(at, h + t * a.h_stride), *sy = staged(at + row_bytes, dy + t * a.H), *sd = DH ? staged(at + 2 * row_bytes, dh + t * a.H) : nullptr;
+    const auto get = [&](const T* row, int c, float (&f)[N]) {
+      if constexpr (VEC) Pack<T>::get(reinterpret_cast<const uint4*>(row)[c], f);
+      else f[0] = as_float<T>(row[c]);
+    };
+    const float r = next_r;
+    if (t + gridDim.x < a.T) next_r = __ldg(a.rstd + t + gridDim.x);
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
+      if (c >= groups) break;
+      float fh[N], fy[N];
+      get(sh, c, fh);
+      get(sy, c, fy);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const float p = fy[k] * (fh[k] * r);
+        dw[i][k] += p;
+        sum = fmaf(p, w[i][k], sum);
+      }
+    }
+    const float mean = row_sum(sum, s_part[buf], warp, warps) / static_cast<float>(a.H);
+    T* dx = static_cast<T*>(a.dx) + t * a.H;
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
+      if (c >= groups) break;
+      float fh[N], fy[N], fd[N];
+      get(sh, c, fh);
+      get(sy, c, fy);
+      if (DH) get(sd, c, fd);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        fy[k] = r * (fy[k] * w[i][k] - fh[k] * r * mean);
+        if (DH) fy[k] += fd[k];
+      }
+      if constexpr (VEC) __stcs(reinterpret_cast<uint4*>(dx) + c, Pack<T>::put(fy));
+      else dx[c] = as_type<T>(fy[0]);
+    }
+    if (++s == stages) s = 0;
+  }
+  float* out = a.partials + static_cast<size_t>(blockIdx.x) * a.H;
+#pragma unroll
+  for (int i = 0; i < IPT; ++i) {
+    const int c = threadIdx.x + i * blockDim.x;
+    if (c >= groups) break;
+#pragma unroll
+    for (int k = 0; k < N; ++k) out[c * N + k] = dw[i][k];
+  }
+}
+
+// Forward of rows that are not whole aligned words: an element a column group.
+template <class T, class W, bool RES>
+__global__ void __launch_bounds__(staged_threads(false)) row_norm_staged_kernel(const RowNormArgs a, const int stages) {
+  constexpr int kInputs = RES ? 2 : 1, IPT = kElements;
+  extern __shared__ __align__(16) unsigned char s_rows[];
+  __shared__ float s_part[2][32];
+  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5, row_bytes = staged_bytes(a.H, sizeof(T));
+  grid_dependency_wait();
+  launch_dependents();
+  const T *x = static_cast<const T*>(a.x), *res = static_cast<const T*>(a.residual);
+  const auto request = [&](long long t, int s) {
+    if (t < a.T) {
+      unsigned char* to = s_rows + static_cast<size_t>(s) * kInputs * row_bytes;
+      stage_row(to, x + t * a.x_stride, a.H);
+      if (RES) stage_row(to + row_bytes, res + t * a.residual_stride, a.H);
+    }
+    copy_commit();
+  };
+  for (int s = 0; s + 1 < stages; ++s) request(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
+  float w[IPT];
+#pragma unroll
+  for (int i = 0; i < IPT; ++i) w[i] = as_float<W>(static_cast<const W*>(a.weight)[min(static_cast<int>(threadIdx.x + i * blockDim.x), a.H - 1)]);
+  int s = 0, buf = 0;
+  for (long long t = blockIdx.x; t < a.T; t += gridDim.x, buf ^= 1) {
+    copy_wait(stages - 2);
+    __syncthreads();
+    request(t + static_cast<long long>(stages - 1) * gridDim.x, s == 0 ? stages - 1 : s - 1);
+    const unsigned char* at = s_rows + static_cast<size_t>(s) * kInputs * row_bytes;
+    const T *sx = staged(at, x + t * a.x_stride), *sr = RES ? staged(at + row_bytes, res + t * a.residual_stride) : nullptr;
+    float f[IPT], ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
+      f[i] = 0.0f;
+      if (c >= a.H) break;
+      f[i] = as_float<T>(sx[c]);
+      if (RES) {
+        const T v = as_type<T>(f[i] + as_float<T>(sr[c]));
+        static_cast<T*>(a.h)[t * a.H + c] = v;
+        f[i] = as_float<T>(v);
+      }
+      ss = fmaf(f[i], f[i], ss);
+    }
+    const float r = rsqrtf(row_sum(ss, s_part[buf], warp, warps) / static_cast<float>(a.H) + a.eps);
+    if (a.rstd != nullptr && threadIdx.x == 0) a.rstd[t] = r;
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
+      if (c >= a.H) break;
+      static_cast<T*>(a.y)[t * a.H + c] = as_type<T>(f[i] * r * w[i]);
+    }
+    if (++s == stages) s = 0;
+  }
+}
+
 template <class T, class W, bool DH>
 __global__ void __launch_bounds__(256) row_norm_bwd_any_kernel(const RowNormBwdArgs a) {
   extern __shared__ float s_dw[];            // [H], a column always by the same thread
@@ -361,16 +541,33 @@ __global__ void __launch_bounds__(1024) fold_columns_kernel(const float* __restr
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-// How a row is spread: C chunks of 16 bytes a lane, warps a row, rows a block; C = 0: element by element.
+// How a row is spread: C chunks of 16 bytes a lane, warps a row, rows a block; C = 0: in no such way.
 struct Spread { int C, wpr, rows; };
-Spread spread(int H, bool rows_bf16, bool vector, int most_c) {
+Spread spread(int H, bool rows_bf16, bool vector, int most_c, int most_warps) {
   const int n = rows_bf16 ? 8 : 4, chunks = H / n;
-  if (!vector || H % n || chunks == 0) return {0, 8, 1};
+  if (!vector || chunks == 0) return {0, 8, 1};
   for (int c = 1; c <= most_c; c *= 2) {
     const int wpr = (chunks + 32 * c - 1) / (32 * c);
-    if (wpr <= warps_for(c)) return {c, wpr, std::max(1, 8 / wpr)};
+    if (wpr <= 8 || (wpr <= most_warps && 2 * c > most_c)) return {c, wpr, std::max(1, 8 / wpr)};
   }
   return {0, 8, 1};
+}
+// How rows are staged: column groups a thread, threads, rows in shared memory, blocks an SM; stages = 0: they do not fit.
+struct Stages { int ipt, threads, stages, per_sm; size_t smem; };
+Stages staging(int H, int size, bool vector, int inputs) {
+  const int n = vector ? 16 / size : 1, groups = H / n, most = staged_threads(vector);
+  Stages g{vector ? size : kElements, 0, 0, 0, 0};   // vector: 16 columns a thread, or 32
+  if (vector && groups > g.ipt * most) g.ipt *= 2;
+  if (groups > g.ipt * most) return g;
+  g.threads = std::max(32, ((groups + g.ipt - 1) / g.ipt + 31) / 32 * 32);
+  const int row = inputs * staged_bytes(H, size);
+  // as many blocks as registers allow (at most 64 a thread, or 128), and at least two rows in each
+  for (g.per_sm = std::max(1, std::min(16, most / g.threads)); g.per_sm > 0; --g.per_sm) {
+    g.stages = std::min(4, kStagedSmem / g.per_sm / row);
+    if (g.stages >= 2) { g.smem = static_cast<size_t>(g.stages) * row; return g; }
+  }
+  g.stages = 0;
+  return g;
 }
 
 template <class F>
@@ -381,20 +578,30 @@ auto with_types(bool rows_bf16, bool weight_bf16, F f) {
 
 }  // namespace
 
-cudaError_t launch_row_norm(const RowNormArgs& args, cudaStream_t stream) {
+cudaError_t launch_row_norm(const RowNormArgs& args, int sms, cudaStream_t stream) {
   RowNormArgs a = args;
   if (a.T < 0 || a.H < 1 || a.H > kRowNormMaxHidden || (a.q != nullptr && (a.H % 128 || a.scales == nullptr))) return cudaErrorInvalidValue;
   if (a.T == 0) return cudaSuccess;
   const int n = a.rows_bf16 ? 8 : 4;
-  const bool vector = aligned16(a.x) && a.x_stride % n == 0 && aligned16(a.residual) && a.residual_stride % n == 0 && aligned16(a.weight);
-  const Spread sp = spread(a.H, a.rows_bf16 != 0, vector, 8);
+  const bool vector = a.H % n == 0 && aligned16(a.x) && a.x_stride % n == 0 && aligned16(a.residual) && a.residual_stride % n == 0 && aligned16(a.weight);
+  const Spread sp = spread(a.H, a.rows_bf16 != 0, vector, 8, 16);
   a.warps_per_row = sp.wpr;
   const int block = 32 * sp.wpr * sp.rows, grid = (a.T + sp.rows - 1) / sp.rows;
+  const Stages st = sp.C == 0 && a.q == nullptr ? staging(a.H, a.rows_bf16 ? 2 : 4, false, a.residual ? 2 : 1) : Stages{};
   const cudaError_t e = with_types(a.rows_bf16 != 0, a.weight_bf16 != 0, [&](auto t, auto w) {
     using T = decltype(t);
     using W = decltype(w);
     const auto go = [&](auto res, auto quant) {
       constexpr bool RES = decltype(res)::value, QUANT = decltype(quant)::value;
+      if constexpr (!QUANT) {
+        if (st.stages > 0) {
+          const auto with = [&](auto kern) {
+            const cudaError_t err = allow_smem(kern, st.smem);
+            return err != cudaSuccess ? err : launch_early(kern, dim3(std::min(a.T, sms * st.per_sm)), st.threads, st.smem, stream, a, st.stages);
+          };
+          return with(row_norm_staged_kernel<T, W, RES>);
+        }
+      }
       switch (sp.C) {
         case 1: return launch_early(row_norm_kernel<T, W, 1, RES, QUANT>, dim3(grid), block, 0, stream, a);
         case 2: return launch_early(row_norm_kernel<T, W, 2, RES, QUANT>, dim3(grid), block, 0, stream, a);
@@ -411,24 +618,29 @@ cudaError_t launch_row_norm(const RowNormArgs& args, cudaStream_t stream) {
 }
 
 namespace {
-Spread bwd_spread(const RowNormBwdArgs& a) {
+struct BwdPlan { Spread sp; Stages st; bool vector; };
+BwdPlan bwd_plan(const RowNormBwdArgs& a) {
   const int n = a.rows_bf16 ? 8 : 4;
-  const bool vector = aligned16(a.h) && a.h_stride % n == 0 && aligned16(a.dy) && aligned16(a.dh) && aligned16(a.weight);
-  return spread(a.H, a.rows_bf16 != 0, vector, 4);
+  const bool vector = a.H % n == 0 && aligned16(a.h) && a.h_stride % n == 0 && aligned16(a.dy) && aligned16(a.dh) && aligned16(a.weight);
+  const Spread sp = spread(a.H, a.rows_bf16 != 0, vector, a.rows_bf16 ? 2 : 4, kBwdWarps);   // 16 columns a lane
+  return {sp, sp.C == 0 ? staging(a.H, a.rows_bf16 ? 2 : 4, vector, a.dh ? 3 : 2) : Stages{}, vector};
 }
 }  // namespace
 
 int row_norm_bwd_blocks(const RowNormBwdArgs& a, int sms) {
-  const Spread sp = bwd_spread(a);
-  // What an SM holds at once: four blocks of eight warps, or two of 16; element by element, what the sums in shared memory leave.
-  const int per_sm = std::max(1, sp.C > 0 ? 32 / (sp.wpr * sp.rows) : std::min(8, 200 * 1024 / (4 * a.H)));
-  return std::max(1, std::min(sms * per_sm, (a.T + 4 * sp.rows - 1) / (4 * sp.rows)));   // four rows at least for every partial sum
+  const BwdPlan p = bwd_plan(a);
+  // What an SM holds at once; element by element, what the sums in shared memory leave.
+  const int rows = p.sp.C > 0 ? p.sp.rows : 1, per_sm = p.sp.C > 0 ? std::max(1, (p.sp.C * (a.rows_bf16 ? 8 : 4) <= 8 ? 32 : 16) / (p.sp.wpr * rows)) : p.st.stages > 0 ? p.st.per_sm : std::max(1, std::min(8, 200 * 1024 / (4 * a.H)));
+  const int least = a.T <= 8 * sms ? 2 : 4;   // rows for every partial sum
+  return std::max(1, std::min(sms * per_sm, (a.T + least * rows - 1) / (least * rows)));
 }
 
 cudaError_t launch_row_norm_bwd(const RowNormBwdArgs& args, int blocks, cudaStream_t stream) {
   RowNormBwdArgs a = args;
   if (a.T < 1 || a.H < 1 || a.H > kRowNormMaxHidden || blocks < 1 || a.partials == nullptr) return cudaErrorInvalidValue;
-  const Spread sp = bwd_spread(a);
+  const BwdPlan plan = bwd_plan(a);
+  const Spread sp = plan.sp;
+  const Stages st = plan.st;
   a.warps_per_row = sp.wpr;
   cudaError_t e = with_types(a.rows_bf16 != 0, a.weight_bf16 != 0, [&](auto t, auto w) {
     using T = decltype(t);
@@ -436,6 +648,15 @@ cudaError_t launch_row_norm_bwd(const RowNormBwdArgs& args, int blocks, cudaStre
     const auto go = [&](auto dh) {
       constexpr bool DH = decltype(dh)::value;
       const int block = 32 * sp.wpr * sp.rows;
+      if (st.stages > 0) {
+        const auto with = [&](auto kern) {
+          const cudaError_t err = allow_smem(kern, st.smem);
+          return err != cudaSuccess ? err : launch_early(kern, dim3(blocks), st.threads, st.smem, stream, a, st.stages);
+        };
+        if (!plan.vector) return with(row_norm_bwd_staged_kernel<T, W, kElements, false, DH>);
+        constexpr int kWords = sizeof(T);   // 16 columns
+        return st.ipt == kWords ? with(row_norm_bwd_staged_kernel<T, W, kWords, true, DH>) : with(row_norm_bwd_staged_kernel<T, W, 2 * kWords, true, DH>);
+      }
       const size_t smem = sp.C == 0 || sp.rows > 1 ? sizeof(float) * a.H : 0;
       const auto with = [&](auto kern, int threads) {
         const cudaError_t err = allow_smem(kern, smem);
@@ -444,7 +665,9 @@ cudaError_t launch_row_norm_bwd(const RowNormBwdArgs& args, int blocks, cudaStre
       switch (sp.C) {
         case 1: return with(row_norm_bwd_kernel<T, W, 1, DH>, block);
         case 2: return with(row_norm_bwd_kernel<T, W, 2, DH>, block);
-        case 4: return with(row_norm_bwd_kernel<T, W, 4, DH>, block);
+        case 4:
+          if constexpr (sizeof(T) == 4) return with(row_norm_bwd_kernel<T, W, 4, DH>, block);
+          else return cudaErrorInvalidValue;
         default: return with(row_norm_bwd_any_kernel<T, W, DH>, 256);
       }
     };

@@ -91,7 +91,7 @@ Norm row_norm(const torch::Tensor& x, const torch::Tensor& weight, double eps, c
     rstd = torch::empty({xm.size(0)}, x.options().dtype(torch::kFloat32));
     a.rstd = rstd.data_ptr<float>();
   }
-  cuda_check(launch_row_norm(a, cur_stream()), "add_rms_norm");
+  cuda_check(launch_row_norm(a, sm_count(x), cur_stream()), "add_rms_norm");
   return {y, h, q, scales, rstd};
 }
 

@@ -37,7 +37,7 @@ def check_y(y, want, dtype):
 
 @pytest.mark.parametrize("wtype", [BF, F32])
 @pytest.mark.parametrize("dtype", [BF, F32])
-@pytest.mark.parametrize("T,H", [(1, 1), (1, 4096), (3, 7), (5, 128), (17, 1001), (64, 1000), (33, 2048), (9, 7168), (7, 16384), (4, 32768), (3, 49152), (300, 264)])
+@pytest.mark.parametrize("T,H", [(1, 1), (1, 4096), (3, 7), (5, 128), (17, 1001), (64, 1000), (33, 2048), (9, 7168), (7, 16384), (4, 32768), (3, 49152), (300, 264), (1300, 1003), (700, 8200), (160, 16383), (90, 9000), (640, 4104)])
 def test_forward_and_gradients(T, H, dtype, wtype):
     x, res = rand((T, H), dtype, 1), rand((T, H), dtype, 2, 2.0)
     w = (1 + rand((H,), F32, 3, 0.2)).to(wtype)
