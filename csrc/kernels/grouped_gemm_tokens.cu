@@ -57,10 +57,12 @@ constexpr int kABytes = kHalfM * BK * 2;          // 16 KiB
 __host__ __device__ constexpr int stage_bytes(int tile_n) { return kABytes + tile_n / 2 * BK * 2; }   // B: half of the widest tile's tokens
 // Warps: TMA, MMA, then four epilogue warps; for wide tiles two groups of four from warp 4 on, whose registers (they hold
 // accumulators) come from the first four.
+// With one weight matrix (dense) there are two groups for tiles of one accumulator too: a launch is often one round of tiles, whose way out nothing hides.
 __host__ __device__ constexpr int first_epilogue_warp(int sub) { return sub == 1 ? 2 : 4; }
-__host__ __device__ constexpr int threads_for(int sub) { return 32 * first_epilogue_warp(sub) + 128 * sub; }
+__host__ __device__ constexpr int groups_for(int sub, bool dense) { return dense ? 2 : sub; }
+__host__ __device__ constexpr int threads_for(int sub, bool dense) { return 32 * first_epilogue_warp(sub) + 128 * groups_for(sub, dense); }
 constexpr int kLaunchRegs = 168, kOtherRegs = 72, kEpilogueRegs = 216;   // a thread, wide tiles
-static_assert(kOtherRegs + 2 * kEpilogueRegs <= 3 * kLaunchRegs && threads_for(2) * kLaunchRegs <= 65536, "what the epilogue takes, the others have given");
+static_assert(kOtherRegs + 2 * kEpilogueRegs <= 3 * kLaunchRegs && threads_for(2, false) * kLaunchRegs <= 65536, "what the epilogue takes, the others have given");
 constexpr int kStepTokens = 32;                   // tokens per epilogue step = rows of a TMA store
 constexpr int kBox = kStepTokens * 128;           // 4 KiB: 32 tokens x 64 features
 
@@ -122,10 +124,11 @@ __device__ __forceinline__ float as_f(uint32_t x) { return __uint_as_float(x); }
 __device__ __forceinline__ int acc_n(int n, int sub) { return sub == 0 ? min(n, kTokAccN) : max(n - kTokAccN, 0); }
 
 template <GemmMode MODE, GemmEpilogue EPI, int SUB, class Args>
-__global__ void __launch_bounds__(threads_for(SUB), 1)
+__global__ void __launch_bounds__(threads_for(SUB, tok_dense<Args>::value), 1)
 grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ TokMapsX map_x, const __grid_constant__ CUtensorMap map_c,
                            const __grid_constant__ CUtensorMap map_c2, const __grid_constant__ CUtensorMap map_c3, const Args p) {
   constexpr bool DENSE = tok_dense<Args>::value;
+  constexpr int GROUPS = groups_for(SUB, DENSE);   // of epilogue warps
   static_assert(EPI != GemmEpilogue::kLinear || (DENSE && SUB == 1 && MODE == GemmMode::kForward), "one weight matrix, tiles of one accumulator");
   constexpr bool A_MN = MODE == GemmMode::kDgrad;
   constexpr int kRing = epi_boxes(EPI) * kBox;
@@ -141,8 +144,8 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) { mbar_init(&ctl->full[s], 1); mbar_init(&ctl->empty[s], 1); }
-    for (int a = 0; a < kAccStages; ++a) { mbar_init(&ctl->acc_full[a], 1); mbar_init(&ctl->acc_empty[a], 2 * 4 * SUB); mbar_init(&ctl->epi_load[a], 1); }
-    mbar_init(&ctl->meet, 4 * SUB);
+    for (int a = 0; a < kAccStages; ++a) { mbar_init(&ctl->acc_full[a], 1); mbar_init(&ctl->acc_empty[a], 2 * 4 * GROUPS); mbar_init(&ctl->epi_load[a], 1); }
+    mbar_init(&ctl->meet, 4 * GROUPS);
     ctl->abort_flag = 0;
     mbar_fence_init();
     prefetch_tmap(&map_w);
@@ -329,12 +332,12 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
   } else {
     if constexpr (SUB == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegs));
     // ---------------- epilogue (both CTAs, each for its 128 features) ----------------
-    // A wide tile has two groups of four warps, which take the 32-token steps in turn: a group owns half of the ring, and one group
+    // Two groups of four warps, where there are two, take the 32-token steps in turn: a group owns half of the ring, and one group
     // converts while the other's stores and loads are under way.
     const int quarter = warp & 3, group = (warp - first_epilogue_warp(SUB)) >> 2;
     const int et = (threadIdx.x - 32 * first_epilogue_warp(SUB)) & 127;   // 0..127 in the group
     const bool issuer = et == 0;
-    const int first_step = SUB == 1 ? 0 : group;
+    const int first_step = GROUPS == 1 ? 0 : group;
     grid_dependency_wait();   // what is written below may still be read by earlier kernels
     launch_dependents();
     // The other arrival counters are cleared for the next launch; this launch's are back at zero once all parts have arrived.
@@ -344,7 +347,7 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
     bool ok = true;
     // All epilogue warps, twice per part of a tile (phases 0 and 1 of the barrier). Two groups wait with a limit: one of them may have given up.
     auto meet = [&](uint32_t phase) {
-      if (SUB == 1) { epi_bar(); return; }
+      if (GROUPS == 1) { epi_bar(); return; }
       __syncwarp();
       if (!ok) return;
       if (lane == 0) mbar_arrive(&ctl->meet);
@@ -376,7 +379,7 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
           if (!ok) break;
           float4* out = reinterpret_cast<float4*>(p.partials + ((static_cast<size_t>(pair * 2 + (sg.part == 0 ? 1 : 0)) * 2 + cta) * SUB + sub) * kTokPartialFloats) + et;
           const uint32_t t_row = acc_row(sub);
-          for (int st = first_step; st < steps_of(sub); st += SUB) {
+          for (int st = first_step; st < steps_of(sub); st += GROUPS) {
             uint32_t r[32];
             tmem_ld_16x32(t_row + st * kStepTokens, r);
             tmem_ld_16x32(t_row + (16u << 16) + st * kStepTokens, r + 16);
@@ -434,9 +437,9 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
         for (int jj = 0; jj < 2; ++jj) stmatrix_trans(box_row(box, lane, jj, chunk), h[4 * jj], h[4 * jj + 1], h[4 * jj + 2], h[4 * jj + 3]);
       };
       auto acquire = [&]() {
-        if (issuer) bulk_wait_read<SUB == 1 ? 1 : 0>();   // the stores that read this half of the ring are done with it
+        if (issuer) bulk_wait_read<GROUPS == 1 ? 1 : 0>();   // the stores that read this half of the ring are done with it
         group_bar(group);
-        return ring + (SUB == 1 ? ring_n & 1u : group) * kRing;
+        return ring + (GROUPS == 1 ? ring_n & 1u : group) * kRing;
       };
       auto load_gu = [&](int sub, int st) {                    // issuer only: gate and up of my 128 features, saved by the forward pass
         uint8_t* b = ring + (st & 1) * kRing;
@@ -448,7 +451,7 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
         if (!issuer) return;
         bulk_wait_read<0>();
         if (first_step < steps_of(sub)) load_gu(sub, first_step);
-        if (SUB == 1 && steps_of(sub) > 1) load_gu(sub, 1);
+        if (GROUPS == 1 && steps_of(sub) > 1) load_gu(sub, 1);
       };
       // One step of 32 tokens on its way out: h are its values as bf16 (plain store; SwiGLU backward, whose d(act) the unfused path
       // stores as bf16 too), r its fp32 values (SwiGLU: gate in r[0..15], up in r[16..31]).
@@ -540,7 +543,8 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
         ++ring_n;
       };
       if constexpr (EPI == GemmEpilogue::kLinear) {
-        // 32 tokens at a time: residual boxes come in by TMA two steps ahead and are overwritten by what goes out.
+        // 32 tokens at a time, by the two groups in turn: residual boxes come in by TMA while the other group is at work, and are overwritten by what goes out.
+        static_assert(GROUPS == 2, "half of the ring, and of the steps, a group");
         auto load_residual = [&](int st) {                     // issuer only
           uint8_t* b = ring + (st & 1) * kRing;
           mbar_arrive_expect_tx(&ctl->epi_load[st & 1], 2 * kBox);
@@ -549,8 +553,7 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
         };
         if (p.has_residual && issuer) {
           bulk_wait_read<0>();
-          load_residual(0);
-          if (steps_of(0) > 1) load_residual(1);
+          if (first_step < steps_of(0)) load_residual(first_step);
         }
         float bias[4];                                          // of features lane / 4 + 8 i
 #pragma unroll
@@ -560,7 +563,7 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
         }
         if (sg.parts == 1) wait_acc(0);
 #pragma unroll 1
-        for (int st = 0; ok && st < steps_of(0); ++st) {
+        for (int st = first_step; ok && st < steps_of(0); st += GROUPS) {
           uint32_t r[32], h[16];
           load_acc(0, st, r);
 #pragma unroll
@@ -625,7 +628,7 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
       } else if constexpr (SUB == 1) {
         if (EPI == GemmEpilogue::kSwiGLUBwd) begin_gu(0);       // the saved tiles arrive while the MMAs still run
         if (sg.parts == 1) wait_acc(0);
-        for (int st = 0; ok && st < steps_of(0); ++st) {
+        for (int st = first_step; ok && st < steps_of(0); st += GROUPS) {
           uint32_t r[32];
           load_acc(0, st, r);
           if constexpr (EPI == GemmEpilogue::kSwiGLU) emit_swiglu(0, st, r);
@@ -740,7 +743,7 @@ cudaError_t launch_sub(const TokGemmMaps& m, const CUtensorMap* c3, Args args, i
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(ctas & ~1);
-  cfg.blockDim = dim3(threads_for(SUB));
+  cfg.blockDim = dim3(threads_for(SUB, tok_dense<Args>::value));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
