@@ -67,22 +67,23 @@ constexpr int kStepTokens = 32;                   // tokens per epilogue step = 
 constexpr int kBox = kStepTokens * 128;           // 4 KiB: 32 tokens x 64 features
 
 struct __align__(8) TokCtl {
-  uint64_t full[kMaxStages], empty[kMaxStages], acc_full[kAccStages], acc_empty[kAccStages], epi_load[2], meet;
+  uint64_t full[kMaxStages], empty[kMaxStages], acc_full[kAccStages], acc_empty[kAccStages], epi_load[4], meet;
   uint32_t tmem_base;
   int abort_flag, last_arrived, widest, share_weights;
   int base[kTokPrefix + 1];                         // tiles of the groups before entry i
 };
-__host__ __device__ constexpr int epi_boxes(GemmEpilogue e) { return e == GemmEpilogue::kStore ? 2 : e == GemmEpilogue::kSwiGLU ? 3 : 4; }   // kLinear: two of the residual and the output, two of the pre-activation
+// Boxes of half of the ring. Dense stores have two buffers of two there; kLinear too, or one with the pre-activation's two boxes.
+__host__ __device__ constexpr int epi_boxes(GemmEpilogue e, bool dense = false) { return e == GemmEpilogue::kStore ? (dense ? 4 : 2) : e == GemmEpilogue::kSwiGLU ? 3 : 4; }
 constexpr int kSmemLimit = 227 * 1024;
-constexpr int other_bytes(GemmEpilogue e) { return 2 * epi_boxes(e) * kBox + 1024 + static_cast<int>(sizeof(TokCtl)); }
+constexpr int other_bytes(GemmEpilogue e, bool dense) { return 2 * epi_boxes(e, dense) * kBox + 1024 + static_cast<int>(sizeof(TokCtl)); }
 // Operand stages that fit. Tiles of up to 256 tokens: 6 of 32 KiB. Where few tokens meet the weights, the loop is bound by
 // HBM and wants weight bytes in flight: tiles of up to 64 tokens leave room for 10 stages of 20 KiB.
-constexpr int stages_for(GemmEpilogue e, int tile_n) {
-  const int n = (kSmemLimit - other_bytes(e)) / stage_bytes(tile_n);
+constexpr int stages_for(GemmEpilogue e, int tile_n, bool dense = false) {
+  const int n = (kSmemLimit - other_bytes(e, dense)) / stage_bytes(tile_n);
   return n < kMaxStages ? n : kMaxStages;
 }
-constexpr int smem_bytes(GemmEpilogue e, int tile_n) { return stages_for(e, tile_n) * stage_bytes(tile_n) + other_bytes(e); }
-static_assert(stages_for(GemmEpilogue::kSwiGLUBwd, kTokAccN) == 6 && stages_for(GemmEpilogue::kSwiGLU, 64) == 10, "stages at both ends of the range");
+constexpr int smem_bytes(GemmEpilogue e, int tile_n, bool dense) { return stages_for(e, tile_n, dense) * stage_bytes(tile_n) + other_bytes(e, dense); }
+static_assert(stages_for(GemmEpilogue::kSwiGLUBwd, kTokAccN) == 6 && stages_for(GemmEpilogue::kStore, kTokAccN, true) == 6 && stages_for(GemmEpilogue::kSwiGLU, 64) == 10, "stages at both ends of the range");
 static_assert(stages_for(GemmEpilogue::kSwiGLUBwd, 2 * kTokAccN) == 4, "stages of wide tiles");
 static_assert(kAccStages * kTokAccN <= kTmemCols, "two accumulators of 256 columns: of two tiles in turn, or both of a wide tile");
 static_assert(kTokPartialFloats == kHalfM * kTokAccN, "a partial is one CTA's accumulator");
@@ -123,15 +124,19 @@ __device__ __forceinline__ float as_f(uint32_t x) { return __uint_as_float(x); }
 // Tokens of a tile of n that accumulator `sub` holds.
 __device__ __forceinline__ int acc_n(int n, int sub) { return sub == 0 ? min(n, kTokAccN) : max(n - kTokAccN, 0); }
 
+// kLinear: two buffers in half of the ring, where the pre-activation does not take the place of one.
+__device__ __forceinline__ int buffers(const TokDenseArgs& p) { return p.keep_pre ? 1 : 2; }
+__device__ __forceinline__ int buffers(const TokGemmArgs&) { return 1; }
+
 template <GemmMode MODE, GemmEpilogue EPI, int SUB, class Args>
 __global__ void __launch_bounds__(threads_for(SUB, tok_dense<Args>::value), 1)
 grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ TokMapsX map_x, const __grid_constant__ CUtensorMap map_c,
                            const __grid_constant__ CUtensorMap map_c2, const __grid_constant__ CUtensorMap map_c3, const Args p) {
   constexpr bool DENSE = tok_dense<Args>::value;
   constexpr int GROUPS = groups_for(SUB, DENSE);   // of epilogue warps
+  constexpr int kRing = epi_boxes(EPI, DENSE) * kBox;
   static_assert(EPI != GemmEpilogue::kLinear || (DENSE && SUB == 1 && MODE == GemmMode::kForward), "one weight matrix, tiles of one accumulator");
   constexpr bool A_MN = MODE == GemmMode::kDgrad;
-  constexpr int kRing = epi_boxes(EPI) * kBox;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int stages = p.stages, stage_size = stage_bytes(p.tile_n);
@@ -144,7 +149,8 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) { mbar_init(&ctl->full[s], 1); mbar_init(&ctl->empty[s], 1); }
-    for (int a = 0; a < kAccStages; ++a) { mbar_init(&ctl->acc_full[a], 1); mbar_init(&ctl->acc_empty[a], 2 * 4 * GROUPS); mbar_init(&ctl->epi_load[a], 1); }
+    for (int a = 0; a < kAccStages; ++a) { mbar_init(&ctl->acc_full[a], 1); mbar_init(&ctl->acc_empty[a], 2 * 4 * GROUPS); }
+    for (int q = 0; q < 4; ++q) mbar_init(&ctl->epi_load[q], 1);
     mbar_init(&ctl->meet, 4 * GROUPS);
     ctl->abort_flag = 0;
     mbar_fence_init();
@@ -436,7 +442,15 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
 #pragma unroll
         for (int jj = 0; jj < 2; ++jj) stmatrix_trans(box_row(box, lane, jj, chunk), h[4 * jj], h[4 * jj + 1], h[4 * jj + 2], h[4 * jj + 3]);
       };
+      // Buffers of a group's half of the ring, which its steps take in turn.
+      const int bufs = !DENSE ? 1 : EPI == GemmEpilogue::kStore ? 2 : EPI == GemmEpilogue::kSwiGLU ? 2 - p.keep_gate_up : EPI == GemmEpilogue::kLinear ? buffers(p) : 1;
+      auto buffer = [&](uint32_t i) { return ring + group * kRing + (bufs == 2 ? i & 1u : 0u) * (EPI == GemmEpilogue::kSwiGLU ? 1 : 2) * kBox; };
       auto acquire = [&]() {
+        if constexpr (DENSE) {
+          if (issuer) { if (bufs == 2) bulk_wait_read<1>(); else bulk_wait_read<0>(); }
+          group_bar(group);
+          return buffer(ring_n);
+        }
         if (issuer) bulk_wait_read<GROUPS == 1 ? 1 : 0>();   // the stores that read this half of the ring are done with it
         group_bar(group);
         return ring + (GROUPS == 1 ? ring_n & 1u : group) * kRing;
@@ -545,15 +559,17 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
       if constexpr (EPI == GemmEpilogue::kLinear) {
         // 32 tokens at a time, by the two groups in turn: residual boxes come in by TMA while the other group is at work, and are overwritten by what goes out.
         static_assert(GROUPS == 2, "half of the ring, and of the steps, a group");
-        auto load_residual = [&](int st) {                     // issuer only
-          uint8_t* b = ring + (st & 1) * kRing;
-          mbar_arrive_expect_tx(&ctl->epi_load[st & 1], 2 * kBox);
+        auto load_residual = [&](int st, uint32_t i) {         // issuer only
+          uint64_t* bar = &ctl->epi_load[2 * group + (i & 1u)];
+          uint8_t* b = buffer(i);
+          mbar_arrive_expect_tx(bar, 2 * kBox);
 #pragma unroll
-          for (int q = 0; q < 2; ++q) tma_load_2d(b + q * kBox, &map_c2, feat0 + q * 64, row_of(0, st), &ctl->epi_load[st & 1]);
+          for (int q = 0; q < 2; ++q) tma_load_2d(b + q * kBox, &map_c2, feat0 + q * 64, row_of(0, st), bar);
         };
         if (p.has_residual && issuer) {
           bulk_wait_read<0>();
-          if (first_step < steps_of(0)) load_residual(first_step);
+          for (int i = 0; i < bufs; ++i)
+            if (first_step + i * GROUPS < steps_of(0)) load_residual(first_step + i * GROUPS, ring_n + i);
         }
         float bias[4];                                          // of features lane / 4 + 8 i
 #pragma unroll
@@ -570,9 +586,9 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
           for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(as_f(r[i]) + bias[(i >> 4) * 2 + (i >> 1 & 1)]);
           uint8_t* b;
           if (p.has_residual) {
-            b = ring + (st & 1) * kRing;
-            if (!(ok = mbar_wait_bounded(&ctl->epi_load[st & 1], (load_ph >> (st & 1)) & 1u, abort_flag, p.status, 500, p.timeout_ns))) break;
-            load_ph ^= 1u << (st & 1);
+            b = buffer(ring_n);
+            if (!(ok = mbar_wait_bounded(&ctl->epi_load[2 * group + (ring_n & 1u)], (load_ph >> (ring_n & 1u)) & 1u, abort_flag, p.status, 500, p.timeout_ns))) break;
+            load_ph ^= 1u << (ring_n & 1u);
           } else {
             b = acquire();
           }
@@ -619,7 +635,7 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
                 if (p.keep_pre) tma_store_2d(&map_c3, b + (2 + q) * kBox, feat0 + q * 64, y);
               }
             bulk_commit();
-            if (p.has_residual && st + 2 < steps_of(0)) { bulk_wait_read<0>(); load_residual(st + 2); }
+            if (p.has_residual && st + bufs * GROUPS < steps_of(0)) { bulk_wait_read<0>(); load_residual(st + bufs * GROUPS, ring_n + bufs); }
           }
           ++ring_n;
         }
@@ -737,13 +753,14 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
 template <GemmMode MODE, GemmEpilogue EPI, int SUB, class Args>
 cudaError_t launch_sub(const TokGemmMaps& m, const CUtensorMap* c3, Args args, int ctas, cudaStream_t stream) {
   auto kern = grouped_gemm_tokens_kernel<MODE, EPI, SUB, Args>;
-  args.stages = stages_for(EPI, args.tile_n);
-  const int smem = smem_bytes(EPI, args.tile_n);
+  constexpr bool dense = tok_dense<Args>::value;
+  args.stages = stages_for(EPI, args.tile_n, dense);
+  const int smem = smem_bytes(EPI, args.tile_n, dense);
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(ctas & ~1);
-  cfg.blockDim = dim3(threads_for(SUB, tok_dense<Args>::value));
+  cfg.blockDim = dim3(threads_for(SUB, dense));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
