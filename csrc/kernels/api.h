@@ -179,10 +179,11 @@ struct TokDenseArgs : TokGemmArgs {
   int has_residual, keep_pre;   // maps.c2, maps.c3
 };
 struct TokDenseMaps : TokGemmMaps {
-  const CUtensorMap* c3;     // kLinear with keep_pre: what the activation is taken of, written as bf16 {64,32}
+  const CUtensorMap* c3;     // kLinear with keep_pre: what the activation is taken of, written as bf16
 };
 bool dense_is_cut(const TokDenseArgs& args, int ctas);
-// kForward: kStore, kSwiGLU, kLinear (maps.c2: the residual {64,32}); kDgrad: kStore.
+// Forward: kStore (tiles of 512 tokens), kSwiGLU, kLinear (tiles of up to 256; maps.c2: the residual; c, c2 and c3 with boxes {32,32} and the 64-byte
+// swizzle); dgrad: kStore and kLinear, the same.
 cudaError_t launch_dense_gemm(GemmMode mode, GemmEpilogue epi, const TokDenseMaps& maps, const TokDenseArgs& args, int ctas, cudaStream_t stream);
 // The same for few tokens (linear_few.cu): forward, any epilogue, no scratch.
 constexpr int kFewTokens = 128;   // of a tile

@@ -258,14 +258,14 @@ torch::Tensor tma_rows(const torch::Tensor& t, int64_t cols) {
   const bool ok = reinterpret_cast<uintptr_t>(m.data_ptr()) % 16 == 0 && m.stride(1) == 1 && (m.size(0) <= 1 || (m.stride(0) % 8 == 0 && m.stride(0) >= cols));
   return ok ? m : m.clone(at::MemoryFormat::Contiguous);
 }
-CUtensorMap rows_map(const torch::Tensor& m, int box_rows) {
+CUtensorMap rows_map(const torch::Tensor& m, int box_rows, int box_cols = 64) {
   const cuuint64_t rows = static_cast<cuuint64_t>(m.size(0)), cols = static_cast<cuuint64_t>(m.size(1)), dims[2] = {cols, rows}, strides[1] = {2 * (rows > 1 ? static_cast<cuuint64_t>(m.stride(0)) : cols)};
-  const cuuint32_t box[2] = {64u, static_cast<cuuint32_t>(box_rows)};
-  return bf16_map(2, reinterpret_cast<int64_t>(m.data_ptr()), dims, strides, box);
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
+  return bf16_map(2, reinterpret_cast<int64_t>(m.data_ptr()), dims, strides, box, box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 struct DenseEpilogue {
-  GemmEpilogue kind = GemmEpilogue::kStore;
+  GemmEpilogue kind = GemmEpilogue::kLinear;
   const torch::Tensor *bias = nullptr, *residual = nullptr, *pre = nullptr;   // pre: pre-activation, or gate|up of kSwiGLU
   Activation act = Activation::kNone;
 };
@@ -282,15 +282,20 @@ void dense_gemm(GemmMode mode, const torch::Tensor& weight, const torch::Tensor&
   a.granule = 32;
   // Where all tokens fit a narrow tile, narrow tiles leave shared memory to the weights in flight.
   a.tile_n = a.dense_rows <= 64 ? 64 : a.dense_rows <= 128 ? 128 : 256;
-  if (ep.kind != GemmEpilogue::kLinear && a.tile_n == 256 &&
-      gemm::tok_wide(ep.kind == GemmEpilogue::kSwiGLU, static_cast<int>(reduction), a.dense_rows, (a.dense_rows + 511) / 512 * (features / 256.0) / (ctas / 2)))
+  GemmEpilogue kind = ep.kind;
+  const bool plain = ep.kind == GemmEpilogue::kLinear && ep.act == Activation::kNone && !ep.bias && !ep.residual && !ep.pre;
+  if ((plain || ep.kind == GemmEpilogue::kSwiGLU) && a.tile_n == 256 &&
+      gemm::tok_wide(ep.kind == GemmEpilogue::kSwiGLU, static_cast<int>(reduction), a.dense_rows, (a.dense_rows + 511) / 512 * (features / 256.0) / (ctas / 2))) {
     a.tile_n = 512;
+    if (plain) kind = GemmEpilogue::kStore;
+  }
   a.band_tiles = gemm::tok_band(0, 64 * a.red_blocks, a.m_tiles, a.tile_n);
   a.back_tiles = gemm::tok_back_tiles(64 * a.red_blocks, a.band_tiles, std::max(a.tile_n, gemm::kTokAccN));
   a.status = dense_status();
   TORCH_CHECK(a.status != nullptr, "linear: no status block on this device");
   a.timeout_ns = timeout_ns;
-  CUtensorMap w, c = rows_map(out, 32), c2, c3;
+  const int cols = kind == GemmEpilogue::kLinear ? 32 : 64;   // of the epilogue's boxes
+  CUtensorMap w, c = rows_map(out, 32, cols), c2, c3;
   TokMapsX xm;
   if (ep.kind == GemmEpilogue::kSwiGLU) {
     // [N / 256 tiles][8 groups of 16 features][gate, up][16][K], fetched as four groups with both halves
@@ -303,13 +308,13 @@ void dense_gemm(GemmMode mode, const torch::Tensor& weight, const torch::Tensor&
   for (int j = 0; j < kTokBoxes; ++j) xm.box[j] = rows_map(x, 16 << j);
   TokDenseMaps maps{};
   maps.w = &w; maps.x = &xm; maps.c = &c;
-  if (ep.kind == GemmEpilogue::kSwiGLU) {
+  if (kind == GemmEpilogue::kSwiGLU) {
     if (ep.pre) { c2 = rows_map(*ep.pre, 32); maps.c2 = &c2; a.keep_gate_up = 1; }
-  } else if (ep.kind == GemmEpilogue::kLinear) {
+  } else if (kind == GemmEpilogue::kLinear) {
     a.act = ep.act;
     if (ep.bias) a.bias = reinterpret_cast<const __nv_bfloat16*>(ep.bias->data_ptr());
-    if (ep.residual) { c2 = rows_map(*ep.residual, 32); maps.c2 = &c2; a.has_residual = 1; }
-    if (ep.pre) { c3 = rows_map(*ep.pre, 32); maps.c3 = &c3; a.keep_pre = 1; }
+    if (ep.residual) { c2 = rows_map(*ep.residual, 32, cols); maps.c2 = &c2; a.has_residual = 1; }
+    if (ep.pre) { c3 = rows_map(*ep.pre, 32, cols); maps.c3 = &c3; a.keep_pre = 1; }
   }
   torch::Tensor partials, counters;
   if (dense_is_cut(a, ctas)) {
@@ -318,7 +323,7 @@ void dense_gemm(GemmMode mode, const torch::Tensor& weight, const torch::Tensor&
     a.partials = partials.data_ptr<float>();
     a.counters = reinterpret_cast<unsigned int*>(counters.data_ptr<int>());
   }
-  cuda_check(launch_dense_gemm(mode, ep.kind, maps, a, ctas, cur_stream()), "linear");
+  cuda_check(launch_dense_gemm(mode, kind, maps, a, ctas, cur_stream()), "linear");
 }
 
 // out [N, K] = dz [T, N]^T . x [T, K]
@@ -380,8 +385,7 @@ LinearOut linear_forward(const torch::Tensor& x, const torch::Tensor& weight, co
   DenseEpilogue ep;
   if (kind == LinearKind::kSwiGLU) {
     ep.kind = GemmEpilogue::kSwiGLU;
-  } else if (bias.has_value() || residual.has_value() || kind != LinearKind::kNone) {
-    ep.kind = GemmEpilogue::kLinear;
+  } else {
     ep.act = static_cast<Activation>(kind);
     if (bias.has_value()) { bm = reinterpret_cast<uintptr_t>(bias->data_ptr()) % 8 == 0 ? *bias : bias->clone(); ep.bias = &bm; }   // read in words of 8 bytes
     if (residual.has_value()) { rm = tma_rows(*residual, cols); ep.residual = &rm; }

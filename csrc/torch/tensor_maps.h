@@ -21,13 +21,13 @@ inline EncodeTiledFn encode_tiled() {
   return fn;
 }
 
-inline CUtensorMap bf16_map(int rank, int64_t ptr, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+inline CUtensorMap bf16_map(int rank, int64_t ptr, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   TORCH_CHECK(ptr % 16 == 0, "tensor map base must be 16-byte aligned");
   for (int i = 0; i + 1 < rank; ++i) TORCH_CHECK(strides[i] % 16 == 0, "tensor map strides must be multiples of 16 bytes");
   alignas(64) CUtensorMap m;
   cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   CUresult r = encode_tiled()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, reinterpret_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                              swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code ", static_cast<int>(r));
   return m;
 }
