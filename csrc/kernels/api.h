@@ -462,11 +462,11 @@ struct BalanceArgs {
   int* chosen;                 // [blocks][E + 1] scratch: counts, live tokens
   float* loss;                 // out
   int* counts;                 // [E] out
-  int* live;                   // out: N
+  int* kept;                   // [E + 1] out: the counts again and N, for the backward pass (the caller's counts are its own to change)
 };
 int balance_blocks(const BalanceArgs& a, int sms);
 cudaError_t launch_balance(const BalanceArgs& a, int blocks, cudaStream_t stream);
-// dlogits [T, E], the logits' type, from the forward pass's counts and N: E / (K N^2) * *dloss * ds/dlogits . c.
+// dlogits [T, E], the logits' type: E / (K N^2) * *dloss * ds/dlogits . c.
 struct BalanceBwdArgs {
   const void* logits;
   long long stride;
@@ -474,8 +474,7 @@ struct BalanceBwdArgs {
   const unsigned char* mask;
   int T, E, K;
   int sigmoid;
-  const int* counts;
-  const int* live;
+  const int* kept;             // the forward pass's
   const float* dloss;
   void* dlogits;               // [T, E] out
 };

@@ -7,7 +7,8 @@
 //
 // A token's scores sum to one, so any constant may be taken from all counts: the gradient uses E c_e - sum of all counts, exact in whole
 // numbers. Taken as they are, counts that are nearly equal (what the loss is for) cancel all but a few bits of an fp32 difference.
-// What bounds it: HBM for many tokens, launches for few. A token's logits are spread over up to 32 lanes (a power of two), which keep their
+// What bounds it: HBM and instructions for many tokens (65536 x 256 in fp32, softmax: forward 19 us and the sums' 9, backward 25, where the bytes take 10 and 20),
+// launches for few. A token's logits are spread over up to 32 lanes (a power of two), which keep their
 // experts' sums over all their tokens in registers; a block leaves its sums, a cluster of blocks adds them in a fixed order, so that the loss
 // does not change from run to run. Up to kOneBlock token groups a single block does it all in one launch.
 #include <cooperative_groups.h>
@@ -25,9 +26,8 @@ using bf16 = __nv_bfloat16;
 constexpr int kFoldCtas = 8, kFoldThreads = 1024;
 constexpr int kOneBlock = 4;     // rounds of the one-block launch
 
-__device__ __forceinline__ float as_logit(float v) { return v == v ? v : -INFINITY; }
-__device__ __forceinline__ float load_logit(const float* p) { return as_logit(__ldg(p)); }
-__device__ __forceinline__ float load_logit(const bf16* p) { return as_logit(__bfloat162float(__ldg(p))); }
+__device__ __forceinline__ float load_logit(const float* p) { return __ldg(p); }
+__device__ __forceinline__ float load_logit(const bf16* p) { return __bfloat162float(__ldg(p)); }
 
 // Sum and maximum over the G neighbouring lanes of a token.
 template <int G> __device__ __forceinline__ float lanes_sum(float v) {
@@ -43,36 +43,37 @@ template <int G> __device__ __forceinline__ float lanes_max(float v) {
 // 1 / sum of a token's scores; none: 0, so that its scores are 0.
 __device__ __forceinline__ float inverse(float total) { return total > 0.0f ? 1.0f / total : 0.0f; }
 
-// l: logits of my experts (-inf past the last) -> their scores; slope, if wanted: sigmoid'(l) / sum of sigmoids (softmax: the score).
+// l: logits of my experts (-inf past the last) -> their shares of the token, to be multiplied by what is returned: 1 / their sum. slope, if wanted:
+// sigmoid'(l), by the same factor (softmax: the share). Every value is taken through a maximum with 0, which turns NaN, a NaN logit's or that of -inf - -inf, into 0.
 template <int G, int P, bool SIGMOID, bool SLOPE>
-__device__ __forceinline__ void scores(float (&l)[P], float (&slope)[SLOPE ? P : 1]) {
+__device__ __forceinline__ float shares(float (&l)[P], float (&slope)[SLOPE ? P : 1]) {
   float total = 0.0f;
   if (SIGMOID) {
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       const float e = __expf(-fabsf(l[i])), d = 1.0f / (1.0f + e);   // exact towards both ends
-      if (SLOPE) slope[i] = e * d * d;
-      l[i] = l[i] >= 0.0f ? d : e * d;
+      if (SLOPE) slope[i] = fmaxf(e * d * d, 0.0f);
+      l[i] = fmaxf(l[i] >= 0.0f ? d : e * d, 0.0f);
       total += l[i];
     }
   } else {
-    float top = l[0];
+    float top = -INFINITY;
 #pragma unroll
-    for (int i = 1; i < P; ++i) top = fmaxf(top, l[i]);
+    for (int i = 0; i < P; ++i) top = fmaxf(top, l[i]);
     top = lanes_max<G>(top);
+    if (top == INFINITY) {   // the infinite ones share the token
+#pragma unroll
+      for (int i = 0; i < P; ++i) l[i] = l[i] == INFINITY ? 0.0f : -INFINITY;
+      top = 0.0f;
+    }
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      // nothing selectable: zeros; an infinite logit: the infinite ones share the token
-      l[i] = top == -INFINITY ? 0.0f : top == INFINITY ? (l[i] == INFINITY ? 1.0f : 0.0f) : __expf(l[i] - top);
+      l[i] = fmaxf(__expf(l[i] - top), 0.0f);
+      if (SLOPE) slope[i] = l[i];
       total += l[i];
     }
   }
-  const float inv = inverse(lanes_sum<G>(total));
-#pragma unroll
-  for (int i = 0; i < P; ++i) {
-    l[i] *= inv;
-    if (SLOPE) slope[i] = SIGMOID ? slope[i] * inv : l[i];
-  }
+  return inverse(lanes_sum<G>(total));
 }
 
 // Column sums and counts of a part of the tokens. A lane's experts are g, g + G, ..., P of them.
@@ -95,23 +96,37 @@ __global__ void __launch_bounds__(P >= 16 ? 512 : 1024, 1) balance_kernel(const 
   for (int i = 0; i < P; ++i) acc[i] = 0.0f;
   int live = 0;
   const long long step = static_cast<long long>(gridDim.x) * warps * kTokens;
-  for (long long t0 = (static_cast<long long>(blockIdx.x) * warps + warp) * kTokens; t0 < a.T; t0 += step) {   // all lanes of a warp alike
+  long long t0 = (static_cast<long long>(blockIdx.x) * warps + warp) * kTokens;
+  float next[P];
+  bool next_on = false;
+  int next_e = -1;                             // of the token's choices, mine
+  const auto request = [&](long long first) {   // the next token is under way while this one is worked on
+    const long long t = first + lane / G;
+    const bool in = t < a.T;
+    const T* row = static_cast<const T*>(a.logits) + (in ? t : 0) * a.stride;
+#pragma unroll
+    for (int i = 0; i < P; ++i) next[i] = in && g + i * G < a.E ? load_logit(row + g + i * G) : -INFINITY;
+    next_e = in && g < a.K ? __ldg(a.topk_idx + t * a.K + g) : -1;
+    next_on = in && (a.mask == nullptr || a.mask[t] != 0);
+  };
+  const auto count = [&](int e) { if (e >= 0 && e < a.E) atomicAdd(s_count + e, 1); };
+  if (t0 < a.T) request(t0);
+  for (; t0 < a.T; t0 += step) {   // all lanes of a warp alike
     const long long t = t0 + lane / G;
-    const bool on = t < a.T && (a.mask == nullptr || a.mask[t] != 0);
-    const T* row = static_cast<const T*>(a.logits) + (on ? t : 0) * a.stride;
+    const bool on = next_on;
+    const int mine = next_e;
     float l[P];
 #pragma unroll
-    for (int i = 0; i < P; ++i) l[i] = on && g + i * G < a.E ? load_logit(row + g + i * G) : -INFINITY;
+    for (int i = 0; i < P; ++i) l[i] = next[i];
+    if (t0 + step < a.T) request(t0 + step);
     if (on) {
       live += g == 0 ? 1 : 0;
-      for (int j = g; j < a.K; j += G) {
-        const int e = __ldg(a.topk_idx + t * a.K + j);
-        if (e >= 0 && e < a.E) atomicAdd(s_count + e, 1);
-      }
+      count(mine);
+      for (int j = g + G; j < a.K; j += G) count(__ldg(a.topk_idx + t * a.K + j));
     }
-    scores<G, P, SIGMOID, false>(l, unused);
+    const float inv = shares<G, P, SIGMOID, false>(l, unused), factor = on ? inv : 0.0f;   // a padded token's logits have no part, whatever they are
 #pragma unroll
-    for (int i = 0; i < P; ++i) acc[i] += on ? l[i] : 0.0f;
+    for (int i = 0; i < P; ++i) acc[i] = fmaf(l[i], factor, acc[i]);
   }
   if (live) atomicAdd(&s_live, live);
 #pragma unroll
@@ -135,7 +150,7 @@ __global__ void __launch_bounds__(P >= 16 ? 512 : 1024, 1) balance_kernel(const 
   for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
     float v = 0.0f;
     for (int w = 0; w < warps; ++w) v += s_sum[w * a.E + e];
-    a.counts[e] = s_count[e];
+    a.counts[e] = a.kept[e] = s_count[e];
     part = fmaf(static_cast<float>(s_count[e]), v, part);
   }
   part = lanes_sum<32>(part);
@@ -145,7 +160,7 @@ __global__ void __launch_bounds__(P >= 16 ? 512 : 1024, 1) balance_kernel(const 
     for (int w = 1; w < warps; ++w) part += s_loss[w];
     const float n = static_cast<float>(max(s_live, 1));
     *a.loss = part / n * (static_cast<float>(a.E) / (static_cast<float>(a.K) * n));
-    *a.live = s_live;
+    a.kept[a.E] = s_live;
   }
 }
 
@@ -197,7 +212,7 @@ __global__ void __cluster_dims__(kFoldCtas, 1, 1) __launch_bounds__(kFoldThreads
       v += *cluster.map_shared_rank(s_sum + e, r);
       n += *cluster.map_shared_rank(s_count + e, r);
     }
-    a.counts[e] = n;
+    a.counts[e] = a.kept[e] = n;
     part = fmaf(static_cast<float>(n), v, part);
   }
   part = lanes_sum<32>(part);
@@ -216,7 +231,7 @@ __global__ void __cluster_dims__(kFoldCtas, 1, 1) __launch_bounds__(kFoldThreads
     for (int r = 0; r < kFoldCtas; ++r) part += s_all[r];
     const float n = static_cast<float>(max(live, 1));
     *a.loss = part / n * (static_cast<float>(a.E) / (static_cast<float>(a.K) * n));
-    *a.live = live;
+    a.kept[a.E] = live;
   }
 }
 
@@ -232,14 +247,14 @@ __global__ void __launch_bounds__(256) balance_bwd_kernel(const BalanceBwdArgs a
   int c[P];
 #pragma unroll
   for (int i = 0; i < P; ++i) {
-    c[i] = g + i * G < a.E ? __ldg(a.counts + g + i * G) : 0;
+    c[i] = g + i * G < a.E ? __ldg(a.kept + g + i * G) : 0;
     all += c[i];
   }
 #pragma unroll
   for (int o = G / 2; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
 #pragma unroll
   for (int i = 0; i < P; ++i) d[i] = g + i * G < a.E ? static_cast<float>(static_cast<long long>(a.E) * c[i] - all) : 0.0f;
-  const float n = static_cast<float>(max(__ldg(a.live), 1)), factor = __ldg(a.dloss) / n / (static_cast<float>(a.K) * n);
+  const float n = static_cast<float>(max(__ldg(a.kept + a.E), 1)), factor = __ldg(a.dloss) / n / (static_cast<float>(a.K) * n);
   const long long step = static_cast<long long>(gridDim.x) * warps * kTokens;
   for (long long t0 = (static_cast<long long>(blockIdx.x) * warps + warp) * kTokens; t0 < a.T; t0 += step) {
     const long long t = t0 + lane / G;
@@ -248,17 +263,17 @@ __global__ void __launch_bounds__(256) balance_bwd_kernel(const BalanceBwdArgs a
     float l[P], slope[P];
 #pragma unroll
     for (int i = 0; i < P; ++i) l[i] = on && g + i * G < a.E ? load_logit(row + g + i * G) : -INFINITY;
-    scores<G, P, SIGMOID, true>(l, slope);
+    const float inv = shares<G, P, SIGMOID, true>(l, slope);
     float mean = 0.0f;
 #pragma unroll
     for (int i = 0; i < P; ++i) mean = fmaf(l[i], d[i], mean);
-    mean = lanes_sum<G>(mean);
+    mean = lanes_sum<G>(mean) * inv;
     if (t >= a.T) continue;
     T* out = static_cast<T*>(a.dlogits) + t * a.E;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       if (g + i * G >= a.E) continue;
-      const float v = on ? slope[i] * (d[i] - mean) * factor : 0.0f;   // the small factor last: slopes may be tiny. A padded token's logits have no part in anything, whatever they are
+      const float v = on ? slope[i] * inv * (d[i] - mean) * factor : 0.0f;   // the small factor last: slopes may be tiny
       if constexpr (sizeof(T) == 2) out[g + i * G] = __float2bfloat16_rn(v);
       else out[g + i * G] = v;
     }

@@ -174,8 +174,7 @@ std::tuple<torch::Tensor, torch::Tensor, OptTensor, OptTensor> add_rms_norm(cons
 }
 
 // ---- balance loss -----------------------------------------------------------------------------------------
-struct Balance { torch::Tensor loss, counts, live; };
-// logits as rows [T, E], and what the mask is read from.
+struct Balance { torch::Tensor loss, counts, kept; };
 torch::Tensor mask_bytes(const OptTensor& mask) { return mask.has_value() ? mask->contiguous() : torch::Tensor(); }
 
 Balance balance(const torch::Tensor& logits, const torch::Tensor& topk_idx, const OptTensor& mask, bool sigmoid) {
@@ -195,8 +194,8 @@ Balance balance(const torch::Tensor& logits, const torch::Tensor& topk_idx, cons
   a.T = rows_of(lm, "balance_loss"); a.E = static_cast<int>(E); a.K = static_cast<int>(topk_idx.size(-1)); a.sigmoid = sigmoid;
   TORCH_CHECK(static_cast<int64_t>(a.T) * a.K <= 0x7fffffff, "balance_loss: more than 2^31 - 1 choices");
   const auto f32 = logits.options().dtype(torch::kFloat32), i32 = logits.options().dtype(torch::kInt32);
-  Balance b{torch::empty({}, f32), torch::empty({E}, i32), torch::empty({}, i32)};
-  a.loss = b.loss.data_ptr<float>(); a.counts = b.counts.data_ptr<int>(); a.live = b.live.data_ptr<int>();
+  Balance b{torch::empty({}, f32), torch::empty({E}, i32), torch::empty({E + 1}, i32)};
+  a.loss = b.loss.data_ptr<float>(); a.counts = b.counts.data_ptr<int>(); a.kept = b.kept.data_ptr<int>();
   const int blocks = balance_blocks(a, sm_count(logits));
   torch::Tensor scratch;
   if (blocks > 1) {
@@ -214,7 +213,7 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
     ctx->set_materialize_grads(false);
     ctx->saved_data["k"] = topk_idx.size(-1);
     ctx->saved_data["sigmoid"] = sigmoid;
-    ctx->save_for_backward({logits, mask_bytes(mask), b.counts, b.live});
+    ctx->save_for_backward({logits, mask_bytes(mask), b.kept});
     ctx->mark_non_differentiable({b.counts});
     return {b.loss, b.counts};
   }
@@ -232,7 +231,7 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
       a.logits = lm.data_ptr(); a.stride = lm.stride(0); a.logits_bf16 = logits.scalar_type() == torch::kBFloat16;
       a.mask = saved[1].defined() ? reinterpret_cast<const unsigned char*>(saved[1].data_ptr()) : nullptr;
       a.T = static_cast<int>(lm.size(0)); a.E = static_cast<int>(logits.size(-1)); a.K = static_cast<int>(ctx->saved_data["k"].toInt()); a.sigmoid = ctx->saved_data["sigmoid"].toBool();
-      a.counts = saved[2].data_ptr<int>(); a.live = saved[3].data_ptr<int>(); a.dloss = dloss.data_ptr<float>(); a.dlogits = dlogits.data_ptr();
+      a.kept = saved[2].data_ptr<int>(); a.dloss = dloss.data_ptr<float>(); a.dlogits = dlogits.data_ptr();
       cuda_check(launch_balance_bwd(a, sm_count(logits), cur_stream()), "balance_loss backward");
     }
     variable_list in = grads;

@@ -191,3 +191,19 @@ def test_its_backward_has_no_gradient():
     (g,) = torch.autograd.grad(fused.balance_loss(leaf, idx)[0], leaf, create_graph=True)
     with pytest.raises(RuntimeError, match="no gradient"):
         g.sum().backward()
+
+
+def test_counts_and_inputs_may_change_before_the_backward_pass():
+    """The counts are the caller's (summed over ranks in place, say); so are the choices. Logits that change are noticed."""
+    logits, idx, _ = make(500, 16, 2, 1)
+    leaf = logits.detach().requires_grad_()
+    (want,) = torch.autograd.grad(fused.balance_loss(leaf, idx)[0], leaf)
+    loss, counts = fused.balance_loss(leaf, idx)
+    counts.mul_(8)
+    idx.zero_()
+    assert torch.equal(torch.autograd.grad(loss, leaf)[0], want)
+    moved = leaf * 1.0
+    loss, _ = fused.balance_loss(moved, idx)
+    moved.add_(1.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()

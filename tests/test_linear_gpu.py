@@ -13,7 +13,8 @@ pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
 HALF = 2.0**-8
 SHAPES = [(1, 8, 8), (1, 4096, 256), (2, 72, 136), (31, 64, 264), (33, 1000, 1736), (64, 2048, 7168), (65, 512, 520), (100, 7168, 1032), (129, 136, 72), (257, 1024, 1024), (300, 8, 2000), (513, 4096, 8),
-          (1235, 1000, 2760), (2000, 200, 4104), (700, 9000, 328)]
+          (1235, 1000, 2760), (2000, 200, 4104), (700, 9000, 328), (50, 136, 20008), (100, 136, 20008),   # narrow tiles in more than a round
+          (100, 8192, 8200), (8200, 8200, 3432), (8200, 3432, 8200)]                                      # wide weight gradients, forward and data gradients
 
 
 def whole(shape, seed, most=2):
@@ -90,7 +91,7 @@ def test_activations_and_gradients(T, K, N, act):
         assert (got.double() - ref).norm() <= 4 * HALF * ref.norm()
 
 
-@pytest.mark.parametrize("T,K,I", [(1, 512, 128), (7, 1000, 256), (130, 7168, 2048), (600, 264, 384), (1100, 2048, 640)])
+@pytest.mark.parametrize("T,K,I", [(1, 512, 128), (7, 1000, 256), (130, 7168, 2048), (600, 264, 384), (1100, 2048, 640), (300, 4104, 52224)])
 def test_swiglu(T, K, I):
     x, w1, w3, dy = normal((T, K), 1), normal((I, K), 2, K**-0.5), normal((I, K), 3, K**-0.5), normal((T, I), 4)
     w = interleave_gate_up(w1.unsqueeze(0), w3.unsqueeze(0))[0].requires_grad_()
