@@ -185,7 +185,7 @@ bool dense_is_cut(const TokDenseArgs& args, int ctas);
 // Forward: kStore (tiles of 512 tokens), kSwiGLU, kLinear (tiles of up to 256; maps.c2: the residual; c, c2 and c3 with boxes {32,32} and the 64-byte
 // swizzle); dgrad: kStore and kLinear, the same.
 cudaError_t launch_dense_gemm(GemmMode mode, GemmEpilogue epi, const TokDenseMaps& maps, const TokDenseArgs& args, int ctas, cudaStream_t stream);
-// The same for few tokens (linear_few.cu): forward, any epilogue, no scratch.
+// The same for few tokens (linear_few.cu): forward with any epilogue and dgrad, no scratch.
 constexpr int kFewTokens = 128;   // of a tile
 struct FewArgs {
   int T, columns;              // tokens, columns of the output
@@ -200,8 +200,8 @@ struct FewArgs {
   unsigned long long timeout_ns;
 };
 bool few_pays(int T, int columns, int red_blocks, bool swiglu, int sms);
-int few_box_rows(int T);       // rows of map_x's boxes {64, rows}; map_w's are {64,128}, SwiGLU {64,64}
-cudaError_t launch_linear_few(Activation act, bool swiglu, const CUtensorMap& map_w, const CUtensorMap& map_x, const FewArgs& args, int sms, cudaStream_t stream);
+int few_box_rows(int T);       // rows of map_x's boxes {64, rows}; map_w's are {64,128}, SwiGLU and dgrad {64,64}
+cudaError_t launch_linear_few(GemmMode mode, Activation act, bool swiglu, const CUtensorMap& map_w, const CUtensorMap& map_x, const FewArgs& args, int sms, cudaStream_t stream);
 // Where dense launches on the current device report a wait that gave up.
 DeviceStatus* dense_status();
 

@@ -38,6 +38,8 @@
 // one wide tile holds and one of 256 does not. Which calls take wide tiles: ops/gemm.py.
 //
 // Barriers as in grouped_gemm_pair.cu. Every wait is bounded. No load is multicast.
+#include <atomic>
+
 #include "gemm_epilogue_tma.cuh"
 #include "early_start.cuh"
 #include "token_walker.h"
@@ -794,8 +796,16 @@ __device__ DeviceStatus g_dense_status;   // one on every device that the librar
 }  // namespace
 
 DeviceStatus* dense_status() {
-  void* p = nullptr;
-  return cudaGetSymbolAddress(&p, g_dense_status) == cudaSuccess ? static_cast<DeviceStatus*>(p) : nullptr;
+  static std::atomic<DeviceStatus*> known[64];   // the same for good; asking the runtime takes most of a microsecond
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+  DeviceStatus* at = known[dev].load(std::memory_order_relaxed);
+  if (at == nullptr) {
+    void* p = nullptr;
+    if (cudaGetSymbolAddress(&p, g_dense_status) != cudaSuccess) return nullptr;
+    known[dev].store(at = static_cast<DeviceStatus*>(p), std::memory_order_relaxed);
+  }
+  return at;
 }
 
 bool dense_is_cut(const TokDenseArgs& args, int ctas) { return dense_split(args, ctas).cut_tiles > 0; }

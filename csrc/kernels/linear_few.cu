@@ -1,4 +1,5 @@
-// A linear layer on a few tokens: out = act(x W^T + bias) + residual, or SwiGLU, in tiles of 128 rows of the weight by up to kFewTokens tokens.
+// A linear layer on a few tokens: out = act(x W^T + bias) + residual, or SwiGLU, in tiles of 128 rows of the weight by up to kFewTokens tokens; and
+// its data gradient, x W, in tiles of 128 of its columns.
 //
 // What bounds it: the weight's bytes. A cluster of CTAs has a tile and shares out the reduction; a CTA streams its part of the weight's
 // rows through shared memory (TMA) as operand A of M = 128 MMAs, the tokens are N (rounded up to 16), so a decode step does no more work
@@ -54,7 +55,8 @@ __device__ __forceinline__ float activated(float z) {
   return ACT == Activation::kRelu ? fmaxf(z, 0.0f) : ACT == Activation::kSilu ? silu(z) : ACT == Activation::kGelu ? gelu(z) : z;
 }
 
-template <Activation ACT, bool SWIGLU, int PARTS>
+// DGRAD: out = x W, the weight's columns are the features (operand A MN-major).
+template <Activation ACT, bool SWIGLU, bool DGRAD, int PARTS>
 __global__ void __launch_bounds__(kThreads) linear_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const FewArgs p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -95,6 +97,9 @@ __global__ void __launch_bounds__(kThreads) linear_few_kernel(const __grid_const
           const int gate = tile / 2 * 256 + tile % 2 * 64;
           tma_load_2d(sa, &map_w, k, gate, &ctl->full[s]);
           tma_load_2d(sa + kFewABytes / 2, &map_w, k, gate + 128, &ctl->full[s]);
+        } else if (DGRAD) {
+#pragma unroll
+          for (int j = 0; j < kRows / 64; ++j) tma_load_2d(sa + j * (BK * 128), &map_w, tile * kRows + j * 64, k, &ctl->full[s]);
         } else {
           tma_load_2d(sa, &map_w, k, tile * kRows, &ctl->full[s]);
         }
@@ -104,7 +109,7 @@ __global__ void __launch_bounds__(kThreads) linear_few_kernel(const __grid_const
     }
   } else if (warp == 1) {
     if (elect_one()) {
-      const uint32_t idesc = make_idesc_bf16(kRows, n, false, false);
+      const uint32_t idesc = make_idesc_bf16(kRows, n, DGRAD, false);
       uint32_t ph = 0;
       bool ok = true;
       for (int i = 0, s = 0; i < blocks; ++i) {
@@ -113,7 +118,7 @@ __global__ void __launch_bounds__(kThreads) linear_few_kernel(const __grid_const
         const uint32_t sa = smem_u32(tiles + s * stage_size), sb = sa + kFewABytes;
 #pragma unroll
         for (int k = 0; k < BK / UMMA_K; ++k)
-          mma_bf16_ss(tmem, make_smem_desc(sa + k * 32, 16, 1024), make_smem_desc(sb + k * 32, 16, 1024), idesc, (i | k) != 0 ? 1u : 0u);
+          mma_bf16_ss(tmem, DGRAD ? make_smem_desc(sa + k * 2048, BK * 128, 1024) : make_smem_desc(sa + k * 32, 16, 1024), make_smem_desc(sb + k * 32, 16, 1024), idesc, (i | k) != 0 ? 1u : 0u);
         mma_commit(&ctl->empty[s]);
         if (++s == stages) { s = 0; ph ^= 1; }
       }
@@ -227,9 +232,9 @@ bool few_pays(int T, int columns, int red_blocks, bool swiglu, int sms) {
   return 2 * tiles <= sms || (tiles <= sms && red_blocks <= 96);
 }
 
-cudaError_t launch_linear_few(Activation act, bool swiglu, const CUtensorMap& map_w, const CUtensorMap& map_x, const FewArgs& args, int sms, cudaStream_t stream) {
+cudaError_t launch_linear_few(GemmMode mode, Activation act, bool swiglu, const CUtensorMap& map_w, const CUtensorMap& map_x, const FewArgs& args, int sms, cudaStream_t stream) {
   FewArgs a = args;
-  if (a.T < 1 || a.columns < 1 || a.red_blocks < 1 || a.status == nullptr || (swiglu && (act != Activation::kNone || a.columns % 128))) return cudaErrorInvalidValue;
+  if (a.T < 1 || a.columns < 1 || a.red_blocks < 1 || a.status == nullptr || (mode != GemmMode::kForward && (mode != GemmMode::kDgrad || swiglu || act != Activation::kNone)) || (swiglu && (act != Activation::kNone || a.columns % 128))) return cudaErrorInvalidValue;
   const int per_tile = swiglu ? kRows / 2 : kRows, tiles = (a.columns + per_tile - 1) / per_tile;
   a.n = few_box_rows(a.T);
   a.stages = few_stages(a.n);
@@ -253,25 +258,28 @@ cudaError_t launch_linear_few(Activation act, bool swiglu, const CUtensorMap& ma
     cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, kern, map_w, map_x, a);
   };
-  const auto with = [&](auto act_c, auto swiglu_c) {
+  const auto with = [&](auto act_c, auto swiglu_c, auto dgrad_c) {
     constexpr Activation ACT = decltype(act_c)::value;
-    constexpr bool SWIGLU = decltype(swiglu_c)::value;
+    constexpr bool SWIGLU = decltype(swiglu_c)::value, DGRAD = decltype(dgrad_c)::value;
     switch (a.parts) {
-      case 1: return go(linear_few_kernel<ACT, SWIGLU, 1>);
-      case 2: return go(linear_few_kernel<ACT, SWIGLU, 2>);
-      case 4: return go(linear_few_kernel<ACT, SWIGLU, 4>);
-      case 8: return go(linear_few_kernel<ACT, SWIGLU, 8>);
+      case 1: return go(linear_few_kernel<ACT, SWIGLU, DGRAD, 1>);
+      case 2: return go(linear_few_kernel<ACT, SWIGLU, DGRAD, 2>);
+      case 4: return go(linear_few_kernel<ACT, SWIGLU, DGRAD, 4>);
+      case 8: return go(linear_few_kernel<ACT, SWIGLU, DGRAD, 8>);
       default: return cudaErrorInvalidValue;
     }
   };
   using std::integral_constant;
+  constexpr std::true_type yes;
+  constexpr std::false_type no;
   using none = integral_constant<Activation, Activation::kNone>;
   cudaError_t e;
-  if (swiglu) e = with(none(), std::true_type());
-  else if (act == Activation::kRelu) e = with(integral_constant<Activation, Activation::kRelu>(), std::false_type());
-  else if (act == Activation::kSilu) e = with(integral_constant<Activation, Activation::kSilu>(), std::false_type());
-  else if (act == Activation::kGelu) e = with(integral_constant<Activation, Activation::kGelu>(), std::false_type());
-  else e = with(none(), std::false_type());
+  if (mode == GemmMode::kDgrad) e = with(none(), no, yes);
+  else if (swiglu) e = with(none(), yes, no);
+  else if (act == Activation::kRelu) e = with(integral_constant<Activation, Activation::kRelu>(), no, no);
+  else if (act == Activation::kSilu) e = with(integral_constant<Activation, Activation::kSilu>(), no, no);
+  else if (act == Activation::kGelu) e = with(integral_constant<Activation, Activation::kGelu>(), no, no);
+  else e = with(none(), no, no);
   if (e == cudaSuccess) note_launch();
   return e;
 }

@@ -343,19 +343,22 @@ void dense_wgrad(const torch::Tensor& dz, const torch::Tensor& x, const torch::T
   cuda_check(launch_grouped_gemm_pair(GemmMode::kWgrad, GemmEpilogue::kStore, rows_map(dz, 64), rows_map(x, 64), rows_map(out, g.wide ? 32 : 128), nullptr, g, ctas, cur_stream()), "linear weight gradient");
 }
 
-// Forward on few rows.
-void dense_few(const torch::Tensor& weight, const torch::Tensor& x, const torch::Tensor& out, const DenseEpilogue& ep, uint64_t timeout_ns) {
-  const bool swiglu = ep.kind == GemmEpilogue::kSwiGLU;
+// The same on few rows, where that pays; false: nothing was done.
+bool dense_few(GemmMode mode, const torch::Tensor& weight, const torch::Tensor& x, const torch::Tensor& out, const DenseEpilogue& ep, uint64_t timeout_ns) {
+  const bool swiglu = ep.kind == GemmEpilogue::kSwiGLU, fwd = mode == GemmMode::kForward;
+  const int64_t red_blocks = (weight.size(fwd ? 1 : 0) + 63) / 64;
+  if (!few_pays(static_cast<int>(x.size(0)), static_cast<int>(out.size(1)), static_cast<int>(red_blocks), swiglu, sm_count(x))) return false;
   FewArgs a{};
   a.T = static_cast<int>(x.size(0)); a.columns = static_cast<int>(out.size(1));
-  a.red_blocks = static_cast<int>((weight.size(1) + 63) / 64);
+  a.red_blocks = static_cast<int>(red_blocks);
   const auto ptr = [](const torch::Tensor* t) { return t ? reinterpret_cast<__nv_bfloat16*>(t->data_ptr()) : nullptr; };
   a.bias = ptr(ep.bias); a.residual = ptr(ep.residual); a.out = ptr(&out); a.pre = ptr(ep.pre);
   a.residual_stride = ep.residual ? ep.residual->stride(0) : 0;
   a.status = dense_status();
   TORCH_CHECK(a.status != nullptr, "linear: no status block on this device");
   a.timeout_ns = timeout_ns;
-  cuda_check(launch_linear_few(ep.act, swiglu, rows_map(weight, swiglu ? 64 : 128), rows_map(x, few_box_rows(a.T)), a, sm_count(x), cur_stream()), "linear");
+  cuda_check(launch_linear_few(mode, ep.act, swiglu, rows_map(weight, swiglu || !fwd ? 64 : 128), rows_map(x, few_box_rows(a.T)), a, sm_count(x), cur_stream()), "linear");
+  return true;
 }
 
 struct LinearOut { torch::Tensor y, pre; };
@@ -390,8 +393,7 @@ LinearOut linear_forward(const torch::Tensor& x, const torch::Tensor& weight, co
     if (residual.has_value()) { rm = tma_rows(*residual, cols); ep.residual = &rm; }
   }
   if (pre) ep.pre = &o.pre;
-  if (few_pays(static_cast<int>(T), static_cast<int>(cols), static_cast<int>((K + 63) / 64), kind == LinearKind::kSwiGLU, sm_count(x))) dense_few(wm, xm, ym, ep, timeout_ns);
-  else dense_gemm(GemmMode::kForward, wm, xm, ym, ep, timeout_ns);
+  if (!dense_few(GemmMode::kForward, wm, xm, ym, ep, timeout_ns)) dense_gemm(GemmMode::kForward, wm, xm, ym, ep, timeout_ns);
   return o;
 }
 
@@ -453,7 +455,8 @@ struct Linear : torch::autograd::Function<Linear> {
         }
         if (want_x) {
           out[0] = torch::empty(shape, dy.options());
-          dense_gemm(GemmMode::kDgrad, tma_rows(saved[1], K), dz, out[0].view({T, K}), {}, timeout_ns);
+          const torch::Tensor wm = tma_rows(saved[1], K), dx = out[0].view({T, K});
+          if (!dense_few(GemmMode::kDgrad, wm, dz, dx, {}, timeout_ns)) dense_gemm(GemmMode::kDgrad, wm, dz, dx, {}, timeout_ns);
         }
         if (want_w) {
           out[1] = torch::empty({N, K}, dy.options());
