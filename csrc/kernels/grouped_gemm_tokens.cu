@@ -812,7 +812,7 @@ bool dense_is_cut(const TokDenseArgs& args, int ctas) { return dense_split(args,
 
 cudaError_t launch_dense_gemm(GemmMode mode, GemmEpilogue epi, const TokDenseMaps& maps, const TokDenseArgs& args, int ctas, cudaStream_t stream) {
   if (ctas < 2 || args.num_groups != 1 || args.dense_rows < 1 || args.features < 1 || args.m_tiles != div_up(args.features, kPairM) || args.red_blocks < 1 || args.band_tiles < 1) return cudaErrorInvalidValue;
-  if (args.tile_n != 64 && args.tile_n != 128 && args.tile_n != kTokAccN && (args.tile_n != 2 * kTokAccN || epi == GemmEpilogue::kLinear)) return cudaErrorInvalidValue;
+  if (args.tile_n < 64 || args.tile_n % 32 != 0 || (args.tile_n > kTokAccN && (args.tile_n != 2 * kTokAccN || epi == GemmEpilogue::kLinear))) return cudaErrorInvalidValue;
   if (args.granule != 32 || args.num_counters != 0 || args.status == nullptr || args.gate_counter != nullptr) return cudaErrorInvalidValue;
   if (dense_is_cut(args, ctas) && (args.partials == nullptr || args.counters == nullptr)) return cudaErrorInvalidValue;
   if (epi == GemmEpilogue::kSwiGLU && mode == GemmMode::kForward && args.features % kPairM == 0 && (args.keep_gate_up != 0) == (maps.c2 != nullptr)) return launch<GemmMode::kForward, GemmEpilogue::kSwiGLU>(maps, args, ctas, stream);

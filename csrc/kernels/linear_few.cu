@@ -5,7 +5,7 @@
 // rows through shared memory (TMA) as operand A of M = 128 MMAs, the tokens are N (rounded up to 16), so a decode step does no more work
 // than its tokens are. The CTAs' fp32 sums meet in distributed shared memory: each CTA adds up an equal share of the tile's features, in the order
 // of the reduction, and finishes them (bias, activation, residual, store): no counters, no scratch in global memory, nothing to
-// clear beforehand, one launch. 1 token, weight from HBM: 4096 -> 14336 21 us (5.6 TB/s), 14336 -> 4096 21 us, 4096 -> 4096 8.2 us (4.1 TB/s; 3 us of a launch are setting up, the
+// clear beforehand, one launch. 1 token, weight from HBM: 4096 -> 14336 21 us (5.6 TB/s), 14336 -> 4096 21 us, 4096 -> 4096 7.5 us (4.5 TB/s; 3 us of a launch are setting up, the
 // first loads and the sums' way). Stages leave room for two CTAs an SM, so that the next launch is set up while this one runs.
 // SwiGLU: the 128 rows are 64 gate rows and the 64 up rows of the same features.
 #include <algorithm>
@@ -206,14 +206,14 @@ __global__ void __launch_bounds__(kThreads) linear_few_kernel(const __grid_const
 }  // namespace
 
 // How many CTAs share a tile's reduction: as many as leave every CTA an SM, more where their parts are long (a CTA's stream alone does not fill an
-// SM's way to memory), eight only where there are few tiles or the parts are very long: a cluster of eight is harder to place, and its sums travel
-// further. us at 1, 2, 4, 8 parts: 32 tiles of 64 blocks (4096 -> 4096, 1 token) 14.6, 9.9, 8.2, 7.4, 64 tokens 20.5, 13.5, 10.7, 12.1; 56 tiles of 32
+// SM's way to memory), eight only where there are few tiles, the parts are very long or up to 16 tokens make the sums small: a cluster of eight is harder
+// to place, and its sums travel further. us at 1, 2, 4, 8 parts: 32 tiles of 64 blocks (4096 -> 4096, 1 token) 14.6, 9.9, 8.2, 7.4, 64 tokens 20.5, 13.5, 10.7, 12.1; 56 tiles of 32
 // (2048 -> 7168), 1 token 8.4, 6.6, 6.9, 10.1; 112 tiles of 64 (4096 -> 14336), 33 tokens 26.2, 21.9, 27.9, 35.9; 224 tiles of 16 (1024 -> 28672),
 // 1 token 11.9, 14.8, 21.4, 32.7; 32 tiles of 224 (14336 -> 4096), 33 tokens 66.5, 37.6, 25.6, 23.2.
 int few_parts(int tiles, int red_blocks, int n, int sms) {
   int parts = 1;
   while (parts < 8 && (n > 32 ? 4 : 2) * parts <= red_blocks &&
-         ((parts == 4 ? 4 : 2) * tiles * parts <= sms || (tiles * parts < sms && red_blocks >= 48 * parts)))
+         ((parts == 4 ? (n <= 16 ? 1 : 4) : 2) * tiles * parts <= sms || (tiles * parts < sms && red_blocks >= 48 * parts)))
     parts *= 2;
   return parts;
 }

@@ -89,6 +89,30 @@ struct TokSplit {
   FASTB_HD int share_of(int u) const { return static_cast<int>(((static_cast<long long>(u) + 1) * shares - 1) / cut_units()); }
 };
 
+// Most tokens of a tile for one weight matrix and `rows` tokens (TokDenseArgs), a multiple of 32 up to 256: of the widths that need no more rounds of the
+// GPU than 256 does (up to three), the one whose launch takes the fewest cycles by the counts above, with 600 a step of 32 tokens for the last tiles' way
+// out, if it saves a twenty-fifth. Narrower tiles keep more pairs busy, and spare the exchange of a cut round. us, 256 -> this: 1235 x 1000 -> 2760
+// (55 tiles, 66 of 224) 14.5 -> 13.9, 600 x 4096 -> 4096 (48, 64 of 160) 28.4 -> 22.2, 1500 x 8192 -> 2048 (48, 72 of 192) 47.5 -> 40.9, SwiGLU of 500 x 7168 -> 4096
+// (32, 64 of 128) 35.5 -> 30.7, 700 x 2048 -> 7168 (84 in two rounds, 140 of 160) 32.5 -> 27.2; more rounds lose: 3000 x 256 -> 3000 in three instead of two 13.3 -> 15.6.
+inline int tok_dense_tile(int rows, int m_tiles, int kb_tile, int pairs) {
+  const int fewest = tok_tiles(ceil_to(rows, 32), kTokAccN);
+  const long long rounds = (static_cast<long long>(fewest) * m_tiles + pairs - 1) / pairs;
+  if (rounds > 3) return kTokAccN;
+  int best = kTokAccN;
+  long long full_cycles = 0, best_cycles = 0;
+  for (int t = fewest; static_cast<long long>(t) * m_tiles <= rounds * pairs; ++t) {
+    const int n = t == fewest ? kTokAccN : ceil_to(div_up(rows, t), 32), tiles = tok_tiles(ceil_to(rows, 32), n) * m_tiles, widest = tok_tile_size(ceil_to(rows, 32), n);
+    if (n < 64) break;
+    const TokSplit s = TokSplit::make(tiles, kb_tile, pairs, widest, tiles > m_tiles);
+    const long long block = tok_block_cycles(widest);
+    long long cycles = div_up(s.whole_tiles, pairs) * kb_tile * block + widest / 32 * 600;
+    if (s.cut_tiles > 0) cycles += (s.stream ? s.cut_units() / s.shares : div_up(kb_tile, s.shares)) * block + tok_exchange_cycles(widest, s.stream ? 2 : s.shares);
+    if (t == fewest) full_cycles = best_cycles = cycles;
+    if (cycles < best_cycles && 25 * cycles <= 24 * full_cycles) { best = n; best_cycles = cycles; }
+  }
+  return best;
+}
+
 // One pair's segments in order: tile, first block, end block, number of parts of the tile, my part, and the pairs that do the
 // parts: first_pair + j * pair_step for part j.
 struct TokSegment { int tile, kb0, kb1, parts, part, first_pair, pair_step; };

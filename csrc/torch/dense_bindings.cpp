@@ -1,5 +1,6 @@
 // Bindings of the dense side of a block: row norm, balance loss, linear layers. Their kernels run on the current stream of the
 // tensors' own device, whichever device is current.
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -42,6 +43,10 @@ variable_list once(const char* op, const variable_list& incoming, variable_list 
 
 bool row_type(const torch::Tensor& t) { return t.scalar_type() == torch::kBFloat16 || t.scalar_type() == torch::kFloat32; }
 
+// A new contiguous tensor on the device of `like`, without the dispatcher's way there (half of what a call of a few rows costs the host is allocation).
+torch::Tensor fresh(at::IntArrayRef shape, const torch::Tensor& like, c10::ScalarType type) { return at::detail::empty_cuda(shape, type, like.device(), c10::nullopt); }
+torch::Tensor fresh(at::IntArrayRef shape, const torch::Tensor& like) { return fresh(shape, like, like.scalar_type()); }
+
 // Rows of t as a matrix whose rows are contiguous; only what cannot be seen as one is copied.
 torch::Tensor as_rows(const torch::Tensor& t, int64_t cols) {
   torch::Tensor m = t.dim() == 2 ? t : t.reshape({-1, cols});
@@ -71,24 +76,24 @@ Norm row_norm(const torch::Tensor& x, const torch::Tensor& weight, double eps, c
   a.weight = weight.data_ptr();
   a.rows_bf16 = x.scalar_type() == torch::kBFloat16; a.weight_bf16 = weight.scalar_type() == torch::kBFloat16;
   a.eps = static_cast<float>(eps);
-  torch::Tensor y = torch::empty(x.sizes(), x.options()), rm;
+  torch::Tensor y = fresh(x.sizes(), x), rm;
   torch::Tensor h, q, scales, rstd;
   a.y = y.data_ptr();
   if (residual.has_value()) {
     rm = as_rows(*residual, H);
     a.residual = rm.data_ptr(); a.residual_stride = rm.stride(0);
-    h = torch::empty(x.sizes(), x.options());
+    h = fresh(x.sizes(), x);
     a.h = h.data_ptr();
   }
   if (quantise) {
-    q = torch::empty(x.sizes(), x.options().dtype(torch::kUInt8));
+    q = fresh(x.sizes(), x, torch::kUInt8);
     auto shape = x.sizes().vec();
     shape.back() = H / 128;
-    scales = torch::empty(shape, x.options().dtype(torch::kFloat32));
+    scales = fresh(shape, x, torch::kFloat32);
     a.q = q.data_ptr<uint8_t>(); a.scales = scales.data_ptr<float>();
   }
   if (keep) {
-    rstd = torch::empty({xm.size(0)}, x.options().dtype(torch::kFloat32));
+    rstd = fresh({xm.size(0)}, x, torch::kFloat32);
     a.rstd = rstd.data_ptr<float>();
   }
   cuda_check(launch_row_norm(a, sm_count(x), cur_stream()), "add_rms_norm");
@@ -108,11 +113,11 @@ std::tuple<torch::Tensor, torch::Tensor> row_norm_bwd(const torch::Tensor& h, co
   a.dy = ym.data_ptr(); a.dh = dm.defined() ? dm.data_ptr() : nullptr;
   a.T = rows_of(hm, "add_rms_norm"); a.H = static_cast<int>(H);
   a.rows_bf16 = h.scalar_type() == torch::kBFloat16; a.weight_bf16 = weight.scalar_type() == torch::kBFloat16;
-  auto dx = torch::empty(h.sizes(), h.options());
+  auto dx = fresh(h.sizes(), h);
   if (a.T == 0) return {dx, torch::zeros({H}, weight.options())};
-  auto dweight = torch::empty({H}, weight.options());
+  auto dweight = fresh({H}, weight);
   const int blocks = row_norm_bwd_blocks(a, sm_count(h));
-  auto partials = torch::empty({blocks, H}, h.options().dtype(torch::kFloat32));
+  auto partials = fresh({blocks, H}, h, torch::kFloat32);
   a.dx = dx.data_ptr(); a.dweight = dweight.data_ptr(); a.partials = partials.data_ptr<float>();
   cuda_check(launch_row_norm_bwd(a, blocks, cur_stream()), "add_rms_norm backward");
   return {dx, dweight};
@@ -124,7 +129,7 @@ torch::Tensor dequantise_rows(const torch::Tensor& q, const torch::Tensor& scale
   TORCH_CHECK(scales.device() == q.device() && scales.scalar_type() == torch::kFloat32 && scales.is_contiguous() && scales.dim() == q.dim() && scales.numel() * 128 == q.numel() &&
               scales.size(-1) * 128 == q.size(-1), "dequantise_rows: scales must be contiguous fp32 [..., hidden / 128] on q's device");
   c10::cuda::CUDAGuard guard(q.device());
-  auto out = torch::empty(q.sizes(), q.options().dtype(torch::kBFloat16));
+  auto out = fresh(q.sizes(), q, torch::kBFloat16);
   const int H = static_cast<int>(q.size(-1));
   cuda_check(launch_dequant_fp8(q.data_ptr<uint8_t>(), scales.data_ptr<float>(), reinterpret_cast<__nv_bfloat16*>(out.data_ptr()), q.numel() / H, H, nullptr, cur_stream()), "dequantise_rows");
   return out;
@@ -193,13 +198,12 @@ Balance balance(const torch::Tensor& logits, const torch::Tensor& topk_idx, cons
   a.mask = mm.defined() ? reinterpret_cast<const unsigned char*>(mm.data_ptr()) : nullptr;
   a.T = rows_of(lm, "balance_loss"); a.E = static_cast<int>(E); a.K = static_cast<int>(topk_idx.size(-1)); a.sigmoid = sigmoid;
   TORCH_CHECK(static_cast<int64_t>(a.T) * a.K <= 0x7fffffff, "balance_loss: more than 2^31 - 1 choices");
-  const auto f32 = logits.options().dtype(torch::kFloat32), i32 = logits.options().dtype(torch::kInt32);
-  Balance b{torch::empty({}, f32), torch::empty({E}, i32), torch::empty({E + 1}, i32)};
+  Balance b{fresh(at::IntArrayRef{}, logits, torch::kFloat32), fresh({E}, logits, torch::kInt32), fresh({E + 1}, logits, torch::kInt32)};
   a.loss = b.loss.data_ptr<float>(); a.counts = b.counts.data_ptr<int>(); a.kept = b.kept.data_ptr<int>();
   const int blocks = balance_blocks(a, sm_count(logits));
   torch::Tensor scratch;
   if (blocks > 1) {
-    scratch = torch::empty({blocks, 2 * E + 1}, i32);
+    scratch = fresh({blocks, 2 * E + 1}, logits, torch::kInt32);
     a.chosen = scratch.data_ptr<int>();
     a.sums = reinterpret_cast<float*>(a.chosen + blocks * (E + 1));
   }
@@ -211,8 +215,7 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
   static variable_list forward(AutogradContext* ctx, const torch::Tensor& logits, const torch::Tensor& topk_idx, const OptTensor& mask, bool sigmoid) {
     Balance b = balance(logits, topk_idx, mask, sigmoid);
     ctx->set_materialize_grads(false);
-    ctx->saved_data["k"] = topk_idx.size(-1);
-    ctx->saved_data["sigmoid"] = sigmoid;
+    ctx->saved_data["kept"] = std::vector<int64_t>{topk_idx.size(-1), sigmoid};
     ctx->save_for_backward({logits, mask_bytes(mask), b.kept});
     ctx->mark_non_differentiable({b.counts});
     return {b.loss, b.counts};
@@ -220,17 +223,18 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor()};
     const auto saved = ctx->get_saved_variables();
+    const std::vector<int64_t> kept = ctx->saved_data["kept"].toIntVector();
     const torch::Tensor& logits = saved[0];
     torch::Tensor dlogits;
     {
       torch::NoGradGuard no_grad;
       c10::cuda::CUDAGuard guard(logits.device());
       const torch::Tensor lm = as_rows(logits, logits.size(-1)), dloss = grads[0].to(torch::kFloat32);
-      dlogits = torch::empty(logits.sizes(), logits.options());
+      dlogits = fresh(logits.sizes(), logits);
       BalanceBwdArgs a{};
       a.logits = lm.data_ptr(); a.stride = lm.stride(0); a.logits_bf16 = logits.scalar_type() == torch::kBFloat16;
       a.mask = saved[1].defined() ? reinterpret_cast<const unsigned char*>(saved[1].data_ptr()) : nullptr;
-      a.T = static_cast<int>(lm.size(0)); a.E = static_cast<int>(logits.size(-1)); a.K = static_cast<int>(ctx->saved_data["k"].toInt()); a.sigmoid = ctx->saved_data["sigmoid"].toBool();
+      a.T = static_cast<int>(lm.size(0)); a.E = static_cast<int>(logits.size(-1)); a.K = static_cast<int>(kept[0]); a.sigmoid = static_cast<int>(kept[1]);
       a.kept = saved[2].data_ptr<int>(); a.dloss = dloss.data_ptr<float>(); a.dlogits = dlogits.data_ptr();
       cuda_check(launch_balance_bwd(a, sm_count(logits), cur_stream()), "balance_loss backward");
     }
@@ -280,7 +284,7 @@ void dense_gemm(GemmMode mode, const torch::Tensor& weight, const torch::Tensor&
   a.m_tiles = static_cast<int>((features + 255) / 256); a.red_blocks = static_cast<int>((reduction + 63) / 64);
   a.granule = 32;
   // Where all tokens fit a narrow tile, narrow tiles leave shared memory to the weights in flight.
-  a.tile_n = a.dense_rows <= 64 ? 64 : a.dense_rows <= 128 ? 128 : 256;
+  a.tile_n = a.dense_rows <= 64 ? 64 : a.dense_rows <= 128 ? 128 : gemm::tok_dense_tile(a.dense_rows, a.m_tiles, a.red_blocks, ctas / 2);
   GemmEpilogue kind = ep.kind;
   const bool plain = ep.kind == GemmEpilogue::kLinear && ep.act == Activation::kNone && !ep.bias && !ep.residual && !ep.pre;
   if ((plain || ep.kind == GemmEpilogue::kSwiGLU) && a.tile_n == 256 &&
@@ -317,7 +321,7 @@ void dense_gemm(GemmMode mode, const torch::Tensor& weight, const torch::Tensor&
   }
   torch::Tensor partials, counters;
   if (dense_is_cut(a, ctas)) {
-    partials = torch::empty({tok_partial_floats(ctas, a.tile_n)}, x.options().dtype(torch::kFloat32));
+    partials = fresh({tok_partial_floats(ctas, a.tile_n)}, x, torch::kFloat32);
     counters = torch::zeros({tok_counters(ctas)}, x.options().dtype(torch::kInt32));
     a.partials = partials.data_ptr<float>();
     a.counters = reinterpret_cast<unsigned int*>(counters.data_ptr<int>());
@@ -376,11 +380,11 @@ LinearOut linear_forward(const torch::Tensor& x, const torch::Tensor& weight, co
   shape.back() = cols;
   TORCH_CHECK(!residual.has_value() || (residual->device() == x.device() && residual->scalar_type() == bf && residual->sizes() == at::IntArrayRef(shape)), "linear: residual must be bf16 with the output's shape, on x's device");
   c10::cuda::CUDAGuard guard(x.device());
-  LinearOut o{torch::empty(shape, x.options()), {}};
+  LinearOut o{fresh(shape, x), {}};
   const int64_t T = x.numel() / K;
   TORCH_CHECK(T <= 1 << 30, "linear: more than 2^30 rows");
   const bool pre = keep && kind != LinearKind::kNone;
-  if (pre) o.pre = torch::empty({T, N}, x.options());
+  if (pre) o.pre = fresh({T, N}, x);
   if (T == 0) return o;
   const torch::Tensor xm = tma_rows(x, K), wm = kind == LinearKind::kSwiGLU && !weight.is_contiguous() ? weight.contiguous() : tma_rows(weight, K), ym = o.y.view({T, cols});
   torch::Tensor rm, bm;
@@ -402,25 +406,24 @@ struct Linear : torch::autograd::Function<Linear> {
     const bool through = x.requires_grad() || weight.requires_grad() || wants_grad(bias);   // the gradient goes past the activation
     LinearOut o = linear_forward(x, weight, bias, static_cast<LinearKind>(kind), residual, through, timeout_ns);
     ctx->set_materialize_grads(false);
-    ctx->saved_data["kind"] = kind;
-    ctx->saved_data["timeout_ns"] = timeout_ns;
-    ctx->saved_data["bias"] = bias.has_value();
-    ctx->saved_data["residual"] = residual.has_value();
+    // all numbers in one entry: every entry is a hash of its name on the way in and out
+    std::vector<int64_t> kept{kind, timeout_ns, bias.has_value(), residual.has_value(), weight.size(0), weight.size(1)};
+    kept.insert(kept.end(), x.sizes().begin(), x.sizes().end());
+    ctx->saved_data["kept"] = std::move(kept);
     ctx->save_for_backward({weight.requires_grad() ? x : torch::Tensor(), x.requires_grad() ? weight : torch::Tensor(), o.pre});
-    ctx->saved_data["outputs"] = weight.size(0);
-    ctx->saved_data["inputs"] = weight.size(1);
-    ctx->saved_data["shape"] = x.sizes().vec();
     return {o.y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list out(6);
     if (!grads[0].defined()) return out;
     const auto saved = ctx->get_saved_variables();
-    const bool has_bias = ctx->saved_data["bias"].toBool(), has_residual = ctx->saved_data["residual"].toBool();
+    const std::vector<int64_t> kept = ctx->saved_data["kept"].toIntVector();
+    const auto kind = static_cast<LinearKind>(kept[0]);
+    const uint64_t timeout_ns = static_cast<uint64_t>(kept[1]);
+    const bool has_bias = kept[2], has_residual = kept[3];
+    const int64_t N = kept[4], K = kept[5];
+    const at::IntArrayRef shape(kept.data() + 6, kept.size() - 6);   // of x
     const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1), want_b = has_bias && ctx->needs_input_grad(2), want_r = has_residual && ctx->needs_input_grad(has_bias ? 3 : 2);
-    const auto kind = static_cast<LinearKind>(ctx->saved_data["kind"].toInt());
-    const uint64_t timeout_ns = static_cast<uint64_t>(ctx->saved_data["timeout_ns"].toInt());
-    const int64_t N = ctx->saved_data["outputs"].toInt(), K = ctx->saved_data["inputs"].toInt();
     if (want_r) out[3] = grads[0];
     if (want_x || want_w || want_b) {
       torch::NoGradGuard no_grad;
@@ -428,7 +431,6 @@ struct Linear : torch::autograd::Function<Linear> {
       const torch::Tensor dy = tma_rows(grads[0], kind == LinearKind::kSwiGLU ? N / 2 : N);
       const int64_t T = dy.size(0);
       TORCH_CHECK(dy.scalar_type() == torch::kBFloat16, "linear backward: the gradient must be bf16");
-      const auto shape = ctx->saved_data["shape"].toIntVector();
       if (T == 0) {
         if (want_x) out[0] = torch::zeros(shape, dy.options());
         if (want_w) out[1] = torch::zeros({N, K}, dy.options());
@@ -437,29 +439,29 @@ struct Linear : torch::autograd::Function<Linear> {
         torch::Tensor dz = dy;
         if (kind == LinearKind::kSwiGLU) {
           const torch::Tensor d = dy.contiguous();
-          dz = torch::empty({T, N}, dy.options());
+          dz = fresh({T, N}, dy);
           cuda_check(launch_swiglu_bwd(reinterpret_cast<const __nv_bfloat16*>(saved[2].data_ptr()), reinterpret_cast<const __nv_bfloat16*>(d.data_ptr()), reinterpret_cast<__nv_bfloat16*>(dz.data_ptr()),
                                        T, static_cast<int>(N / 2), nullptr, cur_stream()), "linear backward: swiglu");
         } else if (kind != LinearKind::kNone || want_b) {
           const torch::Tensor d = dy.contiguous();
           torch::Tensor partials;
           const int blocks = linear_dz_blocks(static_cast<int>(T), static_cast<int>(N), sm_count(dy));
-          if (kind != LinearKind::kNone) dz = torch::empty({T, N}, dy.options());
+          if (kind != LinearKind::kNone) dz = fresh({T, N}, dy);
           if (want_b) {
-            out[2] = torch::empty({N}, dy.options());
-            partials = torch::empty({blocks, N}, dy.options().dtype(torch::kFloat32));
+            out[2] = fresh({N}, dy);
+            partials = fresh({blocks, N}, dy, torch::kFloat32);
           }
           const auto ptr = [](const torch::Tensor& t) { return t.defined() ? reinterpret_cast<__nv_bfloat16*>(t.data_ptr()) : nullptr; };
           cuda_check(launch_linear_dz(static_cast<Activation>(kind), ptr(d), ptr(saved[2]), kind != LinearKind::kNone ? ptr(dz) : nullptr, want_b ? partials.data_ptr<float>() : nullptr, static_cast<int>(T),
                                       static_cast<int>(N), blocks, ptr(out[2]), cur_stream()), "linear backward: activation");
         }
         if (want_x) {
-          out[0] = torch::empty(shape, dy.options());
+          out[0] = fresh(shape, dy);
           const torch::Tensor wm = tma_rows(saved[1], K), dx = out[0].view({T, K});
           if (!dense_few(GemmMode::kDgrad, wm, dz, dx, {}, timeout_ns)) dense_gemm(GemmMode::kDgrad, wm, dz, dx, {}, timeout_ns);
         }
         if (want_w) {
-          out[1] = torch::empty({N, K}, dy.options());
+          out[1] = fresh({N, K}, dy);
           dense_wgrad(dz, tma_rows(saved[0], K), out[1], timeout_ns);
         }
       }
