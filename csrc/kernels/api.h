@@ -110,7 +110,8 @@ struct GemmArgs {
                            // over them up to a multiple of 64
   int gate_tile_rows;      // 0: gate_counter / gate_target are indexed by group; > 0: by (row of the grouped matrix) / gate_tile_rows
   int gate_slots;          // entries of gate_counter / gate_target (indices are clamped to the last one)
-  int dense_rows;          // weight gradients without group_off: one group of this many rows
+  int dense_rows;          // weight gradients without group_off: one group of this many rows, or num_groups equal slices of them ...
+  float* sums;             // ... whose sums go here, fp32 [num_groups][fixed_m_tiles][tiles_n][two halves][64 groups of 4 columns][128 rows][4] (direct_epilogue)
   int wide;                // CTA-pair weight gradients: tiles of 512 columns (tiles_n counts those) instead of 256; map_c has boxes {64,32}
 };
 
@@ -481,6 +482,8 @@ struct BalanceBwdArgs {
 cudaError_t launch_balance_bwd(const BalanceBwdArgs& a, int sms, cudaStream_t stream);
 // out[c] = sum over `blocks` rows of partials [blocks][n], in a fixed order; bf16 or fp32.
 cudaError_t launch_fold_columns(const float* partials, int blocks, int n, bool as_bf16, void* out, cudaStream_t stream);
+// out [rows, cols] bf16 = the slices' sums (GemmArgs::sums) added up in order; cols % 8 == 0.
+cudaError_t launch_fold_slices(const float* sums, int slices, int m_tiles, int n_tiles, __nv_bfloat16* out, int rows, int cols, cudaStream_t stream);
 // dz = dy * act'(z) [T, N] (kNone: dz is dy, nothing is written) and, with partials [blocks][N], dbias [N] = the column sums of dz. N % 8 == 0.
 int linear_dz_blocks(int T, int N, int sms);
 cudaError_t launch_linear_dz(Activation act, const __nv_bfloat16* dy, const __nv_bfloat16* z, __nv_bfloat16* dz, float* partials, int T, int N, int blocks, __nv_bfloat16* dbias, cudaStream_t stream);

@@ -64,6 +64,23 @@ __device__ __forceinline__ void epilogue_store_row(__nv_bfloat16* crow, uint32_t
   }
 }
 
+// The same as fp32 sums, [64 groups of four columns][128 rows]: `at` is row r of the first group. A warp's stores are contiguous; row by row in global memory
+// every one of them touched 32 lines.
+__device__ __forceinline__ void epilogue_sums(float4* at, uint32_t t_row, bool zero) {
+#pragma unroll 1
+  for (int c = 0; c < BN / 32; ++c) {
+    uint32_t r[32];
+    if (!zero) { ptx::tmem_ld_32x32(t_row + c * 32, r); ptx::tmem_wait_ld(); }
+    else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) r[i] = 0;
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      __stcg(at + (c * 8 + q) * 128, make_float4(__uint_as_float(r[4 * q]), __uint_as_float(r[4 * q + 1]), __uint_as_float(r[4 * q + 2]), __uint_as_float(r[4 * q + 3])));
+  }
+}
+
 // SwiGLU: the 256 columns of a tile are [128 gate | 128 up] of the same 128 features.
 __device__ __forceinline__ void epilogue_swiglu_row(__nv_bfloat16* arow, __nv_bfloat16* gurow, uint32_t t_row) {
 #pragma unroll 1

@@ -65,11 +65,12 @@ constexpr int kWideThreads = 32 * kWideFirstEpiWarp + 2 * 32 * kEpiWarps;
 constexpr int kLaunchRegs = 168, kOtherRegs = 72, kEpilogueRegs = 216;   // a thread
 static_assert(kOtherRegs + 2 * kEpilogueRegs <= 3 * kLaunchRegs && kWideThreads * kLaunchRegs <= 65536, "what the epilogue takes, the others have given");
 
+constexpr int kMaxSlices = 8;        // of the rows of one matrix (dense weight gradients)
 struct __align__(8) SmemCtl {
   uint64_t full[kStages], empty[kStages], acc_full[kAccStages], acc_empty[kAccStages], q_full[kQStages], q_empty[kQStages];
   uint32_t tmem_base;
   int abort_flag;
-  int dense_off[2];                // the group table of a launch without one
+  int dense_off[kMaxSlices + 1];   // the group table of a launch without one
 };
 constexpr int kSmemBytes = kStages * kStageBytes + kEpiBytes + 1024 + sizeof(SmemCtl);
 constexpr int kSmemBytesFp8 = kStagesFp8 * kStageBytes + kQStages * kQBytes + kEpiBytes + 1024 + sizeof(SmemCtl);
@@ -124,8 +125,8 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     for (int a = 0; a < kAccStages; ++a) { mbar_init(&ctl->acc_full[a], 1); mbar_init(&ctl->acc_empty[a], 2 * kEpiWarps); }
     for (int q = 0; q < kQStages; ++q) { mbar_init(&ctl->q_full[q], 1); mbar_init(&ctl->q_empty[q], 1); }
     ctl->abort_flag = 0;
-    ctl->dense_off[0] = 0;
-    ctl->dense_off[1] = (p.dense_rows + BK - 1) / BK * BK;   // rows past the real ones come in as zeros: they lie outside the matrices
+    if (MODE == GemmMode::kWgrad && p.group_off == nullptr)   // rows past the real ones come in as zeros: they lie outside the matrices
+      for (int g = 0; g <= p.num_groups; ++g) ctl->dense_off[g] = static_cast<int>(static_cast<long long>((p.dense_rows + BK - 1) / BK) * g / p.num_groups) * BK;
     mbar_fence_init();
     prefetch_tmap(&map_a);
     prefetch_tmap(&map_b);
@@ -423,7 +424,10 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
       // first output row of this CTA's half (TMA store coordinate)
       const int c_row0 = (MODE == GemmMode::kWgrad ? tc.g * p.c_rows_per_group : tc.row0) + tc.m_idx * TILE_M + static_cast<int>(cta) * PM;
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + a * BN;
-      if (!TMA_EPI) {
+      if (!TMA_EPI && p.sums != nullptr) {
+        const long long half = ((static_cast<long long>(tc.g) * p.fixed_m_tiles + tc.m_idx) * p.tiles_n + tc.n_idx) * 2 + cta;
+        epilogue_sums(reinterpret_cast<float4*>(p.sums + half * (PM * BN)) + r, t_row, empty_reduction);
+      } else if (!TMA_EPI) {
         epilogue_store_row(p.c + (static_cast<long long>(c_row0) + r) * p.ldc + static_cast<long long>(tc.n_idx) * BN, t_row, empty_reduction);
       } else if (EPI == GemmEpilogue::kStore) {
         epilogue_store_tma(ring, &map_c, tc.n_idx * BN, c_row0, r, t_row, empty_reduction);
@@ -471,7 +475,9 @@ cudaError_t launch_kernel(Kernel kern, int threads, int smem, const CUtensorMap&
 cudaError_t launch_grouped_gemm_pair(GemmMode mode, GemmEpilogue epi, const CUtensorMap& map_a, const CUtensorMap& map_b, const CUtensorMap& map_c,
                                      const CUtensorMap* map_c2, const GemmArgs& args, int ctas, cudaStream_t stream) {
   if (ctas < 2) return cudaErrorInvalidValue;
-  if (args.group_off == nullptr && (mode != GemmMode::kWgrad || args.num_groups != 1 || args.dense_rows < 0 || args.direct_epilogue)) return cudaErrorInvalidValue;
+  if (args.group_off == nullptr && (mode != GemmMode::kWgrad || args.num_groups < 1 || args.num_groups > kMaxSlices || args.dense_rows < 0 || (args.num_groups > 1) != (args.sums != nullptr))) return cudaErrorInvalidValue;
+  if (args.sums != nullptr && args.group_off != nullptr) return cudaErrorInvalidValue;
+  if (args.group_off == nullptr && (args.direct_epilogue != 0) != (args.sums != nullptr)) return cudaErrorInvalidValue;   // rows of bf16 written one by one would pass the matrix's end
   if ((args.c2 != nullptr) != (map_c2 != nullptr)) return cudaErrorInvalidValue;
   const CUtensorMap& c2 = map_c2 ? *map_c2 : map_c;  // unused by the kernel when args.c2 is null
   if (args.a_scales != nullptr) {

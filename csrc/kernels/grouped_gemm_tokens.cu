@@ -74,18 +74,19 @@ struct __align__(8) TokCtl {
   int abort_flag, last_arrived, widest, share_weights;
   int base[kTokPrefix + 1];                         // tiles of the groups before entry i
 };
-// Boxes of half of the ring. Dense stores have two buffers of two there; kLinear has the room of one for each of its four warps.
+// Boxes of half of the ring. Dense stores have two buffers of two there; kLinear has the room of one for each of its four warps, of two with the pre-activation.
 __host__ __device__ constexpr int epi_boxes(GemmEpilogue e, bool dense = false) { return e == GemmEpilogue::kStore ? (dense ? 4 : 2) : e == GemmEpilogue::kSwiGLU ? 3 : 4; }
+__host__ __device__ constexpr int ring_half(GemmEpilogue e, bool dense, bool keep_pre) { return epi_boxes(e, dense) * (e == GemmEpilogue::kLinear && keep_pre ? 2 : 1) * kBox; }
 constexpr int kSmemLimit = 227 * 1024;
-constexpr int other_bytes(GemmEpilogue e, bool dense) { return 2 * epi_boxes(e, dense) * kBox + 1024 + static_cast<int>(sizeof(TokCtl)); }
+constexpr int other_bytes(GemmEpilogue e, bool dense, bool keep_pre) { return 2 * ring_half(e, dense, keep_pre) + 1024 + static_cast<int>(sizeof(TokCtl)); }
 // Operand stages that fit. Tiles of up to 256 tokens: 6 of 32 KiB. Where few tokens meet the weights, the loop is bound by
 // HBM and wants weight bytes in flight: tiles of up to 64 tokens leave room for 10 stages of 20 KiB.
-constexpr int stages_for(GemmEpilogue e, int tile_n, bool dense = false) {
-  const int n = (kSmemLimit - other_bytes(e, dense)) / stage_bytes(tile_n);
+constexpr int stages_for(GemmEpilogue e, int tile_n, bool dense = false, bool keep_pre = false) {
+  const int n = (kSmemLimit - other_bytes(e, dense, keep_pre)) / stage_bytes(tile_n);
   return n < kMaxStages ? n : kMaxStages;
 }
-constexpr int smem_bytes(GemmEpilogue e, int tile_n, bool dense) { return stages_for(e, tile_n, dense) * stage_bytes(tile_n) + other_bytes(e, dense); }
-static_assert(stages_for(GemmEpilogue::kSwiGLUBwd, kTokAccN) == 6 && stages_for(GemmEpilogue::kStore, kTokAccN, true) == 6 && stages_for(GemmEpilogue::kSwiGLU, 64) == 10, "stages at both ends of the range");
+constexpr int smem_bytes(GemmEpilogue e, int tile_n, bool dense, bool keep_pre) { return stages_for(e, tile_n, dense, keep_pre) * stage_bytes(tile_n) + other_bytes(e, dense, keep_pre); }
+static_assert(stages_for(GemmEpilogue::kSwiGLUBwd, kTokAccN) == 6 && stages_for(GemmEpilogue::kStore, kTokAccN, true) == 6 && stages_for(GemmEpilogue::kLinear, kTokAccN, true, true) == 5 && stages_for(GemmEpilogue::kSwiGLU, 64) == 10, "stages at both ends of the range");
 static_assert(stages_for(GemmEpilogue::kSwiGLUBwd, 2 * kTokAccN) == 4, "stages of wide tiles");
 static_assert(kAccStages * kTokAccN <= kTmemCols, "two accumulators of 256 columns: of two tiles in turn, or both of a wide tile");
 static_assert(kTokPartialFloats == kHalfM * kTokAccN, "a partial is one CTA's accumulator");
@@ -146,7 +147,9 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
   uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int stages = p.stages, stage_size = stage_bytes(p.tile_n);
   uint8_t* ring = tiles + stages * stage_size;
-  TokCtl* ctl = reinterpret_cast<TokCtl*>(ring + 2 * kRing);
+  bool keep_pre = false;
+  if constexpr (EPI == GemmEpilogue::kLinear) keep_pre = p.keep_pre != 0;
+  TokCtl* ctl = reinterpret_cast<TokCtl*>(ring + 2 * ring_half(EPI, DENSE, keep_pre));
   if (!p.early) grid_dependency_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cta = static_cast<int>(cluster_cta_rank());  // 0 = leader
@@ -566,10 +569,11 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
         // comes in by TMA while the one before it is worked on, and is overwritten by what goes out. Only short reductions are bound by this: 8192 x
         // 64 -> 8192 with relu 74.7 us with boxes shared by two warps and two barriers a step, 58.5 so; from a reduction of 1024 on the products are.
         static_assert(GROUPS == 2, "half of the steps a group");
-        const int f0 = feat0 + quarter * 32, slots = p.keep_pre ? 1 : 2, me = group * 4 + quarter;
+        const int f0 = feat0 + quarter * 32, me = group * 4 + quarter, slot_bytes = (keep_pre ? 2 : 1) * kWarpBox;
         const bool mine = f0 < p.features, residual = p.has_residual && mine;
-        uint8_t* const boxes = ring + me * 2 * kWarpBox;        // two boxes: buffers in turn, or the output's and the pre-activation's
-        auto slot = [&](uint32_t i) { return boxes + (slots == 2 ? i & 1u : 0u) * kWarpBox; };
+        // Two buffers in turn: a box of the residual and the output, and one of the pre-activation (with a single buffer of both 2985 x 280 -> 6184 took 54 us, with a
+        // stage less and two 48).
+        auto slot = [&](uint32_t i) { return ring + (me * 2 + static_cast<int>(i & 1u)) * slot_bytes; };
         auto load_residual = [&](int st, uint32_t i) {         // lane 0 only
           uint64_t* bar = &ctl->epi_load[2 * me + (i & 1u)];
           mbar_arrive_expect_tx(bar, kWarpBox);
@@ -577,7 +581,7 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
         };
         if (residual && lane == 0) {
           bulk_wait_read<0>();
-          for (int i = 0; i < slots; ++i)
+          for (int i = 0; i < 2; ++i)
             if (first_step + i * GROUPS < steps_of(0)) load_residual(first_step + i * GROUPS, ring_n + i);
         }
         float bias[4];                                          // of features lane / 4 + 8 i
@@ -604,10 +608,10 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
             if (!(ok = mbar_wait_bounded(&ctl->epi_load[2 * me + (ring_n & 1u)], (load_ph >> (ring_n & 1u)) & 1u, abort_flag, p.status, 500, p.timeout_ns))) break;
             load_ph ^= 1u << (ring_n & 1u);
           } else {
-            if (lane == 0) { if (slots == 2) bulk_wait_read<1>(); else bulk_wait_read<0>(); }   // the store that reads this slot is done with it
+            if (lane == 0) bulk_wait_read<1>();   // the store that reads this slot is done with it
             __syncwarp();
           }
-          if (p.keep_pre) {
+          if (keep_pre) {
             to_bf16(r, h);
             put_mine(sb + kWarpBox);
           }
@@ -640,10 +644,10 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
           if (lane == 0) {
             if (mine) {
               tma_store_2d(&map_c, slot(ring_n), f0, row_of(0, st));
-              if (p.keep_pre) tma_store_2d(&map_c3, boxes + kWarpBox, f0, row_of(0, st));
+              if (keep_pre) tma_store_2d(&map_c3, slot(ring_n) + kWarpBox, f0, row_of(0, st));
             }
             bulk_commit();
-            if (residual && st + slots * GROUPS < steps_of(0)) { bulk_wait_read<0>(); load_residual(st + slots * GROUPS, ring_n + slots); }
+            if (residual && st + 2 * GROUPS < steps_of(0)) { bulk_wait_read<0>(); load_residual(st + 2 * GROUPS, ring_n + 2); }
           }
           ++ring_n;
         }
@@ -762,8 +766,10 @@ template <GemmMode MODE, GemmEpilogue EPI, int SUB, class Args>
 cudaError_t launch_sub(const TokGemmMaps& m, const CUtensorMap* c3, Args args, int ctas, cudaStream_t stream) {
   auto kern = grouped_gemm_tokens_kernel<MODE, EPI, SUB, Args>;
   constexpr bool dense = tok_dense<Args>::value;
-  args.stages = stages_for(EPI, args.tile_n, dense);
-  const int smem = smem_bytes(EPI, args.tile_n, dense);
+  bool keep_pre = false;
+  if constexpr (EPI == GemmEpilogue::kLinear) keep_pre = args.keep_pre != 0;
+  args.stages = stages_for(EPI, args.tile_n, dense, keep_pre);
+  const int smem = smem_bytes(EPI, args.tile_n, dense, keep_pre);
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};

@@ -82,7 +82,42 @@ __global__ void __launch_bounds__(kThreads) linear_dz_kernel(const __nv_bfloat16
   if (column < N) partials[static_cast<size_t>(blockIdx.y) * N + column] = v;
 }
 
+// A weight gradient whose rows were shared out: a warp has 32 rows of a half tile and 16 of its columns, a lane a row.
+__global__ void __launch_bounds__(kThreads) fold_slices_kernel(const float* __restrict__ sums, int slices, int m_tiles, int n_tiles, __nv_bfloat16* __restrict__ out, int rows, int cols) {
+  const int lane = threadIdx.x & 31, unit = blockIdx.x * kWarps + (threadIdx.x >> 5), tiles = m_tiles * n_tiles;
+  const int c16 = unit % 16, part = unit / 16 % 4, half = unit / 64 % 2, tile = unit / 128;
+  grid_dependency_wait();
+  launch_dependents();
+  if (tile >= tiles) return;
+  const int row = tile / n_tiles * 256 + half * 128 + part * 32 + lane;
+  const long long col = static_cast<long long>(tile % n_tiles) * 256 + c16 * 16;
+  if (row >= rows || col >= cols) return;
+  const float4* at = reinterpret_cast<const float4*>(sums) + (static_cast<long long>(tile * 2 + half) * 64 + c16 * 4) * 128 + part * 32 + lane;
+  float4 v[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) v[q] = __ldcg(at + q * 128);
+#pragma unroll 2
+  for (int s = 1; s < slices; ++s) {
+    const float4* next = at + static_cast<long long>(s) * tiles * (2 * 64 * 128);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float4 x = __ldcg(next + q * 128);
+      v[q].x += x.x; v[q].y += x.y; v[q].z += x.z; v[q].w += x.w;
+    }
+  }
+  uint4* to = reinterpret_cast<uint4*>(out + static_cast<long long>(row) * cols + col);
+  to[0] = make_uint4(gemm::pack_bf16(v[0].x, v[0].y), gemm::pack_bf16(v[0].z, v[0].w), gemm::pack_bf16(v[1].x, v[1].y), gemm::pack_bf16(v[1].z, v[1].w));
+  if (col + 8 < cols) to[1] = make_uint4(gemm::pack_bf16(v[2].x, v[2].y), gemm::pack_bf16(v[2].z, v[2].w), gemm::pack_bf16(v[3].x, v[3].y), gemm::pack_bf16(v[3].z, v[3].w));
+}
+
 }  // namespace
+
+cudaError_t launch_fold_slices(const float* sums, int slices, int m_tiles, int n_tiles, __nv_bfloat16* out, int rows, int cols, cudaStream_t stream) {
+  if (slices < 1 || m_tiles < 1 || n_tiles < 1 || rows < 1 || rows > 256 * m_tiles || cols < 8 || cols % 8 || cols > 256 * n_tiles || static_cast<long long>(m_tiles) * n_tiles > 1 << 20) return cudaErrorInvalidValue;
+  const cudaError_t e = launch_early(fold_slices_kernel, dim3(m_tiles * n_tiles * 128 / kWarps), kThreads, 0, stream, sums, slices, m_tiles, n_tiles, out, rows, cols);
+  note_launch();
+  return e;
+}
 
 int linear_dz_blocks(int T, int N, int sms) {
   const int columns = (N + 255) / 256;
