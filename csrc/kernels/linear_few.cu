@@ -126,7 +126,8 @@ __global__ void __launch_bounds__(kThreads) linear_few_kernel(const __grid_const
     }
   }
   __syncwarp();
-  const bool ok = mbar_wait_bounded(&ctl->done, 0, abort_flag, p.status, 400, p.timeout_ns);
+  // a warp reads tensor memory as one, so it gives up as one
+  const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctl->done, 0, abort_flag, p.status, 400, p.timeout_ns));
   tc_fence_after_sync();
   __syncthreads();
   // All loads have landed and all products are done: the stages are free for the sums.
