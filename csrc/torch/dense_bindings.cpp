@@ -52,9 +52,11 @@ torch::Tensor as_rows(const torch::Tensor& t, int64_t cols) {
   torch::Tensor m = t.dim() == 2 ? t : t.reshape({-1, cols});
   return m.stride(1) == 1 || cols == 1 ? m : m.contiguous();
 }
-int rows_of(const torch::Tensor& m, const char* what) {
-  TORCH_CHECK(m.size(0) <= 0x7fffffff, what, ": more than 2^31 - 1 rows");
-  return static_cast<int>(m.size(0));
+// Rows of t, so few that a kernel counts past the last one in 32 bits. Asked for before anything is copied or allocated.
+int rows_of(const torch::Tensor& t, int64_t cols, const char* what) {
+  const int64_t rows = t.numel() / cols;
+  TORCH_CHECK(rows <= 1 << 30, what, ": more than 2^30 rows");
+  return static_cast<int>(rows);
 }
 int sm_count(const torch::Tensor& t) { return at::cuda::getDeviceProperties(t.get_device())->multiProcessorCount; }
 
@@ -68,11 +70,11 @@ Norm row_norm(const torch::Tensor& x, const torch::Tensor& weight, double eps, c
               "add_rms_norm: residual must have x's shape, type and device");
   TORCH_CHECK(!quantise || H % 128 == 0, "add_rms_norm: e4m3 rows have a scale per 128 columns, hidden must be a multiple of 128, got ", H);
   TORCH_CHECK(eps >= 0, "add_rms_norm: eps must not be negative");
+  RowNormArgs a{};
+  a.T = rows_of(x, H, "add_rms_norm"); a.H = static_cast<int>(H);
   c10::cuda::CUDAGuard guard(x.device());
   const torch::Tensor xm = as_rows(x, H);
-  RowNormArgs a{};
   a.x = xm.data_ptr(); a.x_stride = xm.stride(0);
-  a.T = rows_of(xm, "add_rms_norm"); a.H = static_cast<int>(H);
   a.weight = weight.data_ptr();
   a.rows_bf16 = x.scalar_type() == torch::kBFloat16; a.weight_bf16 = weight.scalar_type() == torch::kBFloat16;
   a.eps = static_cast<float>(eps);
@@ -111,7 +113,7 @@ std::tuple<torch::Tensor, torch::Tensor> row_norm_bwd(const torch::Tensor& h, co
   a.h = hm.data_ptr(); a.h_stride = hm.stride(0);
   a.weight = weight.data_ptr(); a.rstd = rstd.data_ptr<float>();
   a.dy = ym.data_ptr(); a.dh = dm.defined() ? dm.data_ptr() : nullptr;
-  a.T = rows_of(hm, "add_rms_norm"); a.H = static_cast<int>(H);
+  a.T = rows_of(h, H, "add_rms_norm"); a.H = static_cast<int>(H);
   a.rows_bf16 = h.scalar_type() == torch::kBFloat16; a.weight_bf16 = weight.scalar_type() == torch::kBFloat16;
   auto dx = fresh(h.sizes(), h);
   if (a.T == 0) return {dx, torch::zeros({H}, weight.options())};
@@ -190,14 +192,14 @@ Balance balance(const torch::Tensor& logits, const torch::Tensor& topk_idx, cons
               topk_idx.size(-1) >= 1 && topk_idx.size(-1) <= 0x7fffffff, "balance_loss: topk_idx must be int32 [..., k] on the device of logits, a row per token");
   TORCH_CHECK(!mask.has_value() || (mask->device() == logits.device() && mask->scalar_type() == torch::kBool && mask->sizes() == logits.sizes().slice(0, logits.dim() - 1)),
               "balance_loss: mask must be bool [...] on the device of logits, one value per token");
+  BalanceArgs a{};
+  a.T = rows_of(logits, E, "balance_loss"); a.E = static_cast<int>(E); a.K = static_cast<int>(topk_idx.size(-1)); a.sigmoid = sigmoid;
+  TORCH_CHECK(static_cast<int64_t>(a.T) * a.K <= 0x7fffffff, "balance_loss: more than 2^31 - 1 choices");
   c10::cuda::CUDAGuard guard(logits.device());
   const torch::Tensor lm = as_rows(logits, E), im = topk_idx.contiguous(), mm = mask_bytes(mask);
-  BalanceArgs a{};
   a.logits = lm.data_ptr(); a.stride = lm.stride(0); a.logits_bf16 = logits.scalar_type() == torch::kBFloat16;
   a.topk_idx = im.data_ptr<int>();
   a.mask = mm.defined() ? reinterpret_cast<const unsigned char*>(mm.data_ptr()) : nullptr;
-  a.T = rows_of(lm, "balance_loss"); a.E = static_cast<int>(E); a.K = static_cast<int>(topk_idx.size(-1)); a.sigmoid = sigmoid;
-  TORCH_CHECK(static_cast<int64_t>(a.T) * a.K <= 0x7fffffff, "balance_loss: more than 2^31 - 1 choices");
   Balance b{fresh(at::IntArrayRef{}, logits, torch::kFloat32), fresh({E}, logits, torch::kInt32), fresh({E + 1}, logits, torch::kInt32)};
   a.loss = b.loss.data_ptr<float>(); a.counts = b.counts.data_ptr<int>(); a.kept = b.kept.data_ptr<int>();
   const int blocks = balance_blocks(a, sm_count(logits));
@@ -234,7 +236,7 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
       BalanceBwdArgs a{};
       a.logits = lm.data_ptr(); a.stride = lm.stride(0); a.logits_bf16 = logits.scalar_type() == torch::kBFloat16;
       a.mask = saved[1].defined() ? reinterpret_cast<const unsigned char*>(saved[1].data_ptr()) : nullptr;
-      a.T = static_cast<int>(lm.size(0)); a.E = static_cast<int>(logits.size(-1)); a.K = static_cast<int>(kept[0]); a.sigmoid = static_cast<int>(kept[1]);
+      a.T = rows_of(logits, logits.size(-1), "balance_loss"); a.E = static_cast<int>(logits.size(-1)); a.K = static_cast<int>(kept[0]); a.sigmoid = static_cast<int>(kept[1]);
       a.kept = saved[2].data_ptr<int>(); a.dloss = dloss.data_ptr<float>(); a.dlogits = dlogits.data_ptr();
       cuda_check(launch_balance_bwd(a, sm_count(logits), cur_stream()), "balance_loss backward");
     }
@@ -392,10 +394,9 @@ LinearOut linear_forward(const torch::Tensor& x, const torch::Tensor& weight, co
   auto shape = x.sizes().vec();
   shape.back() = cols;
   TORCH_CHECK(!residual.has_value() || (residual->device() == x.device() && residual->scalar_type() == bf && residual->sizes() == at::IntArrayRef(shape)), "linear: residual must be bf16 with the output's shape, on x's device");
+  const int64_t T = rows_of(x, K, "linear");
   c10::cuda::CUDAGuard guard(x.device());
   LinearOut o{fresh(shape, x), {}};
-  const int64_t T = x.numel() / K;
-  TORCH_CHECK(T <= 1 << 30, "linear: more than 2^30 rows");
   const bool pre = keep && kind != LinearKind::kNone;
   if (pre) o.pre = fresh({T, N}, x);
   if (T == 0) return o;

@@ -71,7 +71,7 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, resid
 
     ``h = x + residual`` rounded to x's type; ``y = h / sqrt(mean(h^2) + eps) * weight`` over the last dimension, rounded once. x: bf16 or
     fp32 [..., hidden], rows in any strides (16-byte aligned rows of whole 16-byte words are fastest); ``residual``: the same shape and type;
-    ``weight``: bf16 or fp32 [hidden]; hidden up to 49152. ``quantise`` (hidden a multiple of 128): ``y`` also as the e4m3 rows that the
+    ``weight``: bf16 or fp32 [hidden]; hidden up to 49152, up to 2^30 rows. ``quantise`` (hidden a multiple of 128): ``y`` also as the e4m3 rows that the
     fp8 dispatch would send for it (``dequantise_rows`` reads them back). Gradients flow through y and h, not through q and scales; the weight's
     gradient is summed in a fixed order."""
     return NormRows(*runtime.ext().add_rms_norm(x, weight, eps, residual, quantise))
@@ -87,7 +87,7 @@ def balance_loss(logits: torch.Tensor, topk_idx: torch.Tensor, mask: Optional[to
 
     ``loss = E / (K N^2) * sum_e counts[e] * sum_t s[t, e]`` over the N live tokens: 1 when choices and scores are spread evenly, more when the
     experts that are chosen often are also those with high scores. ``s``: the softmax of a token's logits, or with ``scores="sigmoid"`` their sigmoids
-    divided by the sum of these. logits: bf16 or fp32 [..., experts] (up to 1024), without a bias that only the choice uses; ``topk_idx``: int32
+    divided by the sum of these. logits: bf16 or fp32 [..., experts] (up to 1024 experts, 2^30 tokens, 2^31 - 1 choices), without a bias that only the choice uses; ``topk_idx``: int32
     [..., k] as the routing returns it (entries outside the experts' range count for none); ``mask``: bool [...], False for padding, which has
     no part in anything. NaN logits count as -inf; a token whose scores are all zero adds no score; without live tokens the loss is 0. Gradients
     flow to the logits only. The result does not change from run to run."""
@@ -105,7 +105,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     x: bf16 [..., inputs]; ``weight``: bf16 [outputs, inputs], both sizes multiples of 8; ``bias``: bf16 [outputs]; ``residual``: bf16 with the
     result's shape. ``activation``: None, "relu", "silu", "gelu" (z Phi(z)), or "swiglu": the weight holds tiles of 128 gate rows and the 128 up rows of
     the same features, as an expert's does (``models.moe.interleave_gate_up``), outputs a multiple of 256, the result [..., outputs / 2] =
-    silu(gate) * up, without bias and residual. Any number of rows from none on; rows that are not contiguous, 16-byte aligned and a multiple of 16 bytes
+    silu(gate) * up, without bias and residual. From none to 2^30 rows; rows that are not contiguous, 16-byte aligned and a multiple of 16 bytes
     apart are copied first. Where a gradient needs it, what the activation was taken of is kept in bf16. A device wait that gave up is
     reported by ``ops.gemm.check()``."""
     if activation not in _ACTIVATIONS:

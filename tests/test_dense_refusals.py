@@ -98,6 +98,26 @@ def test_row_norm_refusals():
             bad()
 
 
+@pytest.mark.gpu
+def test_more_rows_than_are_counted_are_refused_before_anything_is_allocated():
+    def rows(n, cols, dtype=BF):   # one row's memory
+        return torch.zeros(1, cols, device="cuda", dtype=dtype).expand(n, cols)
+
+    n = 2**30 + 1
+    before = torch.cuda.memory_stats()["allocation.all.allocated"]
+    held = [rows(n, 8), torch.ones(8, device="cuda", dtype=BF), rows(n, 2), rows(n, 1, torch.int32), torch.zeros(8, 8, device="cuda", dtype=BF), rows(2**29, 2), rows(2**29, 4, torch.int32)]
+    made = torch.cuda.memory_stats()["allocation.all.allocated"] - before
+    for bad, match in [
+        (lambda: fused.add_rms_norm(held[0], held[1]), "rows"),
+        (lambda: fused.balance_loss(held[2], held[3]), "rows"),
+        (lambda: fused.balance_loss(held[5], held[6]), "choices"),
+        (lambda: fused.linear(held[0], held[4]), "rows"),
+    ]:
+        with pytest.raises(RuntimeError, match=match):
+            bad()
+    assert torch.cuda.memory_stats()["allocation.all.allocated"] - before == made
+
+
 def test_memory_plan_counts_a_shared_expert():
     from fast_b200.models import DEEPSEEK_V3_MOE_LAYER, MIXTRAL_8X7B_BLOCK, flops_per_step, memory_plan, step_roofline
 
