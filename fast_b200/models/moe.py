@@ -215,6 +215,10 @@ class MoELayer(nn.Module):
             return out
         return fused.linear(fused.linear(x, self.shared_w13, activation="swiglu"), self.shared_w2, residual=out)
 
+    def _drop_balance(self) -> None:
+        """Before a pass keeps anything: the last one's balance loss holds its graph, and with it the rows it kept where no backward pass has freed them."""
+        self.balance_loss = self.expert_counts = None
+
     def _note_balance(self, logits: torch.Tensor, mask: Optional[torch.Tensor]) -> None:
         if self.balance is not None:
             self.balance_loss, self.expert_counts = fused.balance_loss(logits, self.last_route.topk_idx, mask=mask, scores=self.balance)
@@ -236,6 +240,7 @@ class MoELayer(nn.Module):
                 return self(rows.y, mask), rows.h
             with torch.no_grad():
                 return self._infer(rows.y, None if rows.q is None else (rows.q, rows.scales)), rows.h
+        self._drop_balance()
         total = h.contiguous() if add is None else h + add
         out = _NormRouteMoEFunction.apply(total, norm_w, self.gate, self.w13, self.w2, self.engine, eps, self)
         if self.balance is not None or self.shared_inter:
@@ -251,6 +256,7 @@ class MoELayer(nn.Module):
         """mean((h + MoE(RMSNorm(h; norm_w)))^2), the sum rounded to bf16, as a scalar fp32 tensor. ``mask``: see ``forward``; it has no part in the mean."""
         if not (self._fuses(h) and h.shape[0] > 0) or self.shared_inter:
             return fused.residual_mean_square(h, self.forward_from_residual(h, norm_w, eps, mask=mask))
+        self._drop_balance()
         loss = _NormRouteMoELossFunction.apply(h.contiguous(), norm_w, self.gate, self.w13, self.w2, self.engine, eps, self)
         if self.balance is not None:
             loss, logits = loss
@@ -269,6 +275,7 @@ class MoELayer(nn.Module):
         if not (torch.is_grad_enabled() and self.training):
             with torch.no_grad():
                 return self._infer(x)
+        self._drop_balance()
         logits = (x @ self.gate.t()).float()
         rs = self.engine.route(logits.detach(), self.router_bias)
         self.last_route = rs

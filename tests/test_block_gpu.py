@@ -167,3 +167,23 @@ def test_layer_options_that_are_refused():
     for kw in ({"balance": "l2"}, {"shared_inter": 100}, {"shared_inter": -128}):
         with pytest.raises(ValueError):
             MoELayer(None, 512, 256, 8, 2, 64, **kw)
+
+
+@pytest.mark.parametrize("E,K,shared", [(8, 2, 0), (8, 2, 128), (64, 4, 0)])
+def test_a_pass_that_nothing_was_made_of_is_let_go_before_the_next(E, K, shared):
+    """What a pass keeps for its backward pass hangs on the layer's balance loss: no second one may live beside it."""
+    H, T, eps = 512, 256, 1e-5
+    comm, layer = _layer(E, K, H, 256, balance="softmax", shared_inter=shared)
+    h, nw = _randn(1, T, H).requires_grad_(), torch.ones(H, device="cuda", dtype=BF)
+    seen = []
+    for name in ("route", "route_fused"):
+        def wrapped(*a, _run=getattr(layer.engine, name), **kw):
+            seen.append((layer.balance_loss, layer.expert_counts))
+            return _run(*a, **kw)
+        setattr(layer.engine, name, wrapped)
+    for run in (lambda: layer.forward_from_residual(h, nw, eps), lambda: layer.mean_square_from_residual(h, nw, eps), lambda: layer(h)):
+        for _ in range(2):
+            run()
+            assert layer.balance_loss.requires_grad and int(layer.expert_counts.sum()) == T * K
+    comm.check()
+    assert seen == [(None, None)] * 6
