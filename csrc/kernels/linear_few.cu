@@ -5,8 +5,8 @@
 // rows through shared memory (TMA) as operand A of M = 128 MMAs, the tokens are N (rounded up to 16), so a decode step does no more work
 // than its tokens are. The CTAs' fp32 sums meet in distributed shared memory: each CTA adds up an equal share of the tile's features, in the order
 // of the reduction, and finishes them (bias, activation, residual, store): no counters, no scratch in global memory, nothing to
-// clear beforehand, one launch. 1 token, weight from HBM: 4096 -> 14336 21 us (5.6 TB/s), 14336 -> 4096 21 us, 4096 -> 4096 7.5 us (4.5 TB/s; 3 us of a launch are setting up, the
-// first loads and the sums' way). Stages leave room for two CTAs an SM, so that the next launch is set up while this one runs.
+// clear beforehand, one launch. 1 token, weight from HBM: 4096 -> 14336 21 us (5.6 TB/s), 14336 -> 4096 21 us, 4096 -> 4096 9.0 us (3.7 TB/s; 3 us of a launch are setting up, the
+// first loads and the sums' way). A launch of no more CTAs than SMs has all their shared memory for stages; a larger one, half: two CTAs an SM.
 // SwiGLU: the 128 rows are 64 gate rows and the 64 up rows of the same features.
 #include <algorithm>
 
@@ -22,9 +22,9 @@ using namespace gemm;
 
 constexpr int kRows = 128;                       // of the weight, a tile
 constexpr int kThreads = 256;                    // two warps for every quarter of tensor memory
-constexpr int kMaxStages = 6;
+constexpr int kMaxStages = 12;
 constexpr int kFewABytes = kRows * BK * 2;       // 16 KiB
-constexpr int kFewSmem = 110 * 1024;             // two CTAs an SM
+constexpr int kFewSmem = 110 * 1024, kFewDeepSmem = 220 * 1024;   // of an SM's two CTAs each, or of its only one
 __host__ __device__ constexpr int few_stage(int n) { return kFewABytes + n * BK * 2; }
 
 struct __align__(8) FewCtl {
@@ -32,12 +32,13 @@ struct __align__(8) FewCtl {
   uint32_t tmem_base;
   int abort_flag;
 };
-constexpr int few_stages(int n) { return std::min(kMaxStages, (kFewSmem - 1024 - static_cast<int>(sizeof(FewCtl))) / few_stage(n)); }
+constexpr int few_stages(int n, int smem) { return std::min(kMaxStages, (smem - 1024 - static_cast<int>(sizeof(FewCtl))) / few_stage(n)); }
 // The CTA's sums [n][few_pitch] lie where the stages were. A warp reads several tokens' shares at once: the pitch puts them on different banks.
 __host__ __device__ constexpr int few_pitch(int mine) { return kRows + mine % 32; }
 __host__ __device__ constexpr int few_sums(int n) { return n * (kRows + 16) * 4; }
-constexpr int few_smem(int n) { return std::max(few_stages(n) * few_stage(n), few_sums(n)) + 1024 + static_cast<int>(sizeof(FewCtl)); }
-static_assert(few_stages(16) == 6 && few_stages(kFewTokens) >= 3 && few_smem(kFewTokens) <= kFewSmem, "stages at both ends of the range");
+constexpr int few_smem(int n, int stages) { return std::max(stages * few_stage(n), few_sums(n)) + 1024 + static_cast<int>(sizeof(FewCtl)); }
+static_assert(few_stages(16, kFewSmem) >= 5 && few_stages(kFewTokens, kFewSmem) >= 3 && few_smem(kFewTokens, few_stages(kFewTokens, kFewSmem)) <= kFewSmem &&
+              few_smem(kFewTokens, few_stages(kFewTokens, kFewDeepSmem)) <= kFewDeepSmem && few_smem(16, kMaxStages) <= kFewDeepSmem, "stages at both ends of the range");
 
 __device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
   float4 v;
@@ -206,17 +207,16 @@ __global__ void __launch_bounds__(kThreads) linear_few_kernel(const __grid_const
 
 }  // namespace
 
-// How many CTAs share a tile's reduction: as many as leave every CTA an SM, more where their parts are long (a CTA's stream alone does not fill an
-// SM's way to memory), eight only where there are few tiles, the parts are very long or up to 16 tokens make the sums small: a cluster of eight is harder
-// to place, and its sums travel further. us at 1, 2, 4, 8 parts: 32 tiles of 64 blocks (4096 -> 4096, 1 token) 14.6, 9.9, 8.2, 7.4, 64 tokens 20.5, 13.5, 10.7, 12.1; 56 tiles of 32
-// (2048 -> 7168), 1 token 8.4, 6.6, 6.9, 10.1; 112 tiles of 64 (4096 -> 14336), 33 tokens 26.2, 21.9, 27.9, 35.9; 224 tiles of 16 (1024 -> 28672),
-// 1 token 11.9, 14.8, 21.4, 32.7; 32 tiles of 224 (14336 -> 4096), 33 tokens 66.5, 37.6, 25.6, 23.2.
+// How many CTAs share a tile's reduction: as many as leave every CTA an SM of its own, whose shared memory it then has for stages (what a CTA has under way
+// at a time bounds its stream), and eight blocks of the reduction; eight, two an SM, only where up to 16 tokens make the sums small, for a larger cluster is harder
+// to place and its sums travel further. us with 1, 2, 4, 8 CTAs of half an SM's shared memory / of all of it: 32 tiles of 64 blocks (4096 -> 4096), 1 token
+// 15.1, 10.7, 9.4, 9.3 / 12.8, 9.6, 9.6, 17.2, 64 tokens 21.2, 14.1, 11.8, 13.0 / 13.7, 10.5, 10.8, 22.5, 128 tokens 26.4, 17.0, 13.1, 16.1 / 17.6, 13.2, 11.9, 27.2;
+// 32 tiles of 16, 128 tokens 9.5, 8.2, 7.9, 15.7 / 7.5, 7.4, 7.7, 15.6; 56 of 32 (2048 -> 7168), 48 tokens 12.5, 10.4, 10.3 / 9.0, 9.2, 14.5; 112 of 64 (4096 -> 14336), 64
+// tokens 28.0, 24.1, 31.2 / 23.5, 28.0, 38.6; 32 of 224 (14336 -> 4096), 1 token 45.8, 28.0, 23.0, 22.0 / 38.0, 23.6, 22.7, 31.4.
 int few_parts(int tiles, int red_blocks, int n, int sms) {
   int parts = 1;
-  while (parts < 8 && (n > 32 ? 4 : 2) * parts <= red_blocks &&
-         ((parts == 4 ? (n <= 16 ? 1 : 4) : 2) * tiles * parts <= sms || (tiles * parts < sms && red_blocks >= 48 * parts)))
-    parts *= 2;
-  return parts;
+  while (parts < 4 && 2 * tiles * parts <= sms && 8 * 2 * parts <= red_blocks) parts *= 2;
+  return n <= 16 && parts == 4 && 4 * tiles <= sms && red_blocks >= 64 ? 8 : parts;
 }
 int few_box_rows(int T) {
   const int tiles = (T + kFewTokens - 1) / kFewTokens;
@@ -238,11 +238,11 @@ cudaError_t launch_linear_few(GemmMode mode, Activation act, bool swiglu, const 
   if (a.T < 1 || a.columns < 1 || a.red_blocks < 1 || a.status == nullptr || (mode != GemmMode::kForward && (mode != GemmMode::kDgrad || swiglu || act != Activation::kNone)) || (swiglu && (act != Activation::kNone || a.columns % 128))) return cudaErrorInvalidValue;
   const int per_tile = swiglu ? kRows / 2 : kRows, tiles = (a.columns + per_tile - 1) / per_tile;
   a.n = few_box_rows(a.T);
-  a.stages = few_stages(a.n);
   const int token_tiles = (a.T + a.n - 1) / a.n;
   if (token_tiles > 65535) return cudaErrorInvalidValue;
   a.parts = few_parts(tiles * token_tiles, a.red_blocks, a.n, sms);
-  const int smem = few_smem(a.n);
+  a.stages = std::min(few_stages(a.n, tiles * token_tiles * a.parts <= sms ? kFewDeepSmem : kFewSmem), (a.red_blocks + a.parts - 1) / a.parts);
+  const int smem = few_smem(a.n, a.stages);
   const auto go = [&](auto kern) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
