@@ -196,12 +196,16 @@ struct FewArgs {
   long long residual_stride;
   __nv_bfloat16* out;          // [T, columns]
   __nv_bfloat16* pre;          // what the activation is taken of: [T, columns], SwiGLU [T, 2 columns]; or null
-  int n, stages, parts;        // set by the launcher: tokens of a tile, operand stages, CTAs that share a tile's reduction
+  int n, stages;               // set by the launcher: tokens of a tile, operand stages
   DeviceStatus* status;
   unsigned long long timeout_ns;
 };
-bool few_pays(int T, int columns, int red_blocks, bool swiglu, int sms);
-int few_box_rows(int T);       // rows of map_x's boxes {64, rows}; map_w's are {64,128}, SwiGLU and dgrad {64,64}
+bool few_pays(int T, int columns, int red_blocks, bool swiglu, bool sectors, int sms);   // sectors: the operands' rows start at multiples of 32 bytes
+struct FewPlan {
+  int tiles, token_tiles, n;     // tiles of the weight's rows, of the tokens, and tokens of one: map_x's boxes are {64, n}, map_w's {64, 128}, SwiGLU's and dgrad's {64, 64}
+  int parts, stages;             // CTAs that share a tile's reduction, operand stages of one
+};
+FewPlan few_plan(int T, int columns, int red_blocks, bool swiglu, int sms);
 cudaError_t launch_linear_few(GemmMode mode, Activation act, bool swiglu, const CUtensorMap& map_w, const CUtensorMap& map_x, const FewArgs& args, int sms, cudaStream_t stream);
 // Where dense launches on the current device report a wait that gave up.
 DeviceStatus* dense_status();

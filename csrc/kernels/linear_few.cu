@@ -3,10 +3,11 @@
 //
 // What bounds it: the weight's bytes. A cluster of CTAs has a tile and shares out the reduction; a CTA streams its part of the weight's
 // rows through shared memory (TMA) as operand A of M = 128 MMAs, the tokens are N (rounded up to 16), so a decode step does no more work
-// than its tokens are. The CTAs' fp32 sums meet in distributed shared memory: each CTA adds up an equal share of the tile's features, in the order
-// of the reduction, and finishes them (bias, activation, residual, store): no counters, no scratch in global memory, nothing to
-// clear beforehand, one launch. 1 token, weight from HBM: 4096 -> 14336 21 us (5.6 TB/s), 14336 -> 4096 21 us, 4096 -> 4096 9.0 us (3.7 TB/s; 3 us of a launch are setting up, the
-// first loads and the sums' way). A launch of no more CTAs than SMs has all their shared memory for stages; a larger one, half: two CTAs an SM.
+// than its tokens are. Each CTA finishes an equal share of the tile's features: the others send it their fp32 sums through distributed shared memory, it
+// adds them up in the order of the reduction (bias, activation, residual, store): no counters, no scratch in global memory, nothing to
+// clear beforehand, one launch. 1 token, weight from HBM: 4096 -> 14336 21 us (5.6 TB/s), 14336 -> 4096 21.6 us, 4096 -> 4096 9.0 us (3.7 TB/s; 3 us of a launch are setting up,
+// the first loads and the sums' way). A launch of no more CTAs than SMs has all their shared memory for stages; a larger one, half: two CTAs an SM. With
+// hundreds of tokens the bound is a CTA's way from L2: 32 KiB in 0.23 us, whether or not two CTAs share the tokens in one MMA of M = 256 (512 x 4096 -> 4096 17.8 and 17.7 us).
 // SwiGLU: the 128 rows are 64 gate rows and the 64 up rows of the same features.
 #include <algorithm>
 
@@ -32,19 +33,27 @@ struct __align__(8) FewCtl {
   uint32_t tmem_base;
   int abort_flag;
 };
-constexpr int few_stages(int n, int smem) { return std::min(kMaxStages, (smem - 1024 - static_cast<int>(sizeof(FewCtl))) / few_stage(n)); }
-// The CTA's sums [n][few_pitch] lie where the stages were. A warp reads several tokens' shares at once: the pitch puts them on different banks.
-__host__ __device__ constexpr int few_pitch(int mine) { return kRows + mine % 32; }
-__host__ __device__ constexpr int few_sums(int n) { return n * (kRows + 16) * 4; }
-constexpr int few_smem(int n, int stages) { return std::max(stages * few_stage(n), few_sums(n)) + 1024 + static_cast<int>(sizeof(FewCtl)); }
-static_assert(few_stages(16, kFewSmem) >= 5 && few_stages(kFewTokens, kFewSmem) >= 3 && few_smem(kFewTokens, few_stages(kFewTokens, kFewSmem)) <= kFewSmem &&
-              few_smem(kFewTokens, few_stages(kFewTokens, kFewDeepSmem)) <= kFewDeepSmem && few_smem(16, kMaxStages) <= kFewDeepSmem, "stages at both ends of the range");
+// The fp32 sums: where the stages were, or, where they are few and of several CTAs, beside them: a peer's may come while this CTA still multiplies.
+__host__ __device__ constexpr int few_sums(int n) { return n * kRows * 4; }
+__host__ __device__ constexpr bool few_beside(int n, int parts) { return parts > 1 && n <= 64; }
+__host__ __device__ constexpr int few_room(int n, int parts, int stages) {
+  const int operands = stages * few_stage(n);
+  return few_beside(n, parts) ? operands + few_sums(n) : operands > few_sums(n) ? operands : few_sums(n);
+}
+constexpr int kFewOther = 1024 + static_cast<int>(sizeof(FewCtl));
+constexpr int few_stages(int n, int parts, int smem) { return std::min(kMaxStages, (smem - kFewOther - (few_beside(n, parts) ? few_sums(n) : 0)) / few_stage(n)); }
+constexpr int few_smem(int n, int parts, int stages) { return few_room(n, parts, stages) + kFewOther; }
+constexpr int few_most(int n, int parts, int smem) { return few_smem(n, parts, few_stages(n, parts, smem)); }
+static_assert(few_stages(16, 8, kFewSmem) >= 5 && few_stages(kFewTokens, 1, kFewSmem) >= 3 && few_most(kFewTokens, 1, kFewSmem) <= kFewSmem && few_most(16, 8, kFewSmem) <= kFewSmem &&
+              few_most(64, 4, kFewDeepSmem) <= kFewDeepSmem && few_most(kFewTokens, 4, kFewDeepSmem) <= kFewDeepSmem, "stages at both ends of the range");
 
-__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
+__device__ __forceinline__ float4 ld_sums(uint32_t addr) {
   float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+__device__ __forceinline__ void st_own(uint32_t addr, uint32_t v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ uint2 pack4(const float4& v) { return make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w)); }
 __device__ __forceinline__ float4 unpack4(const __nv_bfloat16* at) {
   const uint2 v = *reinterpret_cast<const uint2*>(at);
@@ -62,11 +71,11 @@ __global__ void __launch_bounds__(kThreads) linear_few_kernel(const __grid_const
   extern __shared__ uint8_t smem_raw[];
   uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int n = p.n, stage_size = few_stage(n), stages = p.stages;
-  float* sums = reinterpret_cast<float*>(tiles);                       // once the products are done
-  FewCtl* ctl = reinterpret_cast<FewCtl*>(tiles + max(stages * stage_size, few_sums(n)));
+  const uint32_t sums = smem_u32(tiles) + (few_beside(n, PARTS) ? stages * stage_size : 0);
+  FewCtl* ctl = reinterpret_cast<FewCtl*>(tiles + few_room(n, PARTS, stages));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = static_cast<int>(cluster_cta_rank());
   const int tile = blockIdx.x / PARTS, t0 = blockIdx.y * n, T = min(n, p.T - t0);   // rows of the weight, tokens
-  constexpr int F = SWIGLU ? kRows / 2 : kRows, MINE = F / PARTS, PITCH = few_pitch(MINE);   // features of a tile, and those that I finish
+  constexpr int F = SWIGLU ? kRows / 2 : kRows, MINE = F / PARTS;   // features of a tile, and those that I finish
   const uint32_t columns = n <= 32 ? 32 : n <= 64 ? 64 : 128;
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) { mbar_init(&ctl->full[s], 1); mbar_init(&ctl->empty[s], 1); }
@@ -79,6 +88,7 @@ __global__ void __launch_bounds__(kThreads) linear_few_kernel(const __grid_const
   if (warp == 1) { tmem_alloc(&ctl->tmem_base, columns); tmem_relinquish(); }
   tc_fence_before_sync();
   __syncthreads();
+  if (few_beside(n, PARTS)) cluster_arrive();
   tc_fence_after_sync();
   const uint32_t tmem = ctl->tmem_base;
   volatile int* abort_flag = &ctl->abort_flag;
@@ -130,78 +140,82 @@ __global__ void __launch_bounds__(kThreads) linear_few_kernel(const __grid_const
   // a warp reads tensor memory as one, so it gives up as one
   const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctl->done, 0, abort_flag, p.status, 400, p.timeout_ns));
   tc_fence_after_sync();
-  __syncthreads();
-  // All loads have landed and all products are done: the stages are free for the sums.
-  if (ok) {
-    const int feature = (warp & 3) * 32 + lane;
-    for (int c = (warp >> 2) * 32; c < n; c += 64) {
-      uint32_t r[32];
-      tmem_ld_32x32(tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + c, r);
-      tmem_wait_ld();
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (c + i < T) sums[(c + i) * PITCH + feature] = __uint_as_float(r[i]);
+  // Four features of a token (SwiGLU: their gates and ups) on their way out.
+  const auto finish = [&](int token, int f, float4 v, const float4& up) {
+    const int t = t0 + token, col = tile * F + f;
+    if (col >= p.columns) return;
+    if (p.bias != nullptr) {
+      const float4 b = unpack4(p.bias + col);
+      v.x += b.x; v.y += b.y; v.z += b.z; v.w += b.w;
     }
+    const long long at = static_cast<long long>(t) * p.columns + col;
+    if (SWIGLU) {
+      if (p.pre != nullptr) {
+        __nv_bfloat16* gu = p.pre + static_cast<long long>(t) * p.columns * 2 + tile / 2 * 256 + tile % 2 * 64 + f;
+        *reinterpret_cast<uint2*>(gu) = pack4(v);
+        *reinterpret_cast<uint2*>(gu + 128) = pack4(up);
+      }
+      v.x = silu(v.x) * up.x; v.y = silu(v.y) * up.y; v.z = silu(v.z) * up.z; v.w = silu(v.w) * up.w;
+    } else {
+      if (p.pre != nullptr) *reinterpret_cast<uint2*>(p.pre + at) = pack4(v);
+      v.x = activated<ACT>(v.x); v.y = activated<ACT>(v.y); v.z = activated<ACT>(v.z); v.w = activated<ACT>(v.w);
+    }
+    if (p.residual != nullptr) {
+      const float4 r = unpack4(p.residual + t * p.residual_stride + col);
+      v.x += r.x; v.y += r.y; v.z += r.z; v.w += r.w;
+    }
+    *reinterpret_cast<uint2*>(p.out + at) = pack4(v);
+  };
+  const int quarter = warp & 3;                                         // of tensor memory, and of the features
+  const auto load = [&](int c, uint32_t (&r)[32]) {
+    tmem_ld_32x32(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + c, r);
+    tmem_wait_ld();
+  };
+  // Every CTA sends its sums to the CTA of the cluster that finishes them, [part][token][feature], and reads what has come to it: the way to a peer's
+  // shared memory is not waited for value by value, and after one barrier nobody touches another's.
+  constexpr int WIDTH = kRows / PARTS;                                // floats of a token
+  const int fl = quarter * 32 + lane, owner = fl % F / MINE;
+  const uint32_t own = sums + (rank * n * WIDTH + fl / F * MINE + fl % MINE) * 4, to = PARTS > 1 ? map_to_cta(own, owner) : own;
+  if (PARTS > 1 && !few_beside(n, PARTS)) cluster_sync_all();          // the peers' products are done too
+  else if (PARTS > 1) cluster_wait();                                   // the peers are there
+  for (int c = (warp >> 2) * 32; ok && c < T; c += 64) {
+    uint32_t r[32];
+    load(c, r);
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (c + i < T) {
+        if (PARTS > 1) st_cluster(to + (c + i) * WIDTH * 4, r[i]);
+        else st_own(to + (c + i) * WIDTH * 4, r[i]);
+      }
   }
   tc_fence_before_sync();
   __syncthreads();
   if (PARTS > 1) cluster_sync_all();
-  if (ok) {
-    // Four features of a token at a time, U of them in flight: what this takes is the way to the peers' shared memory. Pairs of features one after
-    // the other, by half the threads, took 13 us instead of 8.4 for 48 x 2048 -> 7168.
-    constexpr int Q = MINE / 4, U = PARTS >= 8 ? 2 : 4;
-    const uint32_t base = smem_u32(sums);
-    for (int i0 = threadIdx.x; i0 < T * Q; i0 += U * kThreads) {
-      float4 z[U], u[SWIGLU ? U : 1];
-      const auto gather = [&](int add, float4* to) {
-        float4 w[U][PARTS];
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-          const int i = min(i0 + j * kThreads, T * Q - 1);
-          const uint32_t at = base + static_cast<uint32_t>(i / Q * PITCH + rank * MINE + i % Q * 4 + add) * 4u;
-#pragma unroll
-          for (int q = 0; q < PARTS; ++q) w[j][q] = ld_cluster(PARTS > 1 ? map_to_cta(at, q) : at);
-        }
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-          to[j] = w[j][0];
-#pragma unroll
-          for (int q = 1; q < PARTS; ++q) { to[j].x += w[j][q].x; to[j].y += w[j][q].y; to[j].z += w[j][q].z; to[j].w += w[j][q].w; }
-        }
-      };
-      gather(0, z);
-      if (SWIGLU) gather(F, u);
+  constexpr int Q = MINE / 4, U = SWIGLU || PARTS >= 8 ? 2 : 4;       // U in flight
+  for (int i0 = threadIdx.x; ok && i0 < T * Q; i0 += U * kThreads) {
+    float4 z[U], u[SWIGLU ? U : 1];
+    const auto gather = [&](int add, float4* sum) {                   // in the order of the reduction
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const int i = i0 + j * kThreads, t = t0 + i / Q, f = rank * MINE + i % Q * 4, col = tile * F + f;
-        if (i >= T * Q || col >= p.columns) continue;
-        float4 v = z[j];
-        if (p.bias != nullptr) {
-          const float4 b = unpack4(p.bias + col);
-          v.x += b.x; v.y += b.y; v.z += b.z; v.w += b.w;
+        const int i = min(i0 + j * kThreads, T * Q - 1);
+        const uint32_t at = sums + static_cast<uint32_t>(i / Q * WIDTH + i % Q * 4 + add) * 4u;
+        sum[j] = ld_sums(at);
+#pragma unroll
+        for (int q = 1; q < PARTS; ++q) {
+          const float4 w = ld_sums(at + static_cast<uint32_t>(q * n * WIDTH) * 4u);
+          sum[j].x += w.x; sum[j].y += w.y; sum[j].z += w.z; sum[j].w += w.w;
         }
-        const long long at = static_cast<long long>(t) * p.columns + col;
-        if (SWIGLU) {
-          if (p.pre != nullptr) {
-            __nv_bfloat16* gu = p.pre + static_cast<long long>(t) * p.columns * 2 + tile / 2 * 256 + tile % 2 * 64 + f;
-            *reinterpret_cast<uint2*>(gu) = pack4(v);
-            *reinterpret_cast<uint2*>(gu + 128) = pack4(u[j]);
-          }
-          v.x = silu(v.x) * u[j].x; v.y = silu(v.y) * u[j].y; v.z = silu(v.z) * u[j].z; v.w = silu(v.w) * u[j].w;
-        } else {
-          if (p.pre != nullptr) *reinterpret_cast<uint2*>(p.pre + at) = pack4(v);
-          v.x = activated<ACT>(v.x); v.y = activated<ACT>(v.y); v.z = activated<ACT>(v.z); v.w = activated<ACT>(v.w);
-        }
-        if (p.residual != nullptr) {
-          const float4 r = unpack4(p.residual + t * p.residual_stride + col);
-          v.x += r.x; v.y += r.y; v.z += r.z; v.w += r.w;
-        }
-        *reinterpret_cast<uint2*>(p.out + at) = pack4(v);
       }
+    };
+    gather(0, z);
+    if (SWIGLU) gather(MINE, u);
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int i = i0 + j * kThreads;
+      if (i < T * Q) finish(i / Q, rank * MINE + i % Q * 4, z[j], u[SWIGLU ? j : 0]);
     }
   }
-  __syncthreads();
-  if (PARTS > 1) cluster_sync_all();   // a peer may still read my sums
+  __syncwarp();
   if (warp == 1) tmem_dealloc(tmem, columns);
 }
 
@@ -218,42 +232,50 @@ int few_parts(int tiles, int red_blocks, int n, int sms) {
   while (parts < 4 && 2 * tiles * parts <= sms && 8 * 2 * parts <= red_blocks) parts *= 2;
   return n <= 16 && parts == 4 && 4 * tiles <= sms && red_blocks >= 64 ? 8 : parts;
 }
-int few_box_rows(int T) {
-  const int tiles = (T + kFewTokens - 1) / kFewTokens;
-  return ((T + tiles - 1) / tiles + 15) / 16 * 16;
+FewPlan few_plan(int T, int columns, int red_blocks, bool swiglu, int sms) {
+  FewPlan f{};
+  const int per_tile = swiglu ? kRows / 2 : kRows;
+  f.tiles = (columns + per_tile - 1) / per_tile;
+  f.token_tiles = (T + kFewTokens - 1) / kFewTokens;
+  f.n = ((T + f.token_tiles - 1) / f.token_tiles + 15) / 16 * 16;
+  f.token_tiles = (T + f.n - 1) / f.n;
+  f.parts = few_parts(f.tiles * f.token_tiles, red_blocks, f.n, sms);
+  f.stages = std::min(few_stages(f.n, f.parts, f.tiles * f.token_tiles * f.parts <= sms ? kFewDeepSmem : kFewSmem), (red_blocks + f.parts - 1) / f.parts);
+  return f;
 }
 
-// Against the kernel with tiles of 256 features by up to 256 tokens (grouped_gemm_tokens.cu): ahead while its 128 x 128 tiles are no more than the SMs,
-// unless they are many and long. us, that kernel -> this one: 4096 -> 4096 with 1, 64, 128, 512 tokens 17.3 -> 8.2, 21.0 -> 10.7, 19.9 -> 12.7, 27.7 -> 20.4, with
-// 1024 (256 tiles) 28.9 -> 31.8; 4096 -> 14336 with 128 (112 tiles) 28.1 -> 26.3, 192 (224 tiles) 29.1 -> 31.7; 1024 -> 1024 with 1024 13.3 -> 7.4; 2048 -> 7168
-// with 256 19.2 -> 15.3, with 384 (168 tiles) 17.0 -> 18.2; 14336 -> 4096 with 256 (64 tiles) 55.9 -> 36.3, with 384 (96 tiles) 48.8 -> 54.7.
-bool few_pays(int T, int columns, int red_blocks, bool swiglu, int sms) {
+// Against the kernel with tiles of 256 features by up to 256 tokens (grouped_gemm_tokens.cu), which reads half as much per product but takes 4 us more to
+// begin and end. Ahead with up to 64 tokens, and otherwise the longer the fewer rounds of the GPU its tiles take. us, that kernel -> this one: 1 token 4096 -> 57344
+// 83.0 -> 72.4, 64 tokens 86.3 -> 79.7, 128 tokens 4096 -> 32000 49.9 -> 50.0; half a round (64 tiles), 256 x 14336 -> 4096 49.6 -> 34.1; a round (96 to 128 tiles): 64 blocks of the
+// reduction, 96 x 4096 -> 14336 25.4 -> 23.3, 112 blocks, 500 x 7168 -> 4096 SwiGLU 29.8 -> 29.8, 224 blocks, 384 x 14336 -> 4096 47.2 -> 51.5; two rounds: 16 blocks, 1024 x 1024 -> 4096 12.4 ->
+// 11.0, 32 blocks, 384 x 2048 -> 7168 14.6 -> 17.0; four rounds: 4 blocks, 2048 x 256 -> 4096 11.6 -> 11.2, 8 blocks 13.0 -> 14.4. Rows that do not start at sectors of 32 bytes
+// come in more slowly, which weighs on what reads more: 1235 x 1000 -> 2760 (two rounds, 16 blocks) 12.9 -> 16.7.
+bool few_pays(int T, int columns, int red_blocks, bool swiglu, bool sectors, int sms) {
   const int per_tile = swiglu ? kRows / 2 : kRows;
   const long long tiles = static_cast<long long>((columns + per_tile - 1) / per_tile) * ((T + kFewTokens - 1) / kFewTokens);
-  return 2 * tiles <= sms || (tiles <= sms && red_blocks <= 96);
+  if (T <= 64 || 2 * tiles <= sms) return true;
+  return red_blocks <= (tiles <= sms ? 112 : !sectors ? 0 : tiles <= 2 * sms ? 16 : tiles <= 4 * sms ? 4 : 0);
 }
 
 cudaError_t launch_linear_few(GemmMode mode, Activation act, bool swiglu, const CUtensorMap& map_w, const CUtensorMap& map_x, const FewArgs& args, int sms, cudaStream_t stream) {
   FewArgs a = args;
   if (a.T < 1 || a.columns < 1 || a.red_blocks < 1 || a.status == nullptr || (mode != GemmMode::kForward && (mode != GemmMode::kDgrad || swiglu || act != Activation::kNone)) || (swiglu && (act != Activation::kNone || a.columns % 128))) return cudaErrorInvalidValue;
-  const int per_tile = swiglu ? kRows / 2 : kRows, tiles = (a.columns + per_tile - 1) / per_tile;
-  a.n = few_box_rows(a.T);
-  const int token_tiles = (a.T + a.n - 1) / a.n;
-  if (token_tiles > 65535) return cudaErrorInvalidValue;
-  a.parts = few_parts(tiles * token_tiles, a.red_blocks, a.n, sms);
-  a.stages = std::min(few_stages(a.n, tiles * token_tiles * a.parts <= sms ? kFewDeepSmem : kFewSmem), (a.red_blocks + a.parts - 1) / a.parts);
-  const int smem = few_smem(a.n, a.stages);
+  const FewPlan f = few_plan(a.T, a.columns, a.red_blocks, swiglu, sms);
+  if (f.token_tiles > 65535) return cudaErrorInvalidValue;
+  a.n = f.n;
+  a.stages = f.stages;
+  const int smem = few_smem(f.n, f.parts, f.stages);
   const auto go = [&](auto kern) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(tiles * a.parts, token_tiles);
+    cfg.gridDim = dim3(f.tiles * f.parts, f.token_tiles);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = a.parts; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[0].val.clusterDim.x = f.parts; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     attr[1] = early_start_attribute();
     cfg.attrs = attr;
     cfg.numAttrs = 2;
@@ -262,7 +284,7 @@ cudaError_t launch_linear_few(GemmMode mode, Activation act, bool swiglu, const 
   const auto with = [&](auto act_c, auto swiglu_c, auto dgrad_c) {
     constexpr Activation ACT = decltype(act_c)::value;
     constexpr bool SWIGLU = decltype(swiglu_c)::value, DGRAD = decltype(dgrad_c)::value;
-    switch (a.parts) {
+    switch (f.parts) {
       case 1: return go(linear_few_kernel<ACT, SWIGLU, DGRAD, 1>);
       case 2: return go(linear_few_kernel<ACT, SWIGLU, DGRAD, 2>);
       case 4: return go(linear_few_kernel<ACT, SWIGLU, DGRAD, 4>);

@@ -366,7 +366,8 @@ void dense_wgrad(const torch::Tensor& dz, const torch::Tensor& x, const torch::T
 bool dense_few(GemmMode mode, const torch::Tensor& weight, const torch::Tensor& x, const torch::Tensor& out, const DenseEpilogue& ep, uint64_t timeout_ns) {
   const bool swiglu = ep.kind == GemmEpilogue::kSwiGLU, fwd = mode == GemmMode::kForward;
   const int64_t red_blocks = (weight.size(fwd ? 1 : 0) + 63) / 64;
-  if (!few_pays(static_cast<int>(x.size(0)), static_cast<int>(out.size(1)), static_cast<int>(red_blocks), swiglu, sm_count(x))) return false;
+  const auto sectors = [](const torch::Tensor& t) { return t.stride(0) % 16 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 32 == 0; };
+  if (!few_pays(static_cast<int>(x.size(0)), static_cast<int>(out.size(1)), static_cast<int>(red_blocks), swiglu, sectors(weight) && sectors(x), sm_count(x))) return false;
   FewArgs a{};
   a.T = static_cast<int>(x.size(0)); a.columns = static_cast<int>(out.size(1));
   a.red_blocks = static_cast<int>(red_blocks);
@@ -376,7 +377,7 @@ bool dense_few(GemmMode mode, const torch::Tensor& weight, const torch::Tensor& 
   a.status = dense_status();
   TORCH_CHECK(a.status != nullptr, "linear: no status block on this device");
   a.timeout_ns = timeout_ns;
-  cuda_check(launch_linear_few(mode, ep.act, swiglu, rows_map(weight, swiglu || !fwd ? 64 : 128), rows_map(x, few_box_rows(a.T)), a, sm_count(x), cur_stream()), "linear");
+  cuda_check(launch_linear_few(mode, ep.act, swiglu, rows_map(weight, swiglu || !fwd ? 64 : 128), rows_map(x, few_plan(a.T, a.columns, a.red_blocks, swiglu, sm_count(x)).n), a, sm_count(x), cur_stream()), "linear");
   return true;
 }
 
