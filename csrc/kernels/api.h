@@ -8,6 +8,8 @@
 
 #include "../runtime/device_sync.cuh"
 
+#include "token_walker.h"
+
 namespace fastb {
 
 // Number of kernels this library has launched in this process (for bench accounting).
@@ -174,6 +176,9 @@ cudaError_t launch_grouped_gemm_tokens(GemmMode mode, GemmEpilogue epi, const To
 struct TokDenseArgs : TokGemmArgs {
   int dense_rows;            // tokens
   int features;              // columns of the output
+  // Set by the launcher: the work split, and the token tiles: how many, of how many 32s, and how many of them of one more.
+  gemm::TokSplit split;
+  int t_tiles, t_units, t_wider;
   // kLinear
   const __nv_bfloat16* bias; // [features] or null
   Activation act;

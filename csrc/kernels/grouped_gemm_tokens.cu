@@ -168,8 +168,8 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
     if (EPI != GemmEpilogue::kStore) prefetch_tmap(&map_c2);
   }
   if (warp == 1) { tmem_alloc_pair(&ctl->tmem_base, kTmemCols); tmem_relinquish_pair(); }
-  const int per_entry = tok_per_entry(p.num_groups);
-  if (warp == 2) {
+  const int per_entry = DENSE ? 1 : tok_per_entry(p.num_groups);
+  if (!DENSE && warp == 2) {
     // Prefix sums of the tile counts over the groups, the widest tile, and whether any group has several token tiles.
     int run = 0, widest = 0, most = 0;
     const int entries = div_up(p.num_groups, per_entry);
@@ -199,10 +199,17 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
   volatile int* abort_flag = &ctl->abort_flag;
 
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const TokSplit split = TokSplit::make(ctl->base[div_up(p.num_groups, per_entry)], p.red_blocks, pairs, ctl->widest, ctl->share_weights != 0);
+  const TokSplit split = [&] {
+    if constexpr (DENSE) return p.split;
+    else return TokSplit::make(ctl->base[div_up(p.num_groups, per_entry)], p.red_blocks, pairs, ctl->widest, ctl->share_weights != 0);
+  }();
   TokSegments segs(split, pair);
   TokTiles<Args> walk{p, ctl->base, per_entry};
   TokSegment sg;
+  auto token_tiles = [&](int g) {
+    if constexpr (DENSE) return p.t_tiles;
+    else return tok_tiles(tok_rows(p, g), p.tile_n);
+  };
   auto give_registers = [] {
     if constexpr (SUB == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   };
@@ -225,7 +232,7 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
         // Where the token panels of a band are a good part of the L2 (p.back_tiles) and a group has several bands, every other
         // wave walks the reduction backwards, from the panel ends that the wave before left in L2: 1093 -> 1132 TFLOP/s at a reduction of
         // 14336 and 985 -> 997 at 28672 over 8192 rows of a training step. Where the tokens stay in L2 anyway there is nothing to win.
-        const bool back = sg.parts == 1 && tok_tiles(tok_rows(p, tc.g), p.tile_n) > p.back_tiles && (((sg.tile - split.cut_tiles) / pairs) & 1);
+        const bool back = sg.parts == 1 && token_tiles(tc.g) > p.back_tiles && (((sg.tile - split.cut_tiles) / pairs) & 1);
         const int k_step = back ? -BK : BK, blocks = sg.kb1 - sg.kb0;
         int k = back ? (p.red_blocks - 1) * BK : sg.kb0 * BK;   // column of the operands that comes next
         auto load_w = [&](int at, int st) {
@@ -753,7 +760,11 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
         }
       }
     }
-    if (EPI == GemmEpilogue::kLinear ? lane == 0 : issuer) bulk_wait_all();  // every bulk store of this CTA has landed before anything is torn down
+    if (DENSE) {
+      if (EPI == GemmEpilogue::kLinear ? lane == 0 : issuer) bulk_wait_read<0>();   // the launch's end waits for the rest of the stores' way
+    } else if (issuer) {
+      bulk_wait_all();  // every bulk store of this CTA has landed before anything is torn down
+    }
   }
   // ---------------- teardown: nobody frees tensor memory while the pair still uses it ----------------
   tc_fence_before_sync();
@@ -820,14 +831,18 @@ cudaError_t launch_dense_gemm(GemmMode mode, GemmEpilogue epi, const TokDenseMap
   if (ctas < 2 || args.num_groups != 1 || args.dense_rows < 1 || args.features < 1 || args.m_tiles != div_up(args.features, kPairM) || args.red_blocks < 1 || args.band_tiles < 1) return cudaErrorInvalidValue;
   if (args.tile_n < 64 || args.tile_n % 32 != 0 || (args.tile_n > kTokAccN && (args.tile_n != 2 * kTokAccN || epi == GemmEpilogue::kLinear))) return cudaErrorInvalidValue;
   if (args.granule != 32 || args.num_counters != 0 || args.status == nullptr || args.gate_counter != nullptr) return cudaErrorInvalidValue;
-  if (dense_is_cut(args, ctas) && (args.partials == nullptr || args.counters == nullptr)) return cudaErrorInvalidValue;
-  if (epi == GemmEpilogue::kSwiGLU && mode == GemmMode::kForward && args.features % kPairM == 0 && (args.keep_gate_up != 0) == (maps.c2 != nullptr)) return launch<GemmMode::kForward, GemmEpilogue::kSwiGLU>(maps, args, ctas, stream);
+  TokDenseArgs a = args;
+  const int rows = tok_rows(a, 0);
+  a.split = dense_split(a, ctas);
+  a.t_tiles = tok_tiles(rows, a.tile_n); a.t_units = rows / 32 / a.t_tiles; a.t_wider = rows / 32 - a.t_units * a.t_tiles;
+  if (a.split.cut_tiles > 0 && (a.partials == nullptr || a.counters == nullptr)) return cudaErrorInvalidValue;
+  if (epi == GemmEpilogue::kSwiGLU && mode == GemmMode::kForward && args.features % kPairM == 0 && (args.keep_gate_up != 0) == (maps.c2 != nullptr)) return launch<GemmMode::kForward, GemmEpilogue::kSwiGLU>(maps, a, ctas, stream);
   if (epi == GemmEpilogue::kStore && args.tile_n > kTokAccN)
-    return mode == GemmMode::kForward ? launch_sub<GemmMode::kForward, GemmEpilogue::kStore, 2>(maps, nullptr, args, ctas, stream)
-           : mode == GemmMode::kDgrad ? launch_sub<GemmMode::kDgrad, GemmEpilogue::kStore, 2>(maps, nullptr, args, ctas, stream) : cudaErrorInvalidValue;
+    return mode == GemmMode::kForward ? launch_sub<GemmMode::kForward, GemmEpilogue::kStore, 2>(maps, nullptr, a, ctas, stream)
+           : mode == GemmMode::kDgrad ? launch_sub<GemmMode::kDgrad, GemmEpilogue::kStore, 2>(maps, nullptr, a, ctas, stream) : cudaErrorInvalidValue;
   if (epi == GemmEpilogue::kLinear && (args.has_residual != 0) == (maps.c2 != nullptr) && (args.keep_pre != 0) == (maps.c3 != nullptr))
-    return mode == GemmMode::kForward ? launch_sub<GemmMode::kForward, GemmEpilogue::kLinear, 1>(maps, maps.c3, args, ctas, stream)
-           : mode == GemmMode::kDgrad ? launch_sub<GemmMode::kDgrad, GemmEpilogue::kLinear, 1>(maps, maps.c3, args, ctas, stream) : cudaErrorInvalidValue;
+    return mode == GemmMode::kForward ? launch_sub<GemmMode::kForward, GemmEpilogue::kLinear, 1>(maps, maps.c3, a, ctas, stream)
+           : mode == GemmMode::kDgrad ? launch_sub<GemmMode::kDgrad, GemmEpilogue::kLinear, 1>(maps, maps.c3, a, ctas, stream) : cudaErrorInvalidValue;
   return cudaErrorInvalidValue;
 }
 

@@ -221,6 +221,10 @@ struct TokTiles {
   const int* base;
   int per_entry, entry = 0, g = 0, g_base = 0;
   FASTB_HD TokTile locate(int tile) {
+    if constexpr (tok_dense<Args>::value) {
+      const TokPlace at = tok_place(tile, p.m_tiles, p.t_tiles, p.band_tiles);
+      return TokTile{0, at.m, 32 * (at.t * p.t_units + (at.t < p.t_wider ? at.t : p.t_wider)), 32 * (p.t_units + (at.t < p.t_wider ? 1 : 0))};
+    }
     if (tile >= base[entry + 1]) {
       while (tile >= base[entry + 1]) ++entry;
       g = entry * per_entry; g_base = base[entry];
