@@ -208,7 +208,7 @@ struct FewArgs {
 bool few_pays(int T, int columns, int red_blocks, bool swiglu, bool sectors, int sms);   // sectors: the operands' rows start at multiples of 32 bytes
 struct FewPlan {
   int tiles, token_tiles, n;     // tiles of the weight's rows, of the tokens, and tokens of one: map_x's boxes are {64, n}, map_w's {64, 128}, SwiGLU's and dgrad's {64, 64}
-  int parts, stages;             // CTAs that share a tile's reduction, operand stages of one
+  int parts, stages, smem;       // CTAs that share a tile's reduction, operand stages and shared memory of one
 };
 FewPlan few_plan(int T, int columns, int red_blocks, bool swiglu, int sms);
 cudaError_t launch_linear_few(GemmMode mode, Activation act, bool swiglu, const CUtensorMap& map_w, const CUtensorMap& map_x, const FewArgs& args, int sms, cudaStream_t stream);

@@ -241,6 +241,7 @@ FewPlan few_plan(int T, int columns, int red_blocks, bool swiglu, int sms) {
   f.token_tiles = (T + f.n - 1) / f.n;
   f.parts = few_parts(f.tiles * f.token_tiles, red_blocks, f.n, sms);
   f.stages = std::min(few_stages(f.n, f.parts, f.tiles * f.token_tiles * f.parts <= sms ? kFewDeepSmem : kFewSmem), (red_blocks + f.parts - 1) / f.parts);
+  f.smem = few_smem(f.n, f.parts, f.stages);
   return f;
 }
 
@@ -264,14 +265,13 @@ cudaError_t launch_linear_few(GemmMode mode, Activation act, bool swiglu, const 
   if (f.token_tiles > 65535) return cudaErrorInvalidValue;
   a.n = f.n;
   a.stages = f.stages;
-  const int smem = few_smem(f.n, f.parts, f.stages);
   const auto go = [&](auto kern) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, f.smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(f.tiles * f.parts, f.token_tiles);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = f.smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;

@@ -485,6 +485,10 @@ void bind_moe(py::module_& m) {
         py::arg("band_rows"), py::arg("map_c") = nullptr, py::arg("map_c2") = nullptr, py::arg("direct_epilogue") = false, py::arg("a_scales") = py::none(),
         py::arg("group_rows") = py::none(), py::arg("gate_tile_rows") = 0, py::arg("wide") = false);
   m.def("tok_dense_tile", &gemm::tok_dense_tile, py::arg("rows"), py::arg("m_tiles"), py::arg("kb_tile"), py::arg("pairs"));
+  m.def("few_plan", [](int tokens, int columns, int red_blocks, bool swiglu, int sms) {
+    const FewPlan f = few_plan(tokens, columns, red_blocks, swiglu, sms);
+    return py::make_tuple(f.tiles, f.token_tiles, f.n, f.parts, f.stages, f.smem);
+  }, py::arg("tokens"), py::arg("columns"), py::arg("red_blocks"), py::arg("swiglu"), py::arg("sms"));
   m.def("tok_wide", &gemm::tok_wide, py::arg("swiglu"), py::arg("reduction"), py::arg("mean_rows"), py::arg("waves"));
   m.def("wgrad_wide", &gemm::wgrad_wide, py::arg("row_tiles"), py::arg("columns"), py::arg("pairs"), py::arg("mean_rows"));
   m.def("grouped_gemm_smem_bytes", &grouped_gemm_smem_bytes);

@@ -259,3 +259,19 @@ def test_its_backward_has_no_gradient():
     (g,) = torch.autograd.grad(fused.linear(x, w, activation="silu").float().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="no gradient"):
         g.float().sum().backward()
+
+
+# (tokens, reduction, columns): one, two, four and eight CTAs a tile; their sums beside the stages (up to 64 tokens a tile) and in their place; all of an SM's shared memory and
+# half of it; the last part of the reduction and the last tile cut off.
+FEW = [(1, 4104, 264), (16, 4096, 4736), (13, 8200, 136), (16, 4160, 1000), (17, 4104, 264), (60, 1032, 1000), (64, 520, 4744), (48, 1096, 9480), (100, 2056, 640), (128, 4104, 1288), (90, 1024, 9472),
+       (250, 1104, 2056), (500, 1032, 1000), (400, 200, 9480), (600, 528, 4104), (1000, 128, 4096), (1100, 264, 8328), (2, 72, 40008)]
+
+
+@pytest.mark.parametrize("T,K,N", FEW)
+def test_whole_numbers_are_exact_however_few_tokens_are_shared_out(T, K, N):
+    test_whole_numbers_are_exact(T, K, N)
+
+
+@pytest.mark.parametrize("T,K,I", [(1, 4104, 256), (16, 4096, 2048), (60, 1032, 256), (64, 520, 4864), (100, 2056, 384), (128, 4104, 1152), (250, 1032, 1024), (500, 264, 2432)])
+def test_swiglu_however_few_tokens_are_shared_out(T, K, I):
+    test_swiglu(T, K, I)
