@@ -200,7 +200,7 @@ struct FewArgs {
   const __nv_bfloat16* residual;   // [T, columns], rows residual_stride elements apart, 8-byte aligned, or null
   long long residual_stride;
   __nv_bfloat16* out;          // [T, columns]
-  __nv_bfloat16* pre;          // what the activation is taken of: [T, columns], SwiGLU [T, 2 columns]; or null
+  __nv_bfloat16* pre;          // what the activation is taken of: [T, columns], SwiGLU [T, 4 columns] (gate and up, and what the rounding took from them); or null
   int n, stages;               // set by the launcher: tokens of a tile, operand stages
   DeviceStatus* status;
   unsigned long long timeout_ns;
@@ -496,6 +496,8 @@ cudaError_t launch_fold_slices(const float* sums, int slices, int m_tiles, int n
 // dz = dy * act'(z) [T, N] (kNone: dz is dy, nothing is written) and, with partials [blocks][N], dbias [N] = the column sums of dz. N % 8 == 0.
 int linear_dz_blocks(int T, int N, int sms);
 cudaError_t launch_linear_dz(Activation act, const __nv_bfloat16* dy, const __nv_bfloat16* z, __nv_bfloat16* dz, float* partials, int T, int N, int blocks, __nv_bfloat16* dbias, cudaStream_t stream);
+// dz [T, 2 inter] of SwiGLU (tiles of 128 gates and 128 ups) from dy [T, inter] and pre [T, 4 inter]: z, and what its rounding to bf16 took off.
+cudaError_t launch_linear_swiglu_dz(const __nv_bfloat16* dy, const __nv_bfloat16* pre, __nv_bfloat16* dz, int T, int inter, cudaStream_t stream);
 // AdamW on bf16 parameters with fp32 master weights and moments, several tensors per launch.
 struct AdamWTensor {
   __nv_bfloat16* param;

@@ -15,6 +15,11 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<uint32_t*>(&v);
 }
+// What pack_bf16 takes from the two, as bf16: both together have 16 bits of a value. An infinity leaves nothing.
+__device__ __forceinline__ uint32_t pack_rest(float a, float b) {
+  const float x = __bfloat162float(__float2bfloat16_rn(a)), y = __bfloat162float(__float2bfloat16_rn(b));
+  return pack_bf16(fabsf(x) < INFINITY ? a - x : 0.0f, fabsf(y) < INFINITY ? b - y : 0.0f);
+}
 // 1 / (1 + exp(-x)) and x times that. Built with --use_fast_math (FASTB_FAST_MATH): two operations of the special-function unit; a division, approximate
 // too, takes more of them, for divisors above 2^126, whose reciprocal is zero anyway. Built without: the rounded division.
 #ifdef FASTB_FAST_MATH

@@ -76,7 +76,10 @@ struct __align__(8) TokCtl {
 };
 // Boxes of half of the ring. Dense stores have two buffers of two there; kLinear has the room of one for each of its four warps, of two with the pre-activation.
 __host__ __device__ constexpr int epi_boxes(GemmEpilogue e, bool dense = false) { return e == GemmEpilogue::kStore ? (dense ? 4 : 2) : e == GemmEpilogue::kSwiGLU ? 3 : 4; }
-__host__ __device__ constexpr int ring_half(GemmEpilogue e, bool dense, bool keep_pre) { return epi_boxes(e, dense) * (e == GemmEpilogue::kLinear && keep_pre ? 2 : 1) * kBox; }
+// A dense SwiGLU that keeps gate and up has two more boxes, for what their rounding takes off.
+__host__ __device__ constexpr int ring_half(GemmEpilogue e, bool dense, bool keep_pre) {
+  return (epi_boxes(e, dense) * (e == GemmEpilogue::kLinear && keep_pre ? 2 : 1) + (e == GemmEpilogue::kSwiGLU && dense && keep_pre ? 2 : 0)) * kBox;
+}
 constexpr int kSmemLimit = 227 * 1024;
 constexpr int other_bytes(GemmEpilogue e, bool dense, bool keep_pre) { return 2 * ring_half(e, dense, keep_pre) + 1024 + static_cast<int>(sizeof(TokCtl)); }
 // Operand stages that fit. Tiles of up to 256 tokens: 6 of 32 KiB. Where few tokens meet the weights, the loop is bound by
@@ -149,6 +152,7 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
   uint8_t* ring = tiles + stages * stage_size;
   bool keep_pre = false;
   if constexpr (EPI == GemmEpilogue::kLinear) keep_pre = p.keep_pre != 0;
+  else if constexpr (DENSE && EPI == GemmEpilogue::kSwiGLU) keep_pre = p.keep_gate_up != 0;
   TokCtl* ctl = reinterpret_cast<TokCtl*>(ring + 2 * ring_half(EPI, DENSE, keep_pre));
   if (!DENSE && !p.early) grid_dependency_wait();   // dense: nothing that the set-up reads was written by a kernel (1024 x 2048 -> 4096 18.5 -> 17.0 us, 1235 x 1000 -> 2760 18.8 -> 16.5)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -459,7 +463,7 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
       };
       // Buffers of a group's half of the ring, which its steps take in turn.
       const int bufs = !DENSE ? 1 : EPI == GemmEpilogue::kSwiGLU ? 2 - p.keep_gate_up : 2;
-      auto buffer = [&](uint32_t i) { return ring + group * kRing + (bufs == 2 ? i & 1u : 0u) * (EPI == GemmEpilogue::kSwiGLU ? 1 : 2) * kBox; };
+      auto buffer = [&](uint32_t i) { return ring + group * ring_half(EPI, DENSE, keep_pre) + (bufs == 2 ? i & 1u : 0u) * (EPI == GemmEpilogue::kSwiGLU ? 1 : 2) * kBox; };
       auto acquire = [&]() {
         if constexpr (DENSE) {
           if (issuer) { if (bufs == 2) bulk_wait_read<1>(); else bulk_wait_read<0>(); }
@@ -555,6 +559,12 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
           to_bf16(r, h);
           put(sb + kBox, quarter * 2, h);
           put(sb + 2 * kBox, quarter * 2, h + 8);
+          if constexpr (DENSE) {   // and what the rounding takes from them
+#pragma unroll
+            for (int i = 0; i < 16; ++i) h[i] = pack_rest(as_f(r[2 * i]), as_f(r[2 * i + 1]));
+            put(sb + 3 * kBox, quarter * 2, h);
+            put(sb + 4 * kBox, quarter * 2, h + 8);
+          }
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) h[i] = pack_bf16(silu(as_f(r[2 * i])) * as_f(r[16 + 2 * i]), silu(as_f(r[2 * i + 1])) * as_f(r[17 + 2 * i]));
@@ -566,6 +576,10 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
           if (p.keep_gate_up) {
             tma_store_2d(&map_c2, b + kBox, tc.m * kPairM + cta * 64, y);
             tma_store_2d(&map_c2, b + 2 * kBox, tc.m * kPairM + kHalfM + cta * 64, y);
+            if constexpr (DENSE) {   // the columns behind all gates and ups
+              tma_store_2d(&map_c2, b + 3 * kBox, p.features + tc.m * kPairM + cta * 64, y);
+              tma_store_2d(&map_c2, b + 4 * kBox, p.features + tc.m * kPairM + kHalfM + cta * 64, y);
+            }
           }
           bulk_commit();
         }
@@ -779,6 +793,7 @@ cudaError_t launch_sub(const TokGemmMaps& m, const CUtensorMap* c3, Args args, i
   constexpr bool dense = tok_dense<Args>::value;
   bool keep_pre = false;
   if constexpr (EPI == GemmEpilogue::kLinear) keep_pre = args.keep_pre != 0;
+  else if constexpr (dense && EPI == GemmEpilogue::kSwiGLU) keep_pre = args.keep_gate_up != 0;
   args.stages = stages_for(EPI, args.tile_n, dense, keep_pre);
   const int smem = smem_bytes(EPI, args.tile_n, dense, keep_pre);
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);

@@ -55,6 +55,7 @@ __device__ __forceinline__ float4 ld_sums(uint32_t addr) {
 __device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ void st_own(uint32_t addr, uint32_t v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ uint2 pack4(const float4& v) { return make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w)); }
+__device__ __forceinline__ uint2 rest4(const float4& v) { return make_uint2(pack_rest(v.x, v.y), pack_rest(v.z, v.w)); }
 __device__ __forceinline__ float4 unpack4(const __nv_bfloat16* at) {
   const uint2 v = *reinterpret_cast<const uint2*>(at);
   const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.x)), b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.y));
@@ -151,9 +152,11 @@ __global__ void __launch_bounds__(kThreads) linear_few_kernel(const __grid_const
     const long long at = static_cast<long long>(t) * p.columns + col;
     if (SWIGLU) {
       if (p.pre != nullptr) {
-        __nv_bfloat16* gu = p.pre + static_cast<long long>(t) * p.columns * 2 + tile / 2 * 256 + tile % 2 * 64 + f;
+        __nv_bfloat16* gu = p.pre + static_cast<long long>(t) * p.columns * 4 + tile / 2 * 256 + tile % 2 * 64 + f;
         *reinterpret_cast<uint2*>(gu) = pack4(v);
         *reinterpret_cast<uint2*>(gu + 128) = pack4(up);
+        *reinterpret_cast<uint2*>(gu + 2 * p.columns) = rest4(v);
+        *reinterpret_cast<uint2*>(gu + 2 * p.columns + 128) = rest4(up);
       }
       v.x = silu(v.x) * up.x; v.y = silu(v.y) * up.y; v.z = silu(v.z) * up.z; v.w = silu(v.w) * up.w;
     } else {

@@ -271,7 +271,7 @@ CUtensorMap rows_map(const torch::Tensor& m, int box_rows, int box_cols = 64) {
 
 struct DenseEpilogue {
   GemmEpilogue kind = GemmEpilogue::kLinear;
-  const torch::Tensor *bias = nullptr, *residual = nullptr, *pre = nullptr;   // pre: pre-activation, or gate|up of kSwiGLU
+  const torch::Tensor *bias = nullptr, *residual = nullptr, *pre = nullptr;   // pre: pre-activation, or gate|up of kSwiGLU and what their rounding took off
   Activation act = Activation::kNone;
 };
 
@@ -399,7 +399,7 @@ LinearOut linear_forward(const torch::Tensor& x, const torch::Tensor& weight, co
   c10::cuda::CUDAGuard guard(x.device());
   LinearOut o{fresh(shape, x), {}};
   const bool pre = keep && kind != LinearKind::kNone;
-  if (pre) o.pre = fresh({T, N}, x);
+  if (pre) o.pre = fresh({T, kind == LinearKind::kSwiGLU ? 2 * N : N}, x);   // SwiGLU: with what the rounding took off
   if (T == 0) return o;
   const torch::Tensor xm = tma_rows(x, K), wm = kind == LinearKind::kSwiGLU && !weight.is_contiguous() ? weight.contiguous() : tma_rows(weight, K), ym = o.y.view({T, cols});
   torch::Tensor rm, bm;
@@ -455,8 +455,8 @@ struct Linear : torch::autograd::Function<Linear> {
         if (kind == LinearKind::kSwiGLU) {
           const torch::Tensor d = dy.contiguous();
           dz = fresh({T, N}, dy);
-          cuda_check(launch_swiglu_bwd(reinterpret_cast<const __nv_bfloat16*>(saved[2].data_ptr()), reinterpret_cast<const __nv_bfloat16*>(d.data_ptr()), reinterpret_cast<__nv_bfloat16*>(dz.data_ptr()),
-                                       T, static_cast<int>(N / 2), nullptr, cur_stream()), "linear backward: swiglu");
+          cuda_check(launch_linear_swiglu_dz(reinterpret_cast<const __nv_bfloat16*>(d.data_ptr()), reinterpret_cast<const __nv_bfloat16*>(saved[2].data_ptr()), reinterpret_cast<__nv_bfloat16*>(dz.data_ptr()),
+                                             static_cast<int>(T), static_cast<int>(N / 2), cur_stream()), "linear backward: swiglu");
         } else if (kind != LinearKind::kNone || want_b) {
           const torch::Tensor d = dy.contiguous();
           torch::Tensor partials;

@@ -68,8 +68,8 @@ def memory_plan(cfg: MoEConfig, world: int, capacity_factor: float = 0.0) -> Dic
     workspace = 2 * cap * I + (2 * row if cfg.fp8_dispatch else 0)
     if cfg.training:
         workspace += 2 * cap * (2 * I + I + 2 * I)
-    if cfg.shared_inter:   # the shared expert's activations, and in training its gate|up and their gradients
-        workspace += 2 * T * cfg.shared_inter * (1 if not cfg.training else 2 + 2 + 2)
+    if cfg.shared_inter:   # the shared expert's activations, and in training its gate|up (twice 16 bits each) and their gradients
+        workspace += 2 * T * cfg.shared_inter * (1 if not cfg.training else 4 + 2 + 2)
     params = el * 3 * H * I + H * cfg.num_experts + cfg.vocab * H + 3 * H * cfg.shared_inter
     weights = 2 * params
     grads = 2 * params if cfg.training else 0

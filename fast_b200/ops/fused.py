@@ -106,7 +106,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     result's shape. ``activation``: None, "relu", "silu", "gelu" (z Phi(z)), or "swiglu": the weight holds tiles of 128 gate rows and the 128 up rows of
     the same features, as an expert's does (``models.moe.interleave_gate_up``), outputs a multiple of 256, the result [..., outputs / 2] =
     silu(gate) * up, without bias and residual. From none to 2^30 rows; rows that are not contiguous, 16-byte aligned and a multiple of 16 bytes
-    apart are copied first. Where a gradient needs it, what the activation was taken of is kept in bf16. A device wait that gave up is
+    apart are copied first. Where a gradient needs it, what the activation was taken of is kept in bf16 (swiglu: in two bf16, 16 bits of each value). A device wait that gave up is
     reported by ``ops.gemm.check()``."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"linear: activation must be one of {', '.join(map(repr, _ACTIVATIONS))}, got {activation!r}")

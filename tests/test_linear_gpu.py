@@ -275,3 +275,20 @@ def test_whole_numbers_are_exact_however_few_tokens_are_shared_out(T, K, N):
 @pytest.mark.parametrize("T,K,I", [(1, 4104, 256), (16, 4096, 2048), (60, 1032, 256), (64, 520, 4864), (100, 2056, 384), (128, 4104, 1152), (250, 1032, 1024), (500, 264, 2432)])
 def test_swiglu_however_few_tokens_are_shared_out(T, K, I):
     test_swiglu(T, K, I)
+
+
+@pytest.mark.parametrize("T,K,I", [(60, 512, 1024), (2000, 640, 512), (2000, 128, 4096), (1100, 2048, 2048)])
+def test_swiglu_gradients_have_the_error_of_two_roundings(T, K, I):
+    """That of dz, which both products take in bf16, and of the result. A gate and an up rounded to bf16 on the way would add a third as large: 1.2 times as much."""
+    x, w1, w3, dy = normal((T, K), 1), normal((I, K), 2, K**-0.5), normal((I, K), 3, K**-0.5), normal((T, I), 4)
+    w, leaf = interleave_gate_up(w1.unsqueeze(0), w3.unsqueeze(0))[0].requires_grad_(), x.clone().requires_grad_()
+    dx, dw = torch.autograd.grad(fused.linear(leaf, w, activation="swiglu"), [leaf, w], dy)
+    g, u = (x.double() @ t.double().t() for t in (w1, w3))
+    g.requires_grad_(), u.requires_grad_()
+    dg, du = torch.autograd.grad(torch.nn.functional.silu(g) * u, [g, u], dy.double())
+    rg, ru = dg.to(BF).double(), du.to(BF).double()
+    both = lambda a, b: interleave_gate_up((a.t() @ x.double()).unsqueeze(0), (b.t() @ x.double()).unsqueeze(0))[0]
+    for got, exact, rounded in ((dx, dg @ w1.double() + du @ w3.double(), rg @ w1.double() + ru @ w3.double()), (dw, both(dg, du), both(rg, ru))):
+        # 1.05: the errors are sums of thousands of independent roundings, and gate and up keep 16 bits
+        assert (got.double() - exact).norm() <= 1.05 * (rounded.to(BF).double() - exact).norm()
+    gemm.check()
