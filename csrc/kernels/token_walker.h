@@ -92,8 +92,8 @@ struct TokSplit {
 // Most tokens of a tile for one weight matrix and `rows` tokens (TokDenseArgs), a multiple of 32 up to 256: of the widths that need no more rounds of the
 // GPU than 256 does (up to three), the one whose launch takes the fewest cycles by the counts above, with 600 a step of 32 tokens for the last tiles' way
 // out, if it saves a twenty-fifth. Narrower tiles keep more pairs busy, and spare the exchange of a cut round. us, 256 -> this: 1235 x 1000 -> 2760
-// (55 tiles, 66 of 224) 14.5 -> 13.9, 600 x 4096 -> 4096 (48, 64 of 160) 28.4 -> 22.2, 1500 x 8192 -> 2048 (48, 72 of 192) 47.5 -> 40.9, SwiGLU of 500 x 7168 -> 4096
-// (32, 64 of 128) 35.5 -> 30.7, 700 x 2048 -> 7168 (84 in two rounds, 140 of 160) 32.5 -> 27.2; more rounds lose: 3000 x 256 -> 3000 in three instead of two 13.3 -> 15.6.
+// (55 tiles, 66 of 224) 12.3 -> 11.8, 600 x 4096 -> 4096 (48, 64 of 160) 22.7 -> 19.4, 1500 x 8192 -> 2048 (48, 72 of 192) 48.3 -> 38.9, SwiGLU of 600 x 7168 -> 4096
+// (48, 64 of 160) 40.7 -> 33.4, 700 x 2048 -> 7168 (84 in two rounds, 140 of 160) 26.6 -> 21.3; more rounds lose: 3000 x 520 -> 3000 in three instead of two 15.2 -> 17.2.
 inline int tok_dense_tile(int rows, int m_tiles, int kb_tile, int pairs) {
   const int fewest = tok_tiles(ceil_to(rows, 32), kTokAccN);
   const long long rounds = (static_cast<long long>(fewest) * m_tiles + pairs - 1) / pairs;
