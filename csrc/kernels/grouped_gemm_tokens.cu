@@ -588,7 +588,7 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
       if constexpr (EPI == GemmEpilogue::kLinear) {
         // Every warp by itself, 32 tokens of its 32 features at a time: no barrier among the warps, which meet only at the accumulators. A residual box
         // comes in by TMA while the one before it is worked on, and is overwritten by what goes out. Only short reductions are bound by this: 8192 x
-        // 64 -> 8192 with relu 74.7 us with boxes shared by two warps and two barriers a step, 58.5 so; from a reduction of 1024 on the products are.
+        // 64 -> 8192 with relu 74.7 us with boxes shared by two warps and two barriers a step, 52 so; from a reduction of 1024 on the products are.
         static_assert(GROUPS == 2, "half of the steps a group");
         const int f0 = feat0 + quarter * 32, me = group * 4 + quarter, slot_bytes = (keep_pre ? 2 : 1) * kWarpBox;
         const bool mine = f0 < p.features, residual = p.has_residual && mine;
@@ -844,14 +844,14 @@ bool dense_is_cut(const TokDenseArgs& args, int ctas) { return dense_split(args,
 
 cudaError_t launch_dense_gemm(GemmMode mode, GemmEpilogue epi, const TokDenseMaps& maps, const TokDenseArgs& args, int ctas, cudaStream_t stream) {
   if (ctas < 2 || args.num_groups != 1 || args.dense_rows < 1 || args.features < 1 || args.m_tiles != div_up(args.features, kPairM) || args.red_blocks < 1 || args.band_tiles < 1) return cudaErrorInvalidValue;
-  if (args.tile_n < 64 || args.tile_n % 32 != 0 || (args.tile_n > kTokAccN && (args.tile_n != 2 * kTokAccN || epi == GemmEpilogue::kLinear))) return cudaErrorInvalidValue;
+  if (args.tile_n < 64 || args.tile_n % 32 != 0 || (args.tile_n > kTokAccN && (args.tile_n != 2 * kTokAccN || epi != GemmEpilogue::kStore))) return cudaErrorInvalidValue;
   if (args.granule != 32 || args.num_counters != 0 || args.status == nullptr || args.gate_counter != nullptr) return cudaErrorInvalidValue;
   TokDenseArgs a = args;
   const int rows = tok_rows(a, 0);
   a.split = dense_split(a, ctas);
   a.t_tiles = tok_tiles(rows, a.tile_n); a.t_units = rows / 32 / a.t_tiles; a.t_wider = rows / 32 - a.t_units * a.t_tiles;
   if (a.split.cut_tiles > 0 && (a.partials == nullptr || a.counters == nullptr)) return cudaErrorInvalidValue;
-  if (epi == GemmEpilogue::kSwiGLU && mode == GemmMode::kForward && args.features % kPairM == 0 && (args.keep_gate_up != 0) == (maps.c2 != nullptr)) return launch<GemmMode::kForward, GemmEpilogue::kSwiGLU>(maps, a, ctas, stream);
+  if (epi == GemmEpilogue::kSwiGLU && mode == GemmMode::kForward && args.features % kPairM == 0 && (args.keep_gate_up != 0) == (maps.c2 != nullptr)) return launch_sub<GemmMode::kForward, GemmEpilogue::kSwiGLU, 1>(maps, nullptr, a, ctas, stream);
   if (epi == GemmEpilogue::kStore && args.tile_n > kTokAccN)
     return mode == GemmMode::kForward ? launch_sub<GemmMode::kForward, GemmEpilogue::kStore, 2>(maps, nullptr, a, ctas, stream)
            : mode == GemmMode::kDgrad ? launch_sub<GemmMode::kDgrad, GemmEpilogue::kStore, 2>(maps, nullptr, a, ctas, stream) : cudaErrorInvalidValue;

@@ -289,10 +289,11 @@ void dense_gemm(GemmMode mode, const torch::Tensor& weight, const torch::Tensor&
   a.tile_n = a.dense_rows <= 64 ? 64 : a.dense_rows <= 128 ? 128 : gemm::tok_dense_tile(a.dense_rows, a.m_tiles, a.red_blocks, ctas / 2);
   GemmEpilogue kind = ep.kind;
   const bool plain = ep.kind == GemmEpilogue::kLinear && ep.act == Activation::kNone && !ep.bias && !ep.residual && !ep.pre;
-  if ((plain || ep.kind == GemmEpilogue::kSwiGLU) && a.tile_n == 256 &&
-      gemm::tok_wide(ep.kind == GemmEpilogue::kSwiGLU, static_cast<int>(reduction), a.dense_rows, (a.dense_rows + 511) / 512 * (features / 256.0) / (ctas / 2))) {
+  // SwiGLU, whose kept gate and up would leave three stages, takes no wide tiles: us on them, without: 300 x 4096 -> 104448 233 to 273, 246; kept 312 to 331, 282 to 294;
+  // 280 x 4096 -> 163840 382 to 387, 358 to 362; kept 439 to 448, 422 to 426.
+  if (plain && a.tile_n == 256 && gemm::tok_wide(false, static_cast<int>(reduction), a.dense_rows, (a.dense_rows + 511) / 512 * (features / 256.0) / (ctas / 2))) {
     a.tile_n = 512;
-    if (plain) kind = GemmEpilogue::kStore;
+    kind = GemmEpilogue::kStore;
   }
   a.band_tiles = gemm::tok_band(0, 64 * a.red_blocks, a.m_tiles, a.tile_n);
   a.back_tiles = gemm::tok_back_tiles(64 * a.red_blocks, a.band_tiles, std::max(a.tile_n, gemm::kTokAccN));
