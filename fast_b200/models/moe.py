@@ -147,7 +147,7 @@ class MoELayer(nn.Module):
 
     ``balance`` ("softmax" or "sigmoid" scores, see ``ops.fused.balance_loss``): every training forward pass leaves the router's balance loss over
     this rank's tokens in ``balance_loss`` (with its gradient; add it to the loss, times a coefficient, before the next forward pass) and the
-    experts' counts in ``expert_counts``. ``shared_inter`` > 0: a dense SwiGLU expert of that width (a multiple of 128; replicated on every rank) that every
+    experts' counts in ``expert_counts``; a forward-only pass (``eval()`` or no gradients) makes neither and leaves both None. ``shared_inter`` > 0: a dense SwiGLU expert of that width (a multiple of 128; replicated on every rank) that every
     token goes through, its output added to the routed experts'."""
 
     def __init__(self, comm: Communicator, hidden: int, inter: int, num_experts: int, top_k: int, max_tokens: int, fp8_dispatch: bool = False,
@@ -199,11 +199,13 @@ class MoELayer(nn.Module):
     def forward_graphed(self, x: torch.Tensor) -> torch.Tensor:
         """Replay the captured layer on ``x`` (same shape as at capture). The result lives in a buffer
         owned by the graph and is overwritten by the next replay."""
+        self._drop_balance()
         self._gx.copy_(x)
         self._graph.replay()
         return self._gout
 
     def _infer(self, x: torch.Tensor, quantised=None) -> torch.Tensor:
+        self._drop_balance()
         rs = self.engine.route_and_send(x, self.gate, self.router_bias, quantised)
         self.last_route = rs
         self.engine.experts_forward(self.w13, self.w2, rs, settled=True)
@@ -216,7 +218,8 @@ class MoELayer(nn.Module):
         return fused.linear(fused.linear(x, self.shared_w13, activation="swiglu"), self.shared_w2, residual=out)
 
     def _drop_balance(self) -> None:
-        """Before a pass keeps anything: the last one's balance loss holds its graph, and with it the rows it kept where no backward pass has freed them."""
+        """Before a pass keeps anything: the last one's balance loss holds its graph, and with it the rows it kept where no backward pass has freed them;
+        and after a forward-only pass it would be another batch's."""
         self.balance_loss = self.expert_counts = None
 
     def _note_balance(self, logits: torch.Tensor, mask: Optional[torch.Tensor]) -> None:
@@ -286,7 +289,7 @@ class MoELayer(nn.Module):
 
 class MixtralBlockModel(nn.Module):
     """Embedding -> RMSNorm -> MoE block (+ residual) -> mean-square loss; Mixtral-8x7B shapes by default. ``balance_coef`` > 0 adds that much of the
-    router's balance loss (``moe.balance_loss``), ``shared_inter`` > 0 a shared expert (see ``MoELayer``)."""
+    router's balance loss (``moe.balance_loss``) in training passes (a forward-only pass gives the mean square alone), ``shared_inter`` > 0 a shared expert (see ``MoELayer``)."""
 
     def __init__(self, comm: Communicator, vocab: int = 32000, hidden: int = 4096, inter: int = 14336, num_experts: int = 8, top_k: int = 2,
                  max_tokens: int = 8 * 4096, capacity_rows: Optional[int] = None, seed: int = 0, balance_coef: float = 0.0, shared_inter: int = 0):
@@ -308,7 +311,7 @@ class MixtralBlockModel(nn.Module):
     def forward(self, token_ids: torch.Tensor) -> torch.Tensor:
         h = fused.embedding(token_ids.reshape(-1), self.embed)
         loss = self.moe.mean_square_from_residual(h, self.norm_w, self.eps)
-        return loss + self.balance_coef * self.moe.balance_loss if self.balance_coef else loss
+        return loss if self.moe.balance_loss is None else loss + self.balance_coef * self.moe.balance_loss
 
 
 @torch.no_grad()
