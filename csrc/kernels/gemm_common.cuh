@@ -33,6 +33,12 @@ __device__ __forceinline__ float silu(float x) { return x * sigmoid(x); }
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __expf(-x)); }
 __device__ __forceinline__ float silu(float x) { return x / (1.0f + __expf(-x)); }
 #endif
+// max(x, 0); NaN stays NaN (fmaxf would make it 0, and a diverged row look healthy).
+__device__ __forceinline__ float relu(float x) {
+  float r;
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(x));
+  return r;
+}
 // Phi(z), the normal distribution's integral, with e = exp(-z^2 / 2): Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26,
 // 1 - erf(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + 0.3275911 x), to 1.5e-7 for x >= 0; the other half by symmetry. The exponential serves the
 // density as well. (The general error function made the activation's backward pass a matter of arithmetic: 294 us for 8192 x 14336, where memory wants 107.)

@@ -63,7 +63,7 @@ __device__ __forceinline__ float4 unpack4(const __nv_bfloat16* at) {
 }
 template <Activation ACT>
 __device__ __forceinline__ float activated(float z) {
-  return ACT == Activation::kRelu ? fmaxf(z, 0.0f) : ACT == Activation::kSilu ? silu(z) : ACT == Activation::kGelu ? gelu(z) : z;
+  return ACT == Activation::kRelu ? relu(z) : ACT == Activation::kSilu ? silu(z) : ACT == Activation::kGelu ? gelu(z) : z;
 }
 
 // DGRAD: out = x W, the weight's columns are the features (operand A MN-major).

@@ -15,10 +15,10 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 
-// act'(z)
+// act'(z); that of NaN is NaN
 template <Activation ACT>
 __device__ __forceinline__ float slope(float z) {
-  if (ACT == Activation::kRelu) return z > 0.0f ? 1.0f : 0.0f;
+  if (ACT == Activation::kRelu) return z > 0.0f ? 1.0f : z <= 0.0f ? 0.0f : z;
   if (ACT == Activation::kSilu) {
     const float s = gemm::sigmoid(z);
     return s * (1.0f + z * (1.0f - s));
