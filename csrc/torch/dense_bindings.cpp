@@ -493,14 +493,11 @@ torch::Tensor linear(const torch::Tensor& x, const torch::Tensor& weight, const 
   if (!recorded(x, weight, bias, residual)) return linear_forward(x, weight, bias, static_cast<LinearKind>(kind), residual, false, timeout_ns).y;
   return Linear::apply(x, weight, bias, residual, kind, timeout_ns)[0];
 }
-// What a dense launch on the current device reported, which is forgotten with that: (code, site, detail, seen, want). Synchronises the current stream.
-py::tuple take_dense_status() {
-  DeviceStatus s{}, *d = dense_status();
+// Where linear layers on the current device report a wait that gave up. All of the device's users share it, so reading leaves it as it is.
+std::shared_ptr<StatusPy> dense_block() {
+  DeviceStatus* d = dense_status();
   TORCH_CHECK(d != nullptr, "linear: no status block on this device");
-  cuda_check(cudaStreamSynchronize(cur_stream()), "sync before status read");
-  cuda_check(cudaMemcpy(&s, d, sizeof(s), cudaMemcpyDeviceToHost), "read status");
-  if (s.code != 0) cuda_check(cudaMemset(d, 0, sizeof(s)), "clear status");
-  return py::make_tuple(s.code, s.site, s.detail, s.seen, s.want);
+  return std::make_shared<StatusPy>(d);
 }
 
 }  // namespace
@@ -509,6 +506,6 @@ void bind_dense(py::module_& m) {
   m.def("add_rms_norm", &add_rms_norm, py::arg("x"), py::arg("weight"), py::arg("eps"), py::arg("residual"), py::arg("quantise"));
   m.def("balance_loss", &balance_loss, py::arg("logits"), py::arg("topk_idx"), py::arg("mask"), py::arg("sigmoid"));
   m.def("linear", &linear, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("residual"), py::arg("kind"), py::arg("timeout_s"));
-  m.def("take_dense_status", &take_dense_status);
+  m.def("dense_status", &dense_block);
   m.def("dequantise_rows", &dequantise_rows, py::arg("q"), py::arg("scales"));
 }

@@ -31,11 +31,15 @@ struct HeapPy {
 // ---- status block -------------------------------------------------------------------------------
 struct StatusPy {
   DeviceStatus* d = nullptr;
+  bool owned = true;
+  explicit StatusPy(DeviceStatus* of_others) : d(of_others), owned(false) {}   // a view of a block that stays where it is
   StatusPy() {
     cuda_check(cudaMalloc(reinterpret_cast<void**>(&d), sizeof(DeviceStatus)), "cudaMalloc status");
     cuda_check(cudaMemset(d, 0, sizeof(DeviceStatus)), "clear status");
   }
-  ~StatusPy() { if (d) cudaFree(d); }
+  StatusPy(const StatusPy&) = delete;
+  StatusPy& operator=(const StatusPy&) = delete;
+  ~StatusPy() { if (d && owned) cudaFree(d); }
   // Synchronises the current stream, then returns (code, site, detail, seen, want).
   py::tuple read() const {
     DeviceStatus s;

@@ -107,7 +107,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     the same features, as an expert's does (``models.moe.interleave_gate_up``), outputs a multiple of 256, the result [..., outputs / 2] =
     silu(gate) * up, without bias and residual. From none to 2^30 rows; rows that are not contiguous, 16-byte aligned and a multiple of 16 bytes
     apart are copied first. Where a gradient needs it, what the activation was taken of is kept in bf16 (swiglu: in two bf16, 16 bits of each value). A device wait that gave up is
-    reported by ``ops.gemm.check()``."""
+    reported by ``ops.gemm.check()`` and ``Communicator.check()``."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"linear: activation must be one of {', '.join(map(repr, _ACTIVATIONS))}, got {activation!r}")
     return runtime.ext().linear(x, weight, bias, residual, _ACTIVATIONS[activation], CONFIG.timeout_s)

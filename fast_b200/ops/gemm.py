@@ -40,11 +40,24 @@ def _st():
     return _status
 
 
+def _blocks() -> list:
+    """Where the waits of this module's GEMMs and of ``fused.linear`` on the current device report."""
+    return ([] if _status is None else [_status]) + [runtime.ext().dense_status()]
+
+
 def check() -> None:
-    """Raise if a GEMM launched through this module, or a ``fused.linear`` on the current device, gave up on an mbarrier wait."""
-    for code, site, detail, seen, want in (_st().read(), runtime.ext().take_dense_status()):
+    """Raise if a GEMM launched through this module, or a ``fused.linear`` on the current device, gave up on an mbarrier wait. The report stays, for
+    everybody else who asks (``Communicator.check()`` does), until ``reset()``."""
+    for block in _blocks():
+        code, site, detail, seen, want = block.read()
         if code:
             raise runtime.CollectiveTimeout(code, site, detail, seen, want)
+
+
+def reset() -> None:
+    """Forget what ``check()`` reports."""
+    for block in _blocks():
+        block.clear()
 
 
 def _tmap(t: torch.Tensor, box_rows: int):

@@ -352,21 +352,30 @@ class Communicator:
 
     # ---- health -------------------------------------------------------------------------------------
     def check(self) -> None:
-        """Synchronise the stream and raise ``CollectiveTimeout`` if a device wait gave up."""
-        code, site, detail, seen, want = self.status.read()
-        if code != 0:
-            self.broken = True
-            raise runtime.CollectiveTimeout(code, site, detail, seen, want)
+        """Synchronise the stream and raise ``CollectiveTimeout`` if a device wait gave up: in a collective of this communicator, or in a GEMM or a
+        linear layer on its device, whose results a layer on this communicator may hold (``ops.gemm.check``)."""
+        from ..ops import gemm
+
+        with torch.cuda.device(self.device):
+            code, site, detail, seen, want = self.status.read()
+            if code != 0:
+                self.broken = True
+                raise runtime.CollectiveTimeout(code, site, detail, seen, want)
+            gemm.check()   # no collective: the communicator stays usable
 
     def reset(self) -> None:
-        """After a failed collective: clear status and signal words (collective over the group)."""
+        """After a failed collective: clear status (that of GEMMs and linear layers on the device too) and signal words (collective over the group)."""
         import torch.distributed as dist
+
+        from ..ops import gemm
 
         torch.cuda.synchronize(self.device)
         if self.group is not None or (dist.is_initialized() and self.world > 1):
             dist.barrier(group=self.group)
         self.heap.tensor(self.sig_off, [self._C.SIG_WORDS], torch.int64).zero_()
         self.status.clear()
+        with torch.cuda.device(self.device):
+            gemm.reset()
         self.epoch = 0
         torch.cuda.synchronize(self.device)
         if self.group is not None or (dist.is_initialized() and self.world > 1):
