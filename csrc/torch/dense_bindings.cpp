@@ -1,6 +1,7 @@
 // Bindings of the dense side of a block: row norm, balance loss, linear layers. Their kernels run on the current stream of the
 // tensors' own device, whichever device is current.
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -23,6 +24,13 @@ using torch::autograd::variable_list;
 bool wants_grad(const torch::Tensor& t) { return t.requires_grad(); }
 bool wants_grad(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
 template <class... T> bool recorded(const T&... t) { return c10::GradMode::is_enabled() && (wants_grad(t) || ...); }
+
+// No operator here has a forward-mode derivative: an input's tangent would be lost without a word.
+void no_tangent(const char* op, const torch::Tensor& t) {
+  TORCH_CHECK(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), op, ": there is no forward-mode derivative, and an input has a tangent");
+}
+void no_tangent(const char* op, const OptTensor& t) { if (t.has_value()) no_tangent(op, *t); }
+template <class... T> void no_tangents(const char* op, const T&... t) { (no_tangent(op, t), ...); }
 
 // Gradients that came from kernels have no graph behind them: one that is asked for a gradient of its own says so.
 variable_list once(const char* op, const variable_list& incoming, variable_list grads) {
@@ -126,6 +134,8 @@ std::tuple<torch::Tensor, torch::Tensor> row_norm_bwd(const torch::Tensor& h, co
 }
 
 torch::Tensor dequantise_rows(const torch::Tensor& q, const torch::Tensor& scales) {
+  no_tangents("dequantise_rows", scales);
+  TORCH_CHECK(!recorded(scales), "dequantise_rows: there is no gradient of the scales, and they require one");
   TORCH_CHECK(q.is_cuda() && q.scalar_type() == torch::kUInt8 && q.dim() >= 1 && q.is_contiguous() && q.size(-1) % 128 == 0 && q.size(-1) > 0 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 8 == 0,
               "dequantise_rows: q must be contiguous e4m3 bytes [..., hidden], hidden a multiple of 128");
   TORCH_CHECK(scales.device() == q.device() && scales.scalar_type() == torch::kFloat32 && scales.is_contiguous() && scales.dim() == q.dim() && scales.numel() * 128 == q.numel() &&
@@ -170,6 +180,7 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
 };
 // (y, h, q, scales); h is x without a residual, q and scales are there with quantise.
 std::tuple<torch::Tensor, torch::Tensor, OptTensor, OptTensor> add_rms_norm(const torch::Tensor& x, const torch::Tensor& weight, double eps, const OptTensor& residual, bool quantise) {
+  no_tangents("add_rms_norm", x, weight, residual);
   const auto some = [](const torch::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
   if (!recorded(x, weight, residual)) {
     Norm n = row_norm(x, weight, eps, residual, quantise, false);
@@ -246,6 +257,7 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
   }
 };
 std::tuple<torch::Tensor, torch::Tensor> balance_loss(const torch::Tensor& logits, const torch::Tensor& topk_idx, const OptTensor& mask, bool sigmoid) {
+  no_tangents("balance_loss", logits);
   if (!recorded(logits)) {
     Balance b = balance(logits, topk_idx, mask, sigmoid);
     return {b.loss, b.counts};
@@ -488,6 +500,7 @@ struct Linear : torch::autograd::Function<Linear> {
   }
 };
 torch::Tensor linear(const torch::Tensor& x, const torch::Tensor& weight, const OptTensor& bias, const OptTensor& residual, int kind, double timeout_s) {
+  no_tangents("linear", x, weight, bias, residual);
   TORCH_CHECK(kind >= 0 && kind <= 4 && timeout_s > 0, "linear: activation or limit");
   const int64_t timeout_ns = static_cast<int64_t>(timeout_s * 1e9);
   if (!recorded(x, weight, bias, residual)) return linear_forward(x, weight, bias, static_cast<LinearKind>(kind), residual, false, timeout_ns).y;

@@ -1,6 +1,6 @@
 """Small fused autograd ops around the MoE block: embedding with a segmented-sum backward, the
 mean-square loss of a residual sum computed without materialising fp32 copies, and the dense side of a block (residual
-sum and RMS norm of rows, the router's balance loss, linear layers)."""
+sum and RMS norm of rows, the router's balance loss, linear layers), whose derivatives are reverse mode, once: inputs with a forward-mode tangent are refused."""
 from __future__ import annotations
 
 from typing import NamedTuple, Optional, Tuple
@@ -78,7 +78,8 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, resid
 
 
 def dequantise_rows(q: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
-    """bf16 rows of e4m3 bytes (uint8 [..., hidden]) and fp32 scales [..., hidden / 128], as ``add_rms_norm`` makes them."""
+    """bf16 rows of e4m3 bytes (uint8 [..., hidden]) and fp32 scales [..., hidden / 128], as ``add_rms_norm`` makes them. Has no gradient: scales
+    that require one are refused."""
     return runtime.ext().dequantise_rows(q, scales)
 
 
