@@ -25,6 +25,29 @@ bool wants_grad(const torch::Tensor& t) { return t.requires_grad(); }
 bool wants_grad(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
 template <class... T> bool recorded(const T&... t) { return c10::GradMode::is_enabled() && (wants_grad(t) || ...); }
 
+// The kernels read tensors through their pointers. A fake or wrapped tensor has none (its address reads as null, which would fault on the device); a zero
+// tensor, as some backward passes hand on, has none either; a negated view's memory holds the other sign.
+constexpr c10::DispatchKeySet kNotItsMemory({c10::DispatchKey::Python, c10::DispatchKey::ZeroTensor, c10::DispatchKey::Negative, c10::DispatchKey::Conjugate});
+bool is_its_memory(const torch::Tensor& t) { return t.defined() && t.layout() == torch::kStrided && t.has_storage() && !t.key_set().has_any(kNotItsMemory); }
+void want_memory(const char* op, const torch::Tensor& t) {
+  TORCH_CHECK(is_its_memory(t), op, ": every tensor must be one of plain memory (no fake, wrapped, sparse, zero or negated tensor)");
+}
+void want_memory(const char* op, const OptTensor& t) { if (t.has_value()) want_memory(op, *t); }
+template <class... T> void all_in_memory(const char* op, const T&... t) { (want_memory(op, t), ...); }
+// An incoming gradient, made real where it is a zero tensor or a negated view.
+torch::Tensor real(const char* op, const torch::Tensor& grad) {
+  if (is_its_memory(grad)) return grad;
+  const torch::Tensor g = grad._is_zerotensor() ? at::zeros(grad.sizes(), grad.options()) : grad.resolve_neg();
+  want_memory(op, g);
+  return g;
+}
+
+// What a backward pass kept, as it was: hooks of saved tensors may have brought it back otherwise. last: its last size, or -1 for any; made: by the forward pass itself, contiguous.
+void want_kept(const char* op, const torch::Tensor& t, const torch::Tensor& grad, c10::ScalarType type, int64_t numel, int64_t last, bool made) {
+  TORCH_CHECK(is_its_memory(t) && t.device() == grad.device() && t.scalar_type() == type && t.numel() == numel && (last < 0 || (t.dim() >= 1 && t.size(-1) == last)) && (!made || t.is_contiguous()),
+              op, ": a saved tensor came back on another device, of another type, size or layout");
+}
+
 // No operator here has a forward-mode derivative: an input's tangent would be lost without a word.
 void no_tangent(const char* op, const torch::Tensor& t) {
   TORCH_CHECK(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), op, ": there is no forward-mode derivative, and an input has a tangent");
@@ -115,6 +138,9 @@ std::tuple<torch::Tensor, torch::Tensor> row_norm_bwd(const torch::Tensor& h, co
   TORCH_CHECK(h.is_cuda() && row_type(h) && row_type(weight) && dy.sizes() == h.sizes() && dy.scalar_type() == h.scalar_type() && dy.device() == h.device(), "add_rms_norm backward: gradient of y");
   TORCH_CHECK(!dh.has_value() || (dh->sizes() == h.sizes() && dh->scalar_type() == h.scalar_type() && dh->device() == h.device()), "add_rms_norm backward: gradient of the sum");
   const int64_t H = h.size(-1);
+  want_kept("add_rms_norm backward", h, dy, h.scalar_type(), dy.numel(), H, false);
+  want_kept("add_rms_norm backward", weight, dy, weight.scalar_type(), H, H, true);
+  want_kept("add_rms_norm backward", rstd, dy, torch::kFloat32, dy.numel() / H, dy.numel() / H, true);
   c10::cuda::CUDAGuard guard(h.device());
   const torch::Tensor hm = as_rows(h, H), ym = dy.contiguous(), dm = dh.has_value() ? dh->contiguous() : torch::Tensor();
   RowNormBwdArgs a{};
@@ -134,6 +160,7 @@ std::tuple<torch::Tensor, torch::Tensor> row_norm_bwd(const torch::Tensor& h, co
 }
 
 torch::Tensor dequantise_rows(const torch::Tensor& q, const torch::Tensor& scales) {
+  all_in_memory("dequantise_rows", q, scales);
   no_tangents("dequantise_rows", scales);
   TORCH_CHECK(!recorded(scales), "dequantise_rows: there is no gradient of the scales, and they require one");
   TORCH_CHECK(q.is_cuda() && q.scalar_type() == torch::kUInt8 && q.dim() >= 1 && q.is_contiguous() && q.size(-1) % 128 == 0 && q.size(-1) > 0 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 8 == 0,
@@ -161,12 +188,12 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const bool residual = ctx->saved_data["residual"].toBool();
-    const torch::Tensor dh = residual ? grads[1] : torch::Tensor();
-    torch::Tensor dx, dw;
+    torch::Tensor dx, dw, dh;
     {
       torch::NoGradGuard no_grad;
+      if (residual && grads[1].defined()) dh = real("add_rms_norm backward", grads[1]);
       if (grads[0].defined()) {
-        std::tie(dx, dw) = row_norm_bwd(saved[0], saved[1], saved[2], grads[0], dh.defined() ? OptTensor(dh) : OptTensor());
+        std::tie(dx, dw) = row_norm_bwd(saved[0], saved[1], saved[2], real("add_rms_norm backward", grads[0]), dh.defined() ? OptTensor(dh) : OptTensor());
       } else {   // only the sum was used
         dx = dh;
         if (ctx->needs_input_grad(1)) dw = torch::zeros_like(saved[1]);
@@ -180,6 +207,7 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
 };
 // (y, h, q, scales); h is x without a residual, q and scales are there with quantise.
 std::tuple<torch::Tensor, torch::Tensor, OptTensor, OptTensor> add_rms_norm(const torch::Tensor& x, const torch::Tensor& weight, double eps, const OptTensor& residual, bool quantise) {
+  all_in_memory("add_rms_norm", x, weight, residual);
   no_tangents("add_rms_norm", x, weight, residual);
   const auto some = [](const torch::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
   if (!recorded(x, weight, residual)) {
@@ -228,7 +256,7 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
   static variable_list forward(AutogradContext* ctx, const torch::Tensor& logits, const torch::Tensor& topk_idx, const OptTensor& mask, bool sigmoid) {
     Balance b = balance(logits, topk_idx, mask, sigmoid);
     ctx->set_materialize_grads(false);
-    ctx->saved_data["kept"] = std::vector<int64_t>{topk_idx.size(-1), sigmoid};
+    ctx->saved_data["kept"] = std::vector<int64_t>{topk_idx.size(-1), sigmoid, logits.size(-1), static_cast<int64_t>(logits.scalar_type()), logits.numel() / logits.size(-1)};
     ctx->save_for_backward({logits, mask_bytes(mask), b.kept});
     ctx->mark_non_differentiable({b.counts});
     return {b.loss, b.counts};
@@ -238,11 +266,15 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
     const auto saved = ctx->get_saved_variables();
     const std::vector<int64_t> kept = ctx->saved_data["kept"].toIntVector();
     const torch::Tensor& logits = saved[0];
+    const int64_t E = kept[2];
+    want_kept("balance_loss backward", logits, grads[0], static_cast<c10::ScalarType>(kept[3]), kept[4] * E, E, false);
+    if (saved[1].defined()) want_kept("balance_loss backward", saved[1], grads[0], torch::kBool, kept[4], -1, true);
+    want_kept("balance_loss backward", saved[2], grads[0], torch::kInt32, E + 1, E + 1, true);
     torch::Tensor dlogits;
     {
       torch::NoGradGuard no_grad;
       c10::cuda::CUDAGuard guard(logits.device());
-      const torch::Tensor lm = as_rows(logits, logits.size(-1)), dloss = grads[0].to(torch::kFloat32);
+      const torch::Tensor lm = as_rows(logits, logits.size(-1)), dloss = real("balance_loss backward", grads[0]).to(torch::kFloat32);
       dlogits = fresh(logits.sizes(), logits);
       BalanceBwdArgs a{};
       a.logits = lm.data_ptr(); a.stride = lm.stride(0); a.logits_bf16 = logits.scalar_type() == torch::kBFloat16;
@@ -257,6 +289,7 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
   }
 };
 std::tuple<torch::Tensor, torch::Tensor> balance_loss(const torch::Tensor& logits, const torch::Tensor& topk_idx, const OptTensor& mask, bool sigmoid) {
+  all_in_memory("balance_loss", logits, topk_idx, mask);
   no_tangents("balance_loss", logits);
   if (!recorded(logits)) {
     Balance b = balance(logits, topk_idx, mask, sigmoid);
@@ -456,8 +489,11 @@ struct Linear : torch::autograd::Function<Linear> {
     if (want_x || want_w || want_b) {
       torch::NoGradGuard no_grad;
       c10::cuda::CUDAGuard guard(grads[0].device());
-      const torch::Tensor dy = tma_rows(grads[0], kind == LinearKind::kSwiGLU ? N / 2 : N);
-      const int64_t T = dy.size(0);
+      const torch::Tensor dy = tma_rows(real("linear backward", grads[0]), kind == LinearKind::kSwiGLU ? N / 2 : N);
+      const int64_t T = dy.size(0), kept_width = kind == LinearKind::kSwiGLU ? 2 * N : N;
+      if (want_w) want_kept("linear backward", saved[0], dy, torch::kBFloat16, T * K, K, false);
+      if (want_x) want_kept("linear backward", saved[1], dy, torch::kBFloat16, N * K, K, false);
+      if (kind != LinearKind::kNone) want_kept("linear backward", saved[2], dy, torch::kBFloat16, T * kept_width, kept_width, true);
       TORCH_CHECK(dy.scalar_type() == torch::kBFloat16, "linear backward: the gradient must be bf16");
       if (T == 0) {
         if (want_x) out[0] = torch::zeros(shape, dy.options());
@@ -500,6 +536,7 @@ struct Linear : torch::autograd::Function<Linear> {
   }
 };
 torch::Tensor linear(const torch::Tensor& x, const torch::Tensor& weight, const OptTensor& bias, const OptTensor& residual, int kind, double timeout_s) {
+  all_in_memory("linear", x, weight, bias, residual);
   no_tangents("linear", x, weight, bias, residual);
   TORCH_CHECK(kind >= 0 && kind <= 4 && timeout_s > 0, "linear: activation or limit");
   const int64_t timeout_ns = static_cast<int64_t>(timeout_s * 1e9);
