@@ -25,6 +25,25 @@ __device__ __forceinline__ void epi_bar() { asm volatile("bar.sync 1, 128;" ::: 
 // Named barriers 1 and 2: the four warps of one of two epilogue groups.
 __device__ __forceinline__ void group_bar(int group) { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); }
 
+// The same barrier as a vote: whether all 128 threads say yes. Warps that meet at the group's barrier again go on or give up together: one that has left would be waited for
+// without a limit. Called by whole warps.
+__device__ __forceinline__ bool group_all(int group, bool yes) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred P, Q;\n\t"
+      "setp.ne.b32 P, %2, 0;\n\t"
+      "barrier.cta.red.and.pred Q, %1, 128, P;\n\t"
+      "selp.b32 %0, 1, 0, Q;\n\t}"
+      : "=r"(all)
+      : "r"(1 + group), "r"(yes ? 1u : 0u)
+      : "memory");
+  return all != 0;
+}
+// A wait of a group's four warps, given up together.
+__device__ __forceinline__ bool mbar_wait_group(int group, uint64_t* bar, uint32_t parity, volatile int* abort_flag, DeviceStatus* st, unsigned long long detail, unsigned long long timeout_ns) {
+  return group_all(group, ptx::mbar_wait_warp(bar, parity, abort_flag, st, detail, timeout_ns));
+}
+
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* smem_src, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
                ::"l"(reinterpret_cast<uint64_t>(map)), "r"(ptx::smem_u32(smem_src)), "r"(x), "r"(y)

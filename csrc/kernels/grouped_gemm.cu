@@ -160,7 +160,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
       const bool empty_reduction = tc.red_blocks == 0;  // wgrad of an expert that got no tokens
       if (!empty_reduction) {
         ++acc_it;
-        if (!(ok = mbar_wait_bounded(&ctl->acc_full[a], aph, abort_flag, p.status, 400 + a, p.timeout_ns))) break;
+        if (!(ok = mbar_wait_warp(&ctl->acc_full[a], aph, abort_flag, p.status, 400 + a, p.timeout_ns))) break;
         tc_fence_after_sync();
       }
       const int row_in_tile = quarter * 32 + lane;

@@ -314,7 +314,7 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
           const float sc = m0 + row < real_rows ? __ldg(srow + static_cast<long long>(8 * i) * sgroups + (kb >> 1)) : 0.0f;
           s2[i] = bf16_pair_of(sc * 1.152921504606846976e18f);  // (scale x 2^60) twice
         }
-        if (!(ok = mbar_wait_bounded(&ctl->q_full[cw], (it / kQStages) & 1, abort_flag, p.status, 700 + cw, p.timeout_ns))) break;
+        if (!(ok = mbar_wait_warp(&ctl->q_full[cw], (it / kQStages) & 1, abort_flag, p.status, 700 + cw, p.timeout_ns))) break;
         const uint8_t* qb = q_ring + cw * kQBytes;
         uint8_t* sa = tiles + s * STAGE;
         // No conversion instruction is used. An e4m3 byte (sign s, magnitude g = eeeemmm) read as the bf16 bit
@@ -364,7 +364,7 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
       const bool empty_reduction = tc.red_blocks == 0;
       uint32_t keep[kChunks][kEpiChunkCols / 2];     // bf16 pairs: tensor memory is free again before anything is stored
       if (!empty_reduction) {
-        if (!(ok = mbar_wait_bounded(&ctl->acc_full[a], done & 1, abort_flag, p.status, 400 + a, p.timeout_ns))) break;
+        if (!(ok = mbar_wait_warp(&ctl->acc_full[a], done & 1, abort_flag, p.status, 400 + a, p.timeout_ns))) break;
         ++done;
         tc_fence_after_sync();
       }
@@ -418,7 +418,7 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
       const bool empty_reduction = tc.red_blocks == 0;
       if (!empty_reduction) {
         ++acc_it;
-        if (!(ok = mbar_wait_bounded(&ctl->acc_full[a], aph, abort_flag, p.status, 400 + a, p.timeout_ns))) break;
+        if (!(ok = mbar_wait_group(0, &ctl->acc_full[a], aph, abort_flag, p.status, 400 + a, p.timeout_ns))) break;
         tc_fence_after_sync();
       }
       // first output row of this CTA's half (TMA store coordinate)

@@ -370,13 +370,18 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
       for (int i = et; i < p.num_counters; i += 128) p.counters_next[i] = 0u;
     uint32_t acc_it = 0, ring_n = 0, load_ph = 0u;   // load_ph: one parity bit per half of the ring
     bool ok = true;
+    // kLinear's warps meet nowhere but below, with a limit: each gives up by itself. The others' groups have barriers of their own: a group gives up as one.
+    auto wait_epi = [&](uint64_t* bar, uint32_t parity, unsigned long long detail) {
+      if constexpr (EPI == GemmEpilogue::kLinear) return mbar_wait_warp(bar, parity, abort_flag, p.status, detail, p.timeout_ns);
+      else return mbar_wait_group(group, bar, parity, abort_flag, p.status, detail, p.timeout_ns);
+    };
     // All epilogue warps, twice per part of a tile (phases 0 and 1 of the barrier). Two groups wait with a limit: one of them may have given up.
     auto meet = [&](uint32_t phase) {
       if (GROUPS == 1) { epi_bar(); return; }
       __syncwarp();
       if (!ok) return;
       if (lane == 0) mbar_arrive(&ctl->meet);
-      ok = mbar_wait_bounded(&ctl->meet, phase, abort_flag, p.status, 600 + phase, p.timeout_ns);
+      ok = wait_epi(&ctl->meet, phase, 600 + phase);
     };
     while (ok && segs.next(sg)) {
       const TokTile tc = walk.locate(sg.tile);
@@ -387,7 +392,7 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
       auto acc_row = [&](int sub) { return tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + (it0 + sub) % kAccStages * kTokAccN; };
       auto wait_acc = [&](int sub) {
         const int a = (it0 + sub) % kAccStages;
-        ok = mbar_wait_bounded(&ctl->acc_full[a], ((it0 + sub) / kAccStages) & 1, abort_flag, p.status, 400 + a, p.timeout_ns);
+        ok = wait_epi(&ctl->acc_full[a], ((it0 + sub) / kAccStages) & 1, 400 + a);
         tc_fence_after_sync();
       };
       auto release_acc = [&](int sub) {
@@ -506,7 +511,8 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
           return;
         }
         uint8_t* b = ring + (st & 1) * kRing;
-        if (!(ok = mbar_wait_bounded(&ctl->epi_load[st & 1], (load_ph >> (st & 1)) & 1u, abort_flag, p.status, 500, p.timeout_ns))) return;
+        // The group's vote is the barrier in front of the stores: a warp that gave up works on what the box holds until then.
+        const bool here = mbar_wait_warp(&ctl->epi_load[st & 1], (load_ph >> (st & 1)) & 1u, abort_flag, p.status, 500, p.timeout_ns);
         load_ph ^= 1u << (st & 1);
         const uint32_t gb = smem_u32(b + (quarter >> 1) * kBox), ub = gb + 2 * kBox;
         uint32_t gv[4][4], uv[4][4];
@@ -542,7 +548,7 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
           stmatrix_trans(box_row(ub, lane, e & 1, chunk), uv[e][0], uv[e][1], uv[e][2], uv[e][3]);
         }
         fence_proxy_async_smem();
-        group_bar(group);
+        if (!(ok = group_all(group, here))) return;
         if (issuer) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) tma_store_2d(&map_c, b + q * kBox, 2 * feat0 + q * 64, y);
@@ -626,7 +632,7 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
             for (int e = 0; e < 4; ++e) stmatrix_trans(warp_box_row(box, lane, e & 1, (e >> 1) * 2), h[4 * e], h[4 * e + 1], h[4 * e + 2], h[4 * e + 3]);
           };
           if (residual) {
-            if (!(ok = mbar_wait_bounded(&ctl->epi_load[2 * me + (ring_n & 1u)], (load_ph >> (ring_n & 1u)) & 1u, abort_flag, p.status, 500, p.timeout_ns))) break;
+            if (!(ok = wait_epi(&ctl->epi_load[2 * me + (ring_n & 1u)], (load_ph >> (ring_n & 1u)) & 1u, 500))) break;
             load_ph ^= 1u << (ring_n & 1u);
           } else {
             if (lane == 0) bulk_wait_read<1>();   // the store that reads this slot is done with it

@@ -138,8 +138,7 @@ __global__ void __launch_bounds__(kThreads) linear_few_kernel(const __grid_const
     }
   }
   __syncwarp();
-  // a warp reads tensor memory as one, so it gives up as one
-  const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctl->done, 0, abort_flag, p.status, 400, p.timeout_ns));
+  const bool ok = mbar_wait_warp(&ctl->done, 0, abort_flag, p.status, 400, p.timeout_ns);
   tc_fence_after_sync();
   // Four features of a token (SwiGLU: their gates and ups) on their way out.
   const auto finish = [&](int token, int f, float4 v, const float4& up) {

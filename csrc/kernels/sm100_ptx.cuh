@@ -66,6 +66,12 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   return true;
 }
 
+// The same for all lanes of a warp together. A lane alone would decide for itself, on either side of the moment when the barrier completes or a sibling gives up, and the
+// warp-wide instructions behind the wait (tensor memory and matrix loads, warp barriers) would wait for lanes that have left.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, DeviceStatus* st, unsigned long long detail, unsigned long long timeout_ns) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, st, detail, timeout_ns));
+}
+
 // ---- TMA (tile mode, 2D, no multicast) ----------------------------------------------------------------
 __device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile(
