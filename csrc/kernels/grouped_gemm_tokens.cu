@@ -296,6 +296,7 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
       int s = 0;
       uint32_t ph = 0, acc_it = 0;
       bool ok = true;
+      grid_dependency_wait();   // nothing can arrive before: its limit does not count the time of the kernel in front
       while (ok && segs.next(sg)) {
         const TokTile tc = walk.locate(sg.tile);
         const bool both = SUB == 2 && tc.n > kTokAccN;

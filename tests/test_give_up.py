@@ -90,3 +90,30 @@ def test_launches_that_give_up_leave_the_next_as_if_they_had_not_been(counts, N,
         run(target, 5.0)
         gemm.check()
         assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,K,N", [(300, 512, 20000), (40, 512, 4096)])
+def test_a_limit_does_not_count_the_kernel_in_front(T, K, N):
+    """A linear layer that is set up while a longer kernel in front of it still runs (on a few SMs, waiting for a row that never comes) has its own limit from then on."""
+    from fast_b200 import runtime
+    from fast_b200.ops import fused, gemm
+
+    if not gemm.USE_PAIR:
+        pytest.skip("belongs to the CTA-pair kernels")
+    C = runtime.ext()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, w = (torch.randint(-2, 3, s, generator=g, device="cuda").to(torch.bfloat16) for s in ((T, K), (N, K)))
+    want = fused.linear(x, w)
+    rows, inner = 256, 512
+    a, e = torch.zeros(rows, inner, device="cuda", dtype=torch.bfloat16), torch.zeros(1, 512, inner, device="cuda", dtype=torch.bfloat16)
+    off, live = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([0, rows], [200]))
+    target, counter = torch.tensor([200], device="cuda"), torch.tensor([199], device="cuda")
+    out = torch.zeros(rows, 512, device="cuda", dtype=torch.bfloat16)
+    for _ in range(3):
+        gemm.grouped_gemm_fwd(a, e, off, out, live_rows=live, granule=32, gate=(counter.data_ptr(), target), timeout_s=0.06, ctas=4)
+        got = C.linear(x, w, None, None, 0, 0.01)
+        with pytest.raises(runtime.CollectiveTimeout):
+            gemm.check()
+        assert C.dense_status().read()[0] == 0 and torch.equal(got, want)
+        gemm.reset()
