@@ -33,9 +33,10 @@ constexpr int kThreads = 192;
 constexpr int kEpiWarps = 4;
 
 struct __align__(8) SmemCtl {
-  uint64_t full[kStages], empty[kStages], acc_full[kAccStages], acc_empty[kAccStages];
+  uint64_t full[kStages], empty[kStages], acc_full[kAccStages], acc_empty[kAccStages], products;
   uint32_t tmem_base;
-  int abort_flag;
+  int abort_flag, issued;   // blocks whose loads were requested, where the launch gave up
+  uint32_t accs;            // accumulators that were filled
 };
 constexpr int kSmemBytes = kStages * kStageBytes + 1024 /*alignment slack*/ + sizeof(SmemCtl);
 static_assert(kSmemBytes <= 227 * 1024, "dynamic shared memory of one CTA on sm_100a");
@@ -58,7 +59,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) { mbar_init(&ctl->full[s], 1); mbar_init(&ctl->empty[s], 1); }
     for (int a = 0; a < kAccStages; ++a) { mbar_init(&ctl->acc_full[a], 1); mbar_init(&ctl->acc_empty[a], kEpiWarps); }
-    ctl->abort_flag = 0;
+    mbar_init(&ctl->products, 1);
+    ctl->abort_flag = ctl->issued = 0;
     mbar_fence_init();
     prefetch_tmap(&map_a);
     prefetch_tmap(&map_b);
@@ -115,6 +117,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
           }
         }
       }
+      ctl->issued = static_cast<int>(it);
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
@@ -148,6 +151,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         }
         if (ok) mma_commit(&ctl->acc_full[a]);
       }
+      ctl->accs = acc_it;
+      if (!ok) { mma_commit(&ctl->products); mbar_drain(&ctl->products, 0); }
     }
   } else {
     // ---------------- epilogue: TMEM -> registers -> bf16 -> global ----------------
@@ -183,6 +188,14 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
   // ---------------- teardown ----------------
   tc_fence_before_sync();
   __syncthreads();
+  // A launch that has given up also waits for its products (where their issuer had not given up, the last accumulator's barrier stands for all of them) and for its loads.
+  if (warp == 1) {
+    if (lane == 0 && *abort_flag) {
+      if (ctl->accs > 0) mbar_drain(&ctl->acc_full[(ctl->accs - 1) % kAccStages], ((ctl->accs - 1) / kAccStages) & 1);
+      drain_loads(ctl->full, ctl->issued, kStages);
+    }
+    __syncwarp();
+  }
   if (warp == 1) { tc_fence_after_sync(); tmem_dealloc(tmem_base, kTmemCols); }
 }
 

@@ -67,9 +67,10 @@ static_assert(kOtherRegs + 2 * kEpilogueRegs <= 3 * kLaunchRegs && kWideThreads 
 
 constexpr int kMaxSlices = 8;        // of the rows of one matrix (dense weight gradients)
 struct __align__(8) SmemCtl {
-  uint64_t full[kStages], empty[kStages], acc_full[kAccStages], acc_empty[kAccStages], q_full[kQStages], q_empty[kQStages];
+  uint64_t full[kStages], empty[kStages], acc_full[kAccStages], acc_empty[kAccStages], q_full[kQStages], q_empty[kQStages], products;
   uint32_t tmem_base;
-  int abort_flag;
+  int abort_flag, issued;          // blocks whose loads were requested, where the launch gave up
+  int last_acc, last_phase;        // the accumulator that was filled last, and how often before (-1: none)
   int dense_off[kMaxSlices + 1];   // the group table of a launch without one
 };
 constexpr int kSmemBytes = kStages * kStageBytes + kEpiBytes + 1024 + sizeof(SmemCtl);
@@ -124,7 +125,8 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     for (int s = 0; s < NS; ++s) { mbar_init(&ctl->full[s], A_FP8 ? 1 + 2 : 1); mbar_init(&ctl->empty[s], 1); }
     for (int a = 0; a < kAccStages; ++a) { mbar_init(&ctl->acc_full[a], 1); mbar_init(&ctl->acc_empty[a], 2 * kEpiWarps); }
     for (int q = 0; q < kQStages; ++q) { mbar_init(&ctl->q_full[q], 1); mbar_init(&ctl->q_empty[q], 1); }
-    ctl->abort_flag = 0;
+    mbar_init(&ctl->products, 1);
+    ctl->abort_flag = ctl->issued = 0;
     if (MODE == GemmMode::kWgrad && p.group_off == nullptr)   // rows past the real ones come in as zeros: they lie outside the matrices
       for (int g = 0; g <= p.num_groups; ++g) ctl->dense_off[g] = static_cast<int>(static_cast<long long>((p.dense_rows + BK - 1) / BK) * g / p.num_groups) * BK;
     mbar_fence_init();
@@ -197,6 +199,7 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
             tma_load_2d_pair(sb + j * (BK * 128), &map_b, n0 + j / 2 * BN + j % 2 * 64, tc.row0 + kb * BK, full_leader);
         }
       }
+      ctl->issued = static_cast<int>(it);
     }
   } else if (WIDE && warp == 1) {
     give_registers();
@@ -251,6 +254,8 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         mma_commit_pair(&ctl->acc_full[1], 0x3);
         ++done;
       }
+      ctl->last_acc = 1; ctl->last_phase = static_cast<int>(done) - 1;
+      if (!ok) { mma_commit_pair(&ctl->products, 0x1); mbar_drain(&ctl->products, 0); }
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer (leader CTA only) ----------------
@@ -282,6 +287,8 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         }
         if (ok) mma_commit_pair(&ctl->acc_full[a], 0x3);
       }
+      ctl->last_acc = static_cast<int>(acc_it - 1) & 1; ctl->last_phase = acc_it > 0 ? static_cast<int>((acc_it - 1) / kAccStages) : -1;
+      if (!ok) { mma_commit_pair(&ctl->products, 0x1); mbar_drain(&ctl->products, 0); }
     }
   } else if (A_FP8 && warp >= 2 + kEpiWarps) {
     // ---------------- e4m3 -> bf16 converters (both CTAs, each for its 128 rows of A) ----------------
@@ -445,6 +452,16 @@ grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
   // ---------------- teardown: nobody frees tensor memory while the pair still uses it ----------------
   tc_fence_before_sync();
   __syncthreads();
+  // A launch that has given up also waits for its products (where their issuer had not given up, the last accumulator's barrier stands for all of them) and for its loads: those
+  // of both CTAs on the leader's barriers, e4m3 blocks on the own ones. The follower may have requested blocks that the leader does not expect any more: it stays for as
+  // long as a copy could take.
+  if (threadIdx.x == 0 && *abort_flag) {
+    if (leader && ctl->last_phase >= 0) mbar_drain(&ctl->acc_full[ctl->last_acc], ctl->last_phase & 1);
+    if (A_FP8) drain_loads(ctl->q_full, ctl->issued, kQStages);
+    if (leader) drain_loads(ctl->full, ctl->issued, NS);
+    else mbar_drain(&ctl->products, 0);   // nothing arrives there: a pause
+  }
+  __syncwarp();
   cluster_sync_all();
   if (warp == 1) { tc_fence_after_sync(); tmem_dealloc_pair(tmem_base, kTmemCols); }
 }

@@ -69,8 +69,10 @@ constexpr int kStepTokens = 32;                   // tokens per epilogue step = 
 constexpr int kBox = kStepTokens * 128;           // 4 KiB: 32 tokens x 64 features
 
 struct __align__(8) TokCtl {
-  uint64_t full[kMaxStages], empty[kMaxStages], acc_full[kAccStages], acc_empty[kAccStages], epi_load[16], meet;
+  uint64_t full[kMaxStages], empty[kMaxStages], acc_full[kAccStages], acc_empty[kAccStages], epi_load[16], meet, products;
   uint32_t tmem_base;
+  int next_stage, next_phase;                       // of the loads, when the producer left
+  uint32_t accs;                                    // accumulators that were filled
   int abort_flag, last_arrived, widest, share_weights;
   int base[kTokPrefix + 1];                         // tiles of the groups before entry i
 };
@@ -164,6 +166,7 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
     for (int a = 0; a < kAccStages; ++a) { mbar_init(&ctl->acc_full[a], 1); mbar_init(&ctl->acc_empty[a], 2 * 4 * GROUPS); }
     for (int q = 0; q < 16; ++q) mbar_init(&ctl->epi_load[q], 1);
     mbar_init(&ctl->meet, 4 * GROUPS);
+    mbar_init(&ctl->products, 1);
     ctl->abort_flag = 0;
     mbar_fence_init();
     prefetch_tmap(&map_w);
@@ -266,7 +269,7 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
             asm volatile("fence.proxy.async.global;" ::: "memory");
             gated = slot;
           }
-          if (!ok) break;
+          if (!ok) { s += early; break; }
         }
         for (int i = 0; i < blocks; ++i, k += k_step) {
           if (i >= early) {
@@ -288,6 +291,7 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
           if (++s == stages) { s = 0; ph ^= 1; }
         }
       }
+      ctl->next_stage = s; ctl->next_phase = static_cast<int>(ph);
     }
   } else if (warp == 1) {
     give_registers();
@@ -352,6 +356,8 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
         if (!ok) break;
         if (both) mma_commit_pair(&ctl->acc_full[(it0 + 1) % kAccStages], 0x3);
       }
+      ctl->accs = acc_it;
+      if (!ok) { mma_commit_pair(&ctl->products, 0x1); mbar_drain(&ctl->products, 0); }
     }
   } else if (warp < first_epilogue_warp(SUB)) {
     give_registers();
@@ -619,8 +625,9 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
           bias[i] = p.bias != nullptr && f < p.features ? __bfloat162float(p.bias[f]) : 0.0f;
         }
         if (sg.parts == 1) wait_acc(0);
+        int st = first_step;
 #pragma unroll 1
-        for (int st = first_step; ok && st < steps_of(0); st += GROUPS) {
+        for (; ok && st < steps_of(0); st += GROUPS) {
           uint32_t r[32], h[16];
           load_acc(0, st, r);
           if (p.bias != nullptr) {
@@ -679,7 +686,12 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
           }
           ++ring_n;
         }
-        if (!ok) break;
+        if (!ok) {
+          if (residual && lane == 0)
+            for (int i = 0; i < 2; ++i)
+              if (st + i * GROUPS < steps_of(0)) mbar_drain(&ctl->epi_load[2 * me + ((ring_n + i) & 1u)], (load_ph >> ((ring_n + i) & 1u)) & 1u);
+          break;
+        }
         if (sg.parts == 1) release_acc(0);
       } else if constexpr (SUB == 1) {
         if (EPI == GemmEpilogue::kSwiGLUBwd) begin_gu(0);       // the saved tiles arrive while the MMAs still run
@@ -790,6 +802,15 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
   // ---------------- teardown: nobody frees tensor memory while the pair still uses it ----------------
   tc_fence_before_sync();
   __syncthreads();
+  // A launch that has given up also waits for its products (where their issuer had not given up, the last accumulator's barrier stands for all of them) and for the loads of
+  // both CTAs, which the leader's barriers count. The follower may have requested blocks that the leader does not expect any more: it stays for as long as a copy could take.
+  // (Stages up to the next one were last filled in this phase of their barriers, the others in the one before; those never filled are in that one.)
+  if (leader && threadIdx.x == 0 && *abort_flag) {
+    if (ctl->accs > 0) mbar_drain(&ctl->acc_full[(ctl->accs - 1) % kAccStages], ((ctl->accs - 1) / kAccStages) & 1);
+    for (int i = 0; i < stages; ++i) mbar_drain(&ctl->full[i], ctl->next_phase ^ (i >= ctl->next_stage ? 1 : 0));
+  }
+  if (!leader && threadIdx.x == 0 && *abort_flag) mbar_drain(&ctl->products, 0);   // nothing arrives there: a pause
+  __syncwarp();
   cluster_sync_all();
   if (warp == 1) { tc_fence_after_sync(); tmem_dealloc_pair(tmem_base, kTmemCols); }
 }

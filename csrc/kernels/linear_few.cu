@@ -29,9 +29,9 @@ constexpr int kFewSmem = 110 * 1024, kFewDeepSmem = 220 * 1024;   // of an SM's 
 __host__ __device__ constexpr int few_stage(int n) { return kFewABytes + n * BK * 2; }
 
 struct __align__(8) FewCtl {
-  uint64_t full[kMaxStages], empty[kMaxStages], done;
+  uint64_t full[kMaxStages], empty[kMaxStages], done, products;
   uint32_t tmem_base;
-  int abort_flag;
+  int abort_flag, issued;   // blocks whose loads were requested, where the launch gave up
 };
 // The fp32 sums: where the stages were, or, where they are few and of several CTAs, beside them: a peer's may come while this CTA still multiplies.
 __host__ __device__ constexpr int few_sums(int n) { return n * kRows * 4; }
@@ -81,7 +81,8 @@ __global__ void __launch_bounds__(kThreads) linear_few_kernel(const __grid_const
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) { mbar_init(&ctl->full[s], 1); mbar_init(&ctl->empty[s], 1); }
     mbar_init(&ctl->done, 1);
-    ctl->abort_flag = 0;
+    mbar_init(&ctl->products, 1);
+    ctl->abort_flag = ctl->issued = 0;
     mbar_fence_init();
     prefetch_tmap(&map_w);
     prefetch_tmap(&map_x);
@@ -100,7 +101,8 @@ __global__ void __launch_bounds__(kThreads) linear_few_kernel(const __grid_const
   if (warp == 0) {
     if (elect_one()) {
       uint32_t ph = 0;
-      for (int i = 0, s = 0; i < blocks; ++i) {
+      int i = 0;
+      for (int s = 0; i < blocks; ++i) {
         if (i >= stages && !mbar_wait_bounded(&ctl->empty[s], ph ^ 1, abort_flag, p.status, 100 + s, p.timeout_ns)) break;
         uint8_t* sa = tiles + s * stage_size;
         const int k = (kb0 + i) * BK;
@@ -118,6 +120,7 @@ __global__ void __launch_bounds__(kThreads) linear_few_kernel(const __grid_const
         tma_load_2d(sa + kFewABytes, &map_x, k, t0, &ctl->full[s]);
         if (++s == stages) { s = 0; ph ^= 1; }
       }
+      ctl->issued = i;
     }
   } else if (warp == 1) {
     if (elect_one()) {
@@ -134,7 +137,8 @@ __global__ void __launch_bounds__(kThreads) linear_few_kernel(const __grid_const
         mma_commit(&ctl->empty[s]);
         if (++s == stages) { s = 0; ph ^= 1; }
       }
-      if (ok) mma_commit(&ctl->done);
+      mma_commit(ok ? &ctl->done : &ctl->products);
+      if (!ok) mbar_drain(&ctl->products, 0);
     }
   }
   __syncwarp();
@@ -218,6 +222,11 @@ __global__ void __launch_bounds__(kThreads) linear_few_kernel(const __grid_const
     }
   }
   __syncwarp();
+  // Given up: not before the products and the loads that are still on their way.
+  if (*abort_flag && warp == 1) {
+    if (lane == 0) { mbar_drain(&ctl->done, 0); drain_loads(ctl->full, ctl->issued, stages); }
+    __syncwarp();
+  }
   if (warp == 1) tmem_dealloc(tmem, columns);
 }
 

@@ -72,6 +72,18 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, v
   return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, st, detail, timeout_ns));
 }
 
+// For what is still on its way when a kernel has given up: until the phase is over, or kDrainNs have passed. A block that left with copies into its shared memory or products under
+// way would hand that memory on under them. Reports nothing: the report has been made.
+constexpr unsigned long long kDrainNs = 2000000;   // a copy or a product takes microseconds
+__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
+  const unsigned long long t0 = global_timer_ns();
+  while (!mbar_try_wait(bar, parity) && global_timer_ns() - t0 < kDrainNs) {}
+}
+// The loads of the last `stages` blocks of a ring, of `issued` in all.
+__device__ __forceinline__ void drain_loads(uint64_t* full, int issued, int stages) {
+  for (int i = issued > stages ? issued - stages : 0; i < issued; ++i) mbar_drain(&full[i % stages], (i / stages) & 1);
+}
+
 // ---- TMA (tile mode, 2D, no multicast) ----------------------------------------------------------------
 __device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile(

@@ -117,3 +117,68 @@ def test_a_limit_does_not_count_the_kernel_in_front(T, K, N):
             gemm.check()
         assert C.dense_status().read()[0] == 0 and torch.equal(got, want)
         gemm.reset()
+
+
+def test_a_kernel_that_gives_up_waits_for_what_is_under_way():
+    """Every kernel with a TMA ring: its loads, its products and, with a residual that comes in by TMA, that."""
+    for f in ("grouped_gemm.cu", "grouped_gemm_pair.cu", "grouped_gemm_tokens.cu", "linear_few.cu"):
+        text = _source(f)
+        end = text[text.index("__syncwarp();\n  const bool ok = mbar_wait_warp") if f == "linear_few.cu" else text.rindex("tc_fence_before_sync();\n  __syncthreads();"):]
+        assert "*abort_flag" in end and ("drain_loads(ctl->full" in end or "mbar_drain(&ctl->full" in end), f
+        assert end.index("*abort_flag") < end.index("tmem_dealloc"), f
+        assert re.search(r"mma_commit(_pair)?\((ok \? &ctl->done : )?&ctl->products", text) and "mbar_drain(&ctl->products, 0)" in text, f
+    assert "mbar_drain(&ctl->epi_load" in _source("grouped_gemm_tokens.cu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,K,N,kw", [
+    (1, 1 << 24, 128, {}), (300, 1 << 22, 256, {"bias": True}),         # few tokens: one tile for a cluster of CTAs, and several
+    (2048, 1 << 20, 2048, {"act": 2, "bias": True, "residual": True}),   # tiles of 256 features, a warp's own stores
+    (2048, 1 << 20, 2048, {"act": 4}),                                   # ... a group's stores
+    (4096, 1 << 18, 7168, {}),                                           # tiles of up to 512 tokens
+])
+def test_a_linear_layer_whose_limit_ends_in_the_middle(T, K, N, kw):
+    """The limit (looked at every 256 polls, so some hundred microseconds) is shorter than the reduction's milliseconds: the launch reports that, ends, and the next one is right."""
+    from fast_b200 import runtime
+    from fast_b200.ops import gemm
+
+    C = runtime.ext()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, w = (torch.randint(-1, 2, s, generator=g, device="cuda", dtype=torch.int8).to(torch.bfloat16) for s in ((T, K), (N, K)))
+    act = kw.get("act", 0)
+    b = torch.ones(N, device="cuda", dtype=torch.bfloat16) if kw.get("bias") else None
+    r = torch.ones(T, N, device="cuda", dtype=torch.bfloat16) if kw.get("residual") else None
+    want = C.linear(x, w, b, r, act, 5.0)
+    gemm.check()
+    for _ in range(3):
+        C.linear(x, w, b, r, act, 50e-6)
+        with pytest.raises(runtime.CollectiveTimeout):
+            gemm.check()
+        gemm.reset()
+        again = C.linear(x, w, b, r, act, 5.0)
+        gemm.check()
+        assert torch.equal(again, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,K,N", [(1 << 22, 64, 1024), (1 << 19, 1024, 4096)])   # rows shared out, and a tile a pair of CTAs
+def test_a_weight_gradient_whose_limit_ends_in_the_middle(T, K, N):
+    from fast_b200 import runtime
+    from fast_b200.ops import gemm
+
+    C = runtime.ext()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, w = (torch.randint(-1, 2, s, generator=g, device="cuda", dtype=torch.int8).to(torch.bfloat16) for s in ((T, K), (N, K)))
+    w.requires_grad_()
+    dy = torch.ones(T, N, device="cuda", dtype=torch.bfloat16)
+    want = torch.autograd.grad(C.linear(x, w, None, None, 0, 5.0), w, dy)[0]
+    gemm.check()
+    for _ in range(2):
+        y = C.linear(x, w, None, None, 0, 50e-6)
+        gemm.check()
+        torch.autograd.grad(y, w, dy)
+        with pytest.raises(runtime.CollectiveTimeout):
+            gemm.check()
+        gemm.reset()
+        assert torch.equal(torch.autograd.grad(C.linear(x, w, None, None, 0, 5.0), w, dy)[0], want)
+        gemm.check()
