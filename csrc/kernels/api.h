@@ -172,7 +172,7 @@ cudaError_t launch_grouped_gemm_tokens(GemmMode mode, GemmEpilogue epi, const To
 
 // The same for one weight matrix of any size (sizes that are multiples of 8; what a tile has past the end is zeros on its way in and stays
 // unwritten on its way out). num_groups = 1, no group tables. partials and counters (zeroed, num_counters = 0, counters_next null) only where
-// dense_is_cut says so; counters are zero again afterwards.
+// dense_split cuts tiles; counters are zero again afterwards.
 struct TokDenseArgs : TokGemmArgs {
   int dense_rows;            // tokens
   int features;              // columns of the output
@@ -187,7 +187,7 @@ struct TokDenseArgs : TokGemmArgs {
 struct TokDenseMaps : TokGemmMaps {
   const CUtensorMap* c3;     // kLinear with keep_pre: what the activation is taken of, written as bf16
 };
-bool dense_is_cut(const TokDenseArgs& args, int ctas);
+gemm::TokSplit dense_split(const TokDenseArgs& args, int ctas);
 // Forward: kStore (tiles of 512 tokens), kSwiGLU, kLinear (tiles of up to 256; maps.c2: the residual; c, c2 and c3 with boxes {32,32} and the 64-byte
 // swizzle); dgrad: kStore and kLinear, the same.
 cudaError_t launch_dense_gemm(GemmMode mode, GemmEpilogue epi, const TokDenseMaps& maps, const TokDenseArgs& args, int ctas, cudaStream_t stream);

@@ -846,11 +846,6 @@ cudaError_t launch(const TokGemmMaps& m, const Args& args, int ctas, cudaStream_
   return args.tile_n > kTokAccN ? launch_sub<MODE, EPI, 2>(m, nullptr, args, ctas, stream) : launch_sub<MODE, EPI, 1>(m, nullptr, args, ctas, stream);
 }
 
-TokSplit dense_split(const TokDenseArgs& a, int ctas) {
-  const int rows = tok_rows(a, 0);
-  return TokSplit::make(tok_group_tiles(a, 0), a.red_blocks, ctas / 2, tok_tile_size(rows, a.tile_n), tok_tiles(rows, a.tile_n) > 1);
-}
-
 __device__ DeviceStatus g_dense_status;   // one on every device that the library runs on
 
 }  // namespace
@@ -868,7 +863,10 @@ DeviceStatus* dense_status() {
   return at;
 }
 
-bool dense_is_cut(const TokDenseArgs& args, int ctas) { return dense_split(args, ctas).cut_tiles > 0; }
+TokSplit dense_split(const TokDenseArgs& a, int ctas) {
+  const int rows = tok_rows(a, 0);
+  return TokSplit::make(tok_group_tiles(a, 0), a.red_blocks, ctas / 2, tok_tile_size(rows, a.tile_n), tok_tiles(rows, a.tile_n) > 1);
+}
 
 cudaError_t launch_dense_gemm(GemmMode mode, GemmEpilogue epi, const TokDenseMaps& maps, const TokDenseArgs& args, int ctas, cudaStream_t stream) {
   if (ctas < 2 || args.num_groups != 1 || args.dense_rows < 1 || args.features < 1 || args.m_tiles != div_up(args.features, kPairM) || args.red_blocks < 1 || args.band_tiles < 1) return cudaErrorInvalidValue;

@@ -320,28 +320,31 @@ struct DenseEpilogue {
   Activation act = Activation::kNone;
 };
 
+// How the kernel with tiles of 256 features goes about `rows` tokens (more than 64: fewer are always few, see few_pays). plain: nothing but the product.
+TokDenseArgs dense_args(int rows, int64_t features, int64_t reduction, bool plain, int ctas) {
+  TokDenseArgs a{};
+  a.num_groups = 1;
+  a.dense_rows = rows; a.features = static_cast<int>(features);
+  a.m_tiles = static_cast<int>((features + 255) / 256); a.red_blocks = static_cast<int>((reduction + 63) / 64);
+  a.granule = 32;
+  // Where all tokens fit a narrow tile, narrow tiles leave shared memory to the weights in flight.
+  a.tile_n = rows <= 128 ? 128 : gemm::tok_dense_tile(rows, a.m_tiles, a.red_blocks, ctas / 2);
+  // SwiGLU, whose kept gate and up would leave three stages, takes no wide tiles: us on them, without: 300 x 4096 -> 104448 233 to 273, 246; kept 312 to 331, 282 to 294;
+  // 280 x 4096 -> 163840 382 to 387, 358 to 362; kept 439 to 448, 422 to 426.
+  if (plain && a.tile_n == 256 && gemm::tok_wide(false, static_cast<int>(reduction), rows, (rows + 511) / 512 * (features / 256.0) / (ctas / 2))) a.tile_n = 512;
+  a.band_tiles = gemm::tok_band(0, 64 * a.red_blocks, a.m_tiles, a.tile_n);
+  a.back_tiles = gemm::tok_back_tiles(64 * a.red_blocks, a.band_tiles, std::max(a.tile_n, gemm::kTokAccN));
+  return a;
+}
+
 // forward: out [T, N] = epilogue(x [T, K] . weight [N, K]^T); dgrad: out [T, K] = x [T, N] . weight [N, K]. All bf16 rows as tma_rows makes them.
 void dense_gemm(GemmMode mode, const torch::Tensor& weight, const torch::Tensor& x, const torch::Tensor& out, const DenseEpilogue& ep, uint64_t timeout_ns) {
   const bool fwd = mode == GemmMode::kForward;
   const int64_t N = weight.size(0), K = weight.size(1), features = fwd ? N : K, reduction = fwd ? K : N;
   const int ctas = sm_count(x) & ~1;
-  TokDenseArgs a{};
-  a.num_groups = 1;
-  a.dense_rows = static_cast<int>(x.size(0)); a.features = static_cast<int>(features);
-  a.m_tiles = static_cast<int>((features + 255) / 256); a.red_blocks = static_cast<int>((reduction + 63) / 64);
-  a.granule = 32;
-  // Where all tokens fit a narrow tile, narrow tiles leave shared memory to the weights in flight.
-  a.tile_n = a.dense_rows <= 64 ? 64 : a.dense_rows <= 128 ? 128 : gemm::tok_dense_tile(a.dense_rows, a.m_tiles, a.red_blocks, ctas / 2);
-  GemmEpilogue kind = ep.kind;
   const bool plain = ep.kind == GemmEpilogue::kLinear && ep.act == Activation::kNone && !ep.bias && !ep.residual && !ep.pre;
-  // SwiGLU, whose kept gate and up would leave three stages, takes no wide tiles: us on them, without: 300 x 4096 -> 104448 233 to 273, 246; kept 312 to 331, 282 to 294;
-  // 280 x 4096 -> 163840 382 to 387, 358 to 362; kept 439 to 448, 422 to 426.
-  if (plain && a.tile_n == 256 && gemm::tok_wide(false, static_cast<int>(reduction), a.dense_rows, (a.dense_rows + 511) / 512 * (features / 256.0) / (ctas / 2))) {
-    a.tile_n = 512;
-    kind = GemmEpilogue::kStore;
-  }
-  a.band_tiles = gemm::tok_band(0, 64 * a.red_blocks, a.m_tiles, a.tile_n);
-  a.back_tiles = gemm::tok_back_tiles(64 * a.red_blocks, a.band_tiles, std::max(a.tile_n, gemm::kTokAccN));
+  TokDenseArgs a = dense_args(static_cast<int>(x.size(0)), features, reduction, plain, ctas);
+  const GemmEpilogue kind = a.tile_n == 512 ? GemmEpilogue::kStore : ep.kind;
   a.status = dense_status();
   TORCH_CHECK(a.status != nullptr, "linear: no status block on this device");
   a.timeout_ns = timeout_ns;
@@ -368,7 +371,7 @@ void dense_gemm(GemmMode mode, const torch::Tensor& weight, const torch::Tensor&
     if (ep.pre) { c3 = rows_map(*ep.pre, 32, cols); maps.c3 = &c3; a.keep_pre = 1; }
   }
   torch::Tensor partials, counters;
-  if (dense_is_cut(a, ctas)) {
+  if (dense_split(a, ctas).cut_tiles > 0) {
     partials = fresh({tok_partial_floats(ctas, a.tile_n)}, x, torch::kFloat32);
     counters = torch::zeros({tok_counters(ctas)}, x.options().dtype(torch::kInt32));
     a.partials = partials.data_ptr<float>();
@@ -557,5 +560,18 @@ void bind_dense(py::module_& m) {
   m.def("balance_loss", &balance_loss, py::arg("logits"), py::arg("topk_idx"), py::arg("mask"), py::arg("sigmoid"));
   m.def("linear", &linear, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("residual"), py::arg("kind"), py::arg("timeout_s"));
   m.def("dense_status", &dense_block);
+  // Which way a product of a linear layer goes: whether the kernel for few tokens has it, and otherwise the most tokens of a tile, how many tiles are cut along the reduction, into how many
+  // parts or shares, and whether as a stream.
+  m.def("dense_path", [](int tokens, int64_t features, int64_t reduction, bool swiglu, bool plain, bool sectors, int sms) {
+    const int ctas = sms & ~1;
+    const bool few = few_pays(tokens, static_cast<int>(swiglu ? features / 2 : features), static_cast<int>((reduction + 63) / 64), swiglu, sectors, sms);
+    py::dict d;
+    d["few"] = few;
+    if (few) return d;
+    const TokDenseArgs a = dense_args(tokens, features, reduction, plain && !swiglu, ctas);
+    const gemm::TokSplit s = dense_split(a, ctas);
+    d["tile"] = a.tile_n; d["cut_tiles"] = s.cut_tiles; d["shares"] = s.shares; d["stream"] = s.stream;
+    return d;
+  }, py::arg("tokens"), py::arg("features"), py::arg("reduction"), py::arg("swiglu"), py::arg("plain"), py::arg("sectors"), py::arg("sms") = 148);
   m.def("dequantise_rows", &dequantise_rows, py::arg("q"), py::arg("scales"));
 }
