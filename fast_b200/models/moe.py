@@ -311,7 +311,7 @@ class MixtralBlockModel(nn.Module):
     def forward(self, token_ids: torch.Tensor) -> torch.Tensor:
         h = fused.embedding(token_ids.reshape(-1), self.embed)
         loss = self.moe.mean_square_from_residual(h, self.norm_w, self.eps)
-        return loss if self.moe.balance_loss is None else loss + self.balance_coef * self.moe.balance_loss
+        return loss if not self.balance_coef or self.moe.balance_loss is None else loss + self.balance_coef * self.moe.balance_loss
 
 
 @torch.no_grad()

@@ -63,6 +63,19 @@ def test_a_replayed_pass_drops_the_last_balance_loss(monkeypatch):
     assert layer.balance_loss is None and layer.expert_counts is None
 
 
+@pytest.mark.parametrize("coef,want", [(0.5, 6.5), (0.0, 3.0)])
+def test_a_training_pass_adds_the_balance_loss_only_with_a_coefficient(coef, want, monkeypatch):
+    model, layer = _stubbed(monkeypatch)
+    model.balance_coef = coef
+
+    def trained(h, norm_w, eps):
+        layer.balance_loss = torch.tensor(7.0 if coef else float("nan"))
+        return torch.tensor(3.0)
+
+    monkeypatch.setattr(layer, "mean_square_from_residual", trained)
+    assert model(torch.arange(4)).item() == want
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("E,shared", [(8, 0), (8, 128), (64, 0)])
 def test_evaluation_between_training_steps(E, shared):
