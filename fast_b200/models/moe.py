@@ -102,7 +102,7 @@ class _NormRouteMoEFunction(torch.autograd.Function):
             grad_out = torch.zeros_like(h)
         gx, gw, dw13, dw2 = _experts_backward(eng, grad_out, rs, rs.topk_w, w13, w2, ctx.w2_param)
         if grad_hn is not None:
-            gx = gx + grad_hn
+            gx = gx + grad_hn   # in bf16, as autograd adds the gradients of two consumers: the norm's backward kernel takes one such gradient
         grad_h = torch.empty_like(h)
         d_gate, d_nw = torch.empty_like(gate), torch.empty_like(norm_w)
         eng._C.norm_gate_bwd(h, norm_w, gate, rstd, rs.topk_idx, rs.topk_w, gw, gx, grad_h, d_gate, d_nw, None, None if grad_logits is None else grad_logits.contiguous())
