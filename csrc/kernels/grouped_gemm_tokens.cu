@@ -625,9 +625,12 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
           bias[i] = p.bias != nullptr && f < p.features ? __bfloat162float(p.bias[f]) : 0.0f;
         }
         if (sg.parts == 1) wait_acc(0);
-        int st = first_step;
+        auto drain_residual = [&](int st, uint32_t i) {        // of step st, in slot i, where it was requested
+          if (residual && lane == 0 && st < steps_of(0)) mbar_drain(&ctl->epi_load[2 * me + (i & 1u)], (load_ph >> (i & 1u)) & 1u);
+        };
+        if (!ok) { drain_residual(first_step, ring_n); drain_residual(first_step + GROUPS, ring_n + 1); break; }
 #pragma unroll 1
-        for (; ok && st < steps_of(0); st += GROUPS) {
+        for (int st = first_step; st < steps_of(0); st += GROUPS) {
           uint32_t r[32], h[16];
           load_acc(0, st, r);
           if (p.bias != nullptr) {
@@ -640,7 +643,10 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
             for (int e = 0; e < 4; ++e) stmatrix_trans(warp_box_row(box, lane, e & 1, (e >> 1) * 2), h[4 * e], h[4 * e + 1], h[4 * e + 2], h[4 * e + 3]);
           };
           if (residual) {
-            if (!(ok = wait_epi(&ctl->epi_load[2 * me + (ring_n & 1u)], (load_ph >> (ring_n & 1u)) & 1u, 500))) break;
+            if (!(ok = wait_epi(&ctl->epi_load[2 * me + (ring_n & 1u)], (load_ph >> (ring_n & 1u)) & 1u, 500))) {
+              drain_residual(st, ring_n); drain_residual(st + GROUPS, ring_n + 1);
+              break;
+            }
             load_ph ^= 1u << (ring_n & 1u);
           } else {
             if (lane == 0) bulk_wait_read<1>();   // the store that reads this slot is done with it
@@ -686,12 +692,7 @@ grouped_gemm_tokens_kernel(const __grid_constant__ CUtensorMap map_w, const __gr
           }
           ++ring_n;
         }
-        if (!ok) {
-          if (residual && lane == 0)
-            for (int i = 0; i < 2; ++i)
-              if (st + i * GROUPS < steps_of(0)) mbar_drain(&ctl->epi_load[2 * me + ((ring_n + i) & 1u)], (load_ph >> ((ring_n + i) & 1u)) & 1u);
-          break;
-        }
+        if (!ok) break;
         if (sg.parts == 1) release_acc(0);
       } else if constexpr (SUB == 1) {
         if (EPI == GemmEpilogue::kSwiGLUBwd) begin_gu(0);       // the saved tiles arrive while the MMAs still run

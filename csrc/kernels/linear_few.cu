@@ -137,8 +137,8 @@ __global__ void __launch_bounds__(kThreads) linear_few_kernel(const __grid_const
         mma_commit(&ctl->empty[s]);
         if (++s == stages) { s = 0; ph ^= 1; }
       }
-      mma_commit(ok ? &ctl->done : &ctl->products);
-      if (!ok) mbar_drain(&ctl->products, 0);
+      if (ok) mma_commit(&ctl->done);
+      else { mma_commit(&ctl->products); mbar_drain(&ctl->products, 0); }
     }
   }
   __syncwarp();
@@ -222,8 +222,8 @@ __global__ void __launch_bounds__(kThreads) linear_few_kernel(const __grid_const
     }
   }
   __syncwarp();
-  // Given up: not before the products and the loads that are still on their way.
-  if (*abort_flag && warp == 1) {
+  // Given up: not before the products and the loads that are still on their way. (A warp that saw the products done saw the loads done too.)
+  if (!ok && warp == 1) {
     if (lane == 0) { mbar_drain(&ctl->done, 0); drain_loads(ctl->full, ctl->issued, stages); }
     __syncwarp();
   }

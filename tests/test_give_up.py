@@ -124,8 +124,9 @@ def test_a_kernel_that_gives_up_waits_for_what_is_under_way():
     for f in ("grouped_gemm.cu", "grouped_gemm_pair.cu", "grouped_gemm_tokens.cu", "linear_few.cu"):
         text = _source(f)
         end = text[text.index("__syncwarp();\n  const bool ok = mbar_wait_warp") if f == "linear_few.cu" else text.rindex("tc_fence_before_sync();\n  __syncthreads();"):]
-        assert "*abort_flag" in end and ("drain_loads(ctl->full" in end or "mbar_drain(&ctl->full" in end), f
-        assert end.index("*abort_flag") < end.index("tmem_dealloc"), f
+        told = "if (!ok && warp == 1)" if f == "linear_few.cu" else "*abort_flag)"
+        drained = "mbar_drain(&ctl->full" if f == "grouped_gemm_tokens.cu" else "drain_loads(ctl->full"
+        assert end.index(told) < end.index(drained) < end.rindex("tmem_dealloc"), f
         assert re.search(r"mma_commit(_pair)?\((ok \? &ctl->done : )?&ctl->products", text) and "mbar_drain(&ctl->products, 0)" in text, f
     assert "mbar_drain(&ctl->epi_load" in _source("grouped_gemm_tokens.cu")
 
