@@ -136,10 +136,10 @@ def test_a_kernel_that_gives_up_waits_for_what_is_under_way():
     (1, 1 << 24, 128, {}), (300, 1 << 22, 256, {"bias": True}),         # few tokens: one tile for a cluster of CTAs, and several
     (2048, 1 << 20, 2048, {"act": 2, "bias": True, "residual": True}),   # tiles of 256 features, a warp's own stores
     (2048, 1 << 20, 2048, {"act": 4}),                                   # ... a group's stores
-    (4096, 1 << 18, 7168, {}),                                           # tiles of up to 512 tokens
+    (4096, 1 << 19, 7168, {}),                                           # tiles of up to 512 tokens
 ])
 def test_a_linear_layer_whose_limit_ends_in_the_middle(T, K, N, kw):
-    """The limit (looked at every 256 polls, so some hundred microseconds) is shorter than the reduction's milliseconds: the launch reports that, ends, and the next one is right."""
+    """The limit (looked at every 256 polls: about every millisecond) is shorter than the reduction of a tile, 5 ms and more: the launch reports that, ends, and the next one is right."""
     from fast_b200 import runtime
     from fast_b200.ops import gemm
 
@@ -162,7 +162,7 @@ def test_a_linear_layer_whose_limit_ends_in_the_middle(T, K, N, kw):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("T,K,N", [(1 << 22, 64, 1024), (1 << 19, 1024, 4096)])   # rows shared out, and a tile a pair of CTAs
+@pytest.mark.parametrize("T,K,N", [(1 << 23, 64, 1024), (1 << 20, 1024, 4096)])   # rows shared out, and a tile a pair of CTAs
 def test_a_weight_gradient_whose_limit_ends_in_the_middle(T, K, N):
     from fast_b200 import runtime
     from fast_b200.ops import gemm
